@@ -200,7 +200,8 @@ int b200attn_paged_decode(void* out, int64_t out_row_stride,
  * Prefill over an fp8 paged cache is not implemented (fresh-K/V prefill needs no cache). */
 enum b200attn_cache_dtype {
   B200ATTN_CACHE_BF16 = 0,
-  B200ATTN_CACHE_FP8_E4M3 = 1
+  B200ATTN_CACHE_FP8_E4M3 = 1,
+  B200ATTN_CACHE_INT8 = 2          /* block-scaled caches only (b200attn_paged_write) */
 };
 
 int b200attn_paged_update_cache_ex(void* k_cache, void* v_cache,
@@ -317,6 +318,146 @@ int b200attn_decode_auto_splits(int num_users, int num_kv_heads, int head_size,
  * the ticket region, the fp32 partial outputs and their (max, sum) pairs. */
 size_t b200attn_decode_workspace_bytes(int num_users, int num_q_heads, int head_size,
                                        int num_splits);
+
+/* ------------------------------------------------------------------------------------------
+ * Norms of queries and keys for each head and the rotary embedding in one pass, fused with the
+ * slot-mapping KV-cache write.
+ * No counterpart in the reference's attention path (a model with per-head norms issues them as
+ * separate ops before layers/rotary_embedding.py:51-66); it stands beside
+ * b200attn_rope_kv_scatter_slots.
+ *     x' = x * rsqrt(mean(x^2) + eps) * weight      per head; q_weight / k_weight [head_size]
+ * then the first rotary_dim elements of each head are rotated by positions[t] * inv_freq[i]: pairs
+ * (i, i + rotary_dim / 2) when is_neox_style, (2 i, 2 i + 1) otherwise (rotary_dim a multiple of
+ * 16, <= head_size).  Computed in fp32 (the angle in fp64) and rounded to bf16 once, unlike
+ * b200attn_rope_kv_scatter_slots, which rounds after every operation as the reference layer does.
+ * q_out / k_out may be q / k themselves (same pointer and stride) or memory that overlaps neither
+ * q, k nor v.  weight_f32: the weights are fp32, else bf16.  With slot_mapping the rounded k_out
+ * rows and v go to the caches (cache_dtype bf16 or unscaled e4m3) as b200attn_kv_scatter_slots_ex
+ * writes them; of tokens with the same slot one, unspecified, wins.  slot_mapping == NULL: v and
+ * the caches are not touched and may be NULL.
+ * ------------------------------------------------------------------------------------------ */
+int b200attn_qk_norm_rope_kv_scatter_slots(
+    void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, const void* q,
+    int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+    const void* q_weight, const void* k_weight, int weight_f32, float eps,
+    const int64_t* positions, const float* inv_freq, int rotary_dim, int is_neox_style,
+    void* k_cache, void* v_cache, int cache_dtype, const int64_t* slot_mapping, int num_tokens,
+    int num_q_heads, int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
+    void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Varlen KV-cache write that keeps per-page values: the scales of a block-scaled 8-bit cache and
+ * the key bounds b200attn_select_pages reads.
+ * No counterpart in the reference (its cache write casts without scales, attention.py:692-700).
+ * Tokens cu_q[s] .. cu_q[s+1]-1 of k_new / v_new (row t at t * k_token_stride resp.
+ * v_token_stride, head h at h * head_size) go to positions q_start[s], q_start[s] + 1, ... of
+ * sequence s, through page_table[s, position / block_size].  cu_q == NULL: one token per
+ * sequence (total_tokens == num_seqs).  q_len, when given, limits how many of a sequence's tokens
+ * are written (padded batches).  q_start[s] < 0: nothing is written for s.  total_tokens is the
+ * number of rows and must be at least cu_q[num_seqs].
+ *   cache_dtype BF16: rows as they are; scales must be NULL (use it for its k_bounds).
+ *   cache_dtype INT8 or FP8_E4M3: k_scale / v_scale are fp32 [num_blocks, num_kv_heads]; an element
+ *     reads as code * scale.  A page whose first row is written starts afresh with scale =
+ *     max|x| * (1 / qmax) over its new rows (qmax 127 or 448); a page that goes on keeps its scale while
+ *     that is enough and else grows it by the smallest power of two that is, re-rounding the rows
+ *     that stay (rows before the first new one; later rows are dead).  A NaN or infinity makes the
+ *     scale NaN until the page starts afresh: everything read through it is NaN.
+ *   k_bounds: NULL, or bf16 [num_blocks, num_kv_heads, 2, head_size]: least ([.., 0, :]) and
+ *     greatest key per channel of a page, started afresh and merged like the scales.
+ * The sequences of a call must write to different pages, or the values of a shared page are
+ * unspecified.  Page ids and columns out of range are skipped and reported (diagnostics word 2).
+ * ------------------------------------------------------------------------------------------ */
+int b200attn_paged_write(void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                         void* k_bounds, int cache_dtype, const void* k_new,
+                         int64_t k_token_stride, const void* v_new, int64_t v_token_stride,
+                         const int32_t* page_table, int64_t page_table_stride,
+                         int page_table_width, const int32_t* cu_q, const int32_t* q_len,
+                         const int32_t* q_start, int num_seqs, int total_tokens,
+                         int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
+                         void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Paged GQA decode attention over block-scaled 8-bit caches and / or over a page list per KV head.
+ * No counterpart in the reference; b200attn_paged_decode_ex in every other respect (splits,
+ * workspace, sinks, NaN in masked rows).
+ *   k_scale / v_scale: both NULL (caches bf16, or unscaled e4m3 with head_size 128), or fp32
+ *     [num_blocks, num_kv_heads] of caches written by b200attn_paged_write (cache_dtype INT8 or
+ *     FP8_E4M3, head_size 64 or 128).  Codes are widened exactly; q (scaled by a power of two per
+ *     head) and the softmax weights are rounded to f16, sums are fp32.  NaN scales give NaN rows.
+ *   page_table_head_stride > 0: page_table is [num_users, num_kv_heads, width] with that stride
+ *     between heads, cur_pos is [num_users, num_kv_heads] and counts within the list: the keys
+ *     of the list's pages 0 .. cur_pos / block_size are attended, the last page up to
+ *     cur_pos % block_size (what b200attn_select_pages writes).  No sliding window then.
+ * b200attn_decode_blocks_auto_splits: the split count num_splits = 0 picks for scaled caches. */
+int b200attn_paged_decode_blocks(void* out, int64_t out_row_stride, const void* q,
+                                 int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                 const float* k_scale, const float* v_scale, int cache_dtype,
+                                 const int32_t* page_table, int64_t page_table_stride,
+                                 int64_t page_table_head_stride, int page_table_width,
+                                 const int32_t* cur_pos, int num_users, int num_q_heads,
+                                 int num_kv_heads, int head_size, int block_size,
+                                 int64_t num_blocks, float scale, int sliding_window,
+                                 const float* sinks, int max_context_len, int num_splits,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+int b200attn_decode_blocks_auto_splits(int num_users, int num_kv_heads, int head_size,
+                                       int max_context_len);
+
+/* ------------------------------------------------------------------------------------------
+ * Page selection for block-sparse decode attention.
+ * No counterpart in the reference.  For every user u and KV head h, n = the pages of the context
+ * cur_pos[u] + 1 (at most page_table_width):
+ *     score[p] = max over the head's queries of sum_d min(q_d, 0) kmin[p, d] + max(q_d, 0) kmax[p, d]
+ * with the bounds of page page_table[u, p] (b200attn_paged_write).  If n <= num_pages all pages are
+ * taken, else the first keep_first, the last keep_last (>= 1) and, of the others, those of the
+ * greatest scores; equal scores go to the lower page and a score that is NaN ranks first.  The
+ * choice is that of exact scores (fp32 scores near the border are summed again in fp64).
+ *   out_table [num_users, num_kv_heads, num_pages]: the page ids in context order, 0 behind them;
+ *   out_pos   [num_users, num_kv_heads]: position of the newest key within that list, -1 for a
+ *     user without context (cur_pos < 0).
+ * Both are what b200attn_paged_decode_blocks takes.  num_q_heads / num_kv_heads <= 16.
+ * max_context_len (0: unknown) only shapes the launch.  Workspace:
+ * b200attn_select_pages_workspace_bytes bytes whose first B200ATTN_DECODE_TICKET_BYTES follow the
+ * contract of b200attn_paged_decode's (zero at first use, left zero); the two calls may share a
+ * workspace in stream order.  At most B200ATTN_DECODE_TICKET_BYTES / 4 (user, KV head) pairs.
+ * ------------------------------------------------------------------------------------------ */
+size_t b200attn_select_pages_workspace_bytes(int num_users, int num_kv_heads,
+                                             int page_table_width);
+int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
+                          int64_t q_row_stride, const void* k_bounds, const int32_t* page_table,
+                          int64_t page_table_stride, int page_table_width, const int32_t* cur_pos,
+                          int num_users, int num_q_heads, int num_kv_heads, int head_size,
+                          int block_size, int64_t num_blocks, int num_pages, int keep_first,
+                          int keep_last, int max_context_len, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Chunked prefill over a block-scaled cache, in the two steps of the fp8 form below: widen the
+ * pages the batch reads, then attend over the pool through the identity page table.
+ * k_dst / v_dst: num_seqs * page_table_width pages of [num_kv_heads, block_size, head_size] bf16,
+ * which get code * 2^e (exact); factors: fp32 pairs [num_seqs * page_table_width, num_kv_heads, 2],
+ * what is left of the scales: scale = factor * 2^e with the factor in [1, 2), the K factor itself
+ * and the base-2 logarithm of the V factor.  b200attn_prefill_scaled is b200attn_prefill_ex
+ * (kv_is_paged = 1) over that pool; it applies the factors in fp32, so the 8-bit values reach the
+ * attention unrounded.  Rows that attend a page with a NaN scale come out as NaN. */
+int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, const void* k_cache,
+                                  const void* v_cache, const float* k_scale, const float* v_scale,
+                                  int cache_dtype, const int32_t* page_table,
+                                  int64_t page_table_stride, int page_table_width,
+                                  const int32_t* cu_q, const int32_t* q_start, int num_seqs,
+                                  int num_kv_heads, int head_size, int block_size,
+                                  int64_t num_blocks, void* stream);
+int b200attn_prefill_scaled(void* out, int64_t out_row_stride, const void* q,
+                            int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                            const float* factors, const int32_t* page_table,
+                            int64_t page_table_stride, int page_table_width, const int32_t* cu_q,
+                            const int32_t* cu_q_host, const int32_t* q_start, int num_seqs,
+                            int total_q, int num_q_heads, int num_kv_heads, int head_size,
+                            int block_size, int64_t num_blocks, float scale, int sliding_window,
+                            void* stream);
+
+/* *id_out (host) = the identity of the stream capture `stream` is part of, 0 when it is not being
+ * captured: lets a host keep one workspace per captured graph. */
+int b200attn_capture_id(uint64_t* id_out, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Chunked prefill over an fp8 (e4m3) cache, step 1: widen the pages the batch reads.

@@ -80,6 +80,44 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int,
          c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_int, c_int, c_void_p],
     ),
+    "b200attn_qk_norm_rope_kv_scatter_slots": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+         c_int64, c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_int, c_int, c_void_p,
+         c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p],
+    ),
+    "b200attn_paged_write": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p,
+         c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+         c_int, c_int, c_int64, c_void_p],
+    ),
+    "b200attn_paged_decode_blocks": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+         c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64,
+         c_float, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    "b200attn_decode_blocks_auto_splits": (c_int, [c_int, c_int, c_int, c_int]),
+    "b200attn_select_pages_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "b200attn_select_pages": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+         c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "b200attn_dequant_pages_scaled": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+         c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_void_p],
+    ),
+    "b200attn_prefill_scaled": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int64,
+         c_float, c_int, c_void_p],
+    ),
+    "b200attn_capture_id": (c_int, [c_void_p, c_void_p]),
     "b200attn_decode_auto_splits": (c_int, [c_int, c_int, c_int, c_int]),
     "b200attn_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b200attn_prefill": (

@@ -23,11 +23,13 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 _retired_workspaces: list[torch.Tensor] = []
 
 
-CACHE_BF16, CACHE_FP8_E4M3 = 0, 1     # enum b200attn_cache_dtype
+CACHE_BF16, CACHE_FP8_E4M3, CACHE_INT8 = 0, 1, 2     # enum b200attn_cache_dtype
 TICKET_BYTES = 65536                  # B200ATTN_DECODE_TICKET_BYTES
 
 
 def _cache_dtype(cache: torch.Tensor) -> int:
+    if cache.dtype == torch.int8:
+        return CACHE_INT8
     return CACHE_FP8_E4M3 if cache.dtype == torch.float8_e4m3fn else CACHE_BF16
 
 
@@ -57,13 +59,18 @@ def _need_cuda(*tensors: torch.Tensor) -> None:
             )
 
 
-def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 scaled: bool = False) -> tuple[int, int, int, int]:
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(
             "k_cache and v_cache must both be [num_blocks, num_kv_heads, block_size, head_size]; "
             f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}"
         )
-    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+    if scaled:
+        if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (torch.int8, torch.float8_e4m3fn):
+            raise ValueError("block-scaled caches must both be int8 or both be float8_e4m3fn")
+    elif k_cache.dtype != v_cache.dtype or k_cache.dtype not in (torch.bfloat16,
+                                                                 torch.float8_e4m3fn):
         raise ValueError("caches must both be bfloat16 or both be float8_e4m3fn")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
@@ -85,6 +92,49 @@ def _i32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise ValueError(f"{name} must be int32, got {t.dtype}")
     return t
+
+
+def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors must be on {first.device}, got one on {t.device}")
+
+
+class _on_device:
+    """Makes a tensor's device current for a call into the library (which works on the current
+    device); free of charge when it already is."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+        self.previous = -1
+
+    def __enter__(self):
+        current = torch.cuda.current_device()
+        if current != self.index:
+            self.previous = current
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.previous >= 0:
+            torch.cuda.set_device(self.previous)
+        return False
+
+
+def _check_scales(k_scale, v_scale, k_cache: torch.Tensor) -> bool:
+    """True when the caches are block-scaled; the scales are dense fp32 [num_blocks, num_kv_heads]."""
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("k_scale and v_scale go together")
+    if k_scale is None:
+        return False
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32 or tuple(t.shape) != tuple(k_cache.shape[:2]) \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be a dense float32 tensor [num_blocks, num_kv_heads]")
+    _need_cuda(k_scale, v_scale)
+    _one_device(k_cache, k_scale, v_scale)
+    return True
 
 
 def paged_update_cache(
@@ -255,6 +305,202 @@ def rope_kv_scatter_slots(
     )
 
 
+def _spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory between the first and the last element of two 2-D row tensors meets."""
+    def span(t):
+        lo = t.data_ptr()
+        return lo, lo + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def qk_norm_rope_kv_scatter_slots(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: Optional[torch.Tensor],
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    rotary_dim: int,
+    head_size: int,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    eps: float = 1e-6,
+    k_cache: Optional[torch.Tensor] = None,
+    v_cache: Optional[torch.Tensor] = None,
+    slot_mapping: Optional[torch.Tensor] = None,
+    is_neox_style: bool = True,
+    out_query: Optional[torch.Tensor] = None,
+    out_key: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head (`q_weight` / `k_weight` [head_size], bf16 or fp32,
+    shared by the heads), then the rotary embedding, then, with `slot_mapping`, the cache write of
+    the rotated key and of `value`: `rope_kv_scatter_slots` with the per-head norms in front, in one
+    pass.  Computed in fp32 (angles in fp64) and rounded to bf16 once.  `query` [tokens, nq*hd],
+    `key` / `value` [tokens, nkv*hd], dense rows of any row stride; results go to `out_query` /
+    `out_key` of the same shapes, or in place when these are not given.  An output either is its
+    input or overlaps none of the inputs.  Pairs are (i, i + rotary_dim/2) for `is_neox_style`,
+    (2i, 2i + 1) otherwise.  Caches: bf16 or unscaled e4m3 (`paged_write` fills block-scaled
+    ones).  Returns (out_query, out_key)."""
+    _need_cuda(query, key, value, positions, inv_freq, q_weight, k_weight, k_cache, v_cache,
+               slot_mapping, out_query, out_key)
+    _one_device(query, key, value, positions, inv_freq, q_weight, k_weight, k_cache, v_cache,
+                slot_mapping, out_query, out_key)
+    tokens = positions.numel()
+    if query.dim() != 2 or key.dim() != 2 or query.shape[0] != tokens or key.shape[0] != tokens:
+        raise ValueError("query / key must be [tokens, heads*head_size] with one row per position")
+    if query.shape[1] % head_size or key.shape[1] % head_size:
+        raise ValueError("query / key rows must hold whole heads")
+    outs = []
+    for name, x, out in (("query", query, out_query), ("key", key, out_key)):
+        out = x if out is None else out
+        if out.shape != x.shape:
+            raise ValueError(f"out_{name} must have {name}'s shape")
+        for t in (x, out):
+            if t.dtype != torch.bfloat16 or t.stride(1) != 1:
+                raise ValueError(f"{name} must be bfloat16 with dense rows")
+        outs.append(out)
+    for i, out in enumerate(outs):
+        own_input = (query, key)[i]
+        if out.data_ptr() != own_input.data_ptr() or (tokens > 1 and
+                                                      out.stride(0) != own_input.stride(0)):
+            for x in (query, key, value):
+                if x is not None and x.dim() == 2 and _spans_overlap(out, x):
+                    raise ValueError("an output must be its input or overlap none of the inputs")
+            if _spans_overlap(out, outs[1 - i]):
+                raise ValueError("the outputs must not overlap")
+    nq, nkv = query.shape[1] // head_size, key.shape[1] // head_size
+    if positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise ValueError("positions must be a dense int64 tensor")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2 \
+            or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be dense float32 [rotary_dim / 2]")
+    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("q_weight / k_weight must both be bfloat16 or both be float32")
+    for w in (q_weight, k_weight):
+        if w.numel() != head_size or not w.is_contiguous():
+            raise ValueError("q_weight / k_weight must be dense [head_size]")
+    nb = bs = 0
+    if slot_mapping is not None:
+        if k_cache is None or v_cache is None or value is None:
+            raise ValueError("slot_mapping needs k_cache, v_cache and value")
+        nb, nkv_c, bs, hd_c = _check_cache(k_cache, v_cache)
+        if nkv_c != nkv or hd_c != head_size:
+            raise ValueError("cache geometry differs from key geometry")
+        if value.shape != key.shape or value.dtype != torch.bfloat16 or value.stride(1) != 1:
+            raise ValueError("value must match key")
+        if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < tokens \
+                or not slot_mapping.is_contiguous():
+            raise ValueError("slot_mapping must be dense int64 with one entry per token")
+    if tokens == 0:
+        return outs[0], outs[1]
+
+    def stride(t):
+        return t.stride(0) if tokens > 1 else t.shape[1]
+
+    write = slot_mapping is not None
+    with _on_device(query):
+        _lib.check(
+            "b200attn_qk_norm_rope_kv_scatter_slots",
+            _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
+                outs[0].data_ptr(), stride(outs[0]), outs[1].data_ptr(), stride(outs[1]),
+                query.data_ptr(), stride(query), key.data_ptr(), stride(key),
+                value.data_ptr() if write else None, stride(value) if write else 0,
+                q_weight.data_ptr(), k_weight.data_ptr(),
+                1 if q_weight.dtype == torch.float32 else 0, float(eps), positions.data_ptr(),
+                inv_freq.data_ptr(), rotary_dim, 1 if is_neox_style else 0,
+                k_cache.data_ptr() if write else None, v_cache.data_ptr() if write else None,
+                _cache_dtype(k_cache) if write else CACHE_BF16,
+                slot_mapping.data_ptr() if write else None, tokens, nq, nkv, head_size, bs, nb,
+                _stream(query),
+            ),
+        )
+    return outs[0], outs[1]
+
+
+def _rows_3d(x: torch.Tensor, nheads: int, hd: int, name: str) -> tuple[torch.Tensor, int]:
+    """[tokens, nheads, hd] view of bf16 rows with dense heads, and the row stride."""
+    if x.dim() == 2 and x.shape[1] == nheads * hd:
+        x = x.unflatten(1, (nheads, hd))
+    if x.dim() != 3 or tuple(x.shape[1:]) != (nheads, hd):
+        raise ValueError(f"{name} must be [tokens, {nheads}, {hd}], got {tuple(x.shape)}")
+    return _token_major(x, nheads, hd, name)
+
+
+def paged_write(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    page_table: torch.Tensor,
+    q_start: torch.Tensor,
+    cu_q: Optional[torch.Tensor] = None,
+    q_len: Optional[torch.Tensor] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    k_bounds: Optional[torch.Tensor] = None,
+) -> None:
+    """Varlen KV write that keeps per-page values.  Rows `cu_q[s]:cu_q[s+1]` of `key` / `value`
+    ([tokens, nkv, hd] bf16) go to positions `q_start[s]`, `q_start[s] + 1`, ... of sequence s
+    through `page_table[s]`; without `cu_q` every sequence has one token.  `q_len` limits how many of
+    a sequence's rows are written (padded batches); a negative `q_start` skips the sequence.
+
+    Caches: int8 or float8_e4m3fn with `k_scale` / `v_scale` (fp32 [num_blocks, num_kv_heads], an
+    element reads as code * scale), or bf16 without scales (`k_bounds` is then what the call is
+    for).  A page whose first row is written starts afresh; one that goes on grows its scale by a
+    power of two when a new row needs it and re-rounds the rows that stay.  A NaN or infinity makes
+    the scale NaN, and with it everything read through the page.  `k_bounds` (bf16 [num_blocks,
+    num_kv_heads, 2, head_size]) keeps the least and greatest key of each channel for
+    `select_pages`.  The sequences of one call must write to different pages."""
+    _need_cuda(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len, k_scale, v_scale,
+               k_bounds)
+    _one_device(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len, k_bounds)
+    scaled = _check_scales(k_scale, v_scale, k_cache)
+    nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
+    if not scaled and k_cache.dtype != torch.bfloat16:
+        raise ValueError("an 8-bit cache needs k_scale and v_scale here (kv_scatter_slots writes "
+                         "unscaled e4m3)")
+    if not scaled and k_bounds is None:
+        raise ValueError("a bf16 cache without k_bounds is kv_scatter_slots's")
+    if k_bounds is not None and (k_bounds.dtype != torch.bfloat16 or not k_bounds.is_contiguous()
+                                 or tuple(k_bounds.shape) != (nb, nkv, 2, hd)):
+        raise ValueError("k_bounds must be dense bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
+    key, kstride = _rows_3d(key, nkv, hd, "key")
+    value, vstride = _rows_3d(value, nkv, hd, "value")
+    if key.shape != value.shape:
+        raise ValueError("key and value must have the same shape")
+    _i32(page_table, "page_table")
+    _i32(q_start, "q_start")
+    seqs = q_start.numel()
+    if page_table.dim() != 2 or page_table.shape[0] < seqs or page_table.stride(1) != 1 \
+            or not q_start.is_contiguous():
+        raise ValueError("page_table needs a dense row, and q_start a dense entry, per sequence")
+    if cu_q is None:
+        if key.shape[0] != seqs:
+            raise ValueError("without cu_q, key / value must hold one row per sequence")
+    elif _i32(cu_q, "cu_q").numel() != seqs + 1 or not cu_q.is_contiguous():
+        raise ValueError("cu_q must hold num_seqs + 1 dense entries")
+    if q_len is not None and (_i32(q_len, "q_len").numel() != seqs or not q_len.is_contiguous()):
+        raise ValueError("q_len must hold one dense entry per sequence")
+    if seqs == 0 or key.shape[0] == 0:
+        return
+    with _on_device(k_cache):
+        _lib.check(
+            "b200attn_paged_write",
+            _lib.lib().b200attn_paged_write(
+                k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if scaled else None,
+                v_scale.data_ptr() if scaled else None,
+                k_bounds.data_ptr() if k_bounds is not None else None, _cache_dtype(k_cache),
+                key.data_ptr(), kstride, value.data_ptr(), vstride, page_table.data_ptr(),
+                page_table.stride(0), page_table.shape[1],
+                cu_q.data_ptr() if cu_q is not None else None,
+                q_len.data_ptr() if q_len is not None else None, q_start.data_ptr(), seqs,
+                key.shape[0], nkv, hd, bs, nb, _stream(k_cache),
+            ),
+        )
+
+
 def decode_auto_splits(users: int, nkv: int, hd: int, max_context_len: int) -> int:
     return _lib.lib().b200attn_decode_auto_splits(users, nkv, hd, max_context_len)
 
@@ -279,6 +525,141 @@ def _workspace(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
     return ws
 
 
+_capture_workspaces: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
+
+
+def _scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
+    """Scratch of the block-scaled and page-list ops, `device` current.  Eager calls take the
+    per-stream workspace.  Calls under stream capture take one that belongs to the graph being
+    captured (from its memory pool, its counters zeroed by a node of the graph), so that graphs
+    captured on the same stream may be replayed side by side on others."""
+    if nbytes == 0 or not torch.cuda.is_current_stream_capturing():
+        return _workspace(device, nbytes)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    capture = ctypes.c_uint64(0)
+    _lib.check("b200attn_capture_id",
+               _lib.lib().b200attn_capture_id(ctypes.byref(capture), stream))
+    key = (device.index or 0, stream)
+    have = _capture_workspaces.get(key)
+    if have is None or have[0] != capture.value or have[1].numel() < nbytes:
+        ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        ws[:TICKET_BYTES].zero_()
+        have = (capture.value, ws)
+        _capture_workspaces[key] = have
+    return have[1]
+
+
+def select_pages(
+    query: torch.Tensor,
+    k_bounds: torch.Tensor,
+    page_table: torch.Tensor,
+    cur_pos: torch.Tensor,
+    block_size: int,
+    num_pages: int,
+    keep_first: int = 1,
+    keep_last: int = 1,
+    max_context_len: int = 0,
+    workspace: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Chooses, for every user and KV head, the `num_pages` pages of the context a block-sparse
+    decode attends to: all of them when there are no more, else the first `keep_first`, the last
+    `keep_last` (>= 1) and those whose key bounds allow the largest logit of any of the head's
+    queries (equal scores: the lower page).  `query` [users, nq, hd]; `k_bounds` as `paged_write`
+    keeps them; `page_table` [users, width] and `cur_pos` [users] as for `paged_decode`.
+    Returns (table [users, nkv, num_pages], pos [users, nkv]): hand them to `paged_decode` as
+    `page_table` and `cur_pos`.  `max_context_len` only shapes the launch."""
+    _need_cuda(query, k_bounds, page_table, cur_pos)
+    _one_device(query, k_bounds, page_table, cur_pos, workspace)
+    if k_bounds.dim() != 4 or k_bounds.shape[2] != 2 or k_bounds.dtype != torch.bfloat16 \
+            or not k_bounds.is_contiguous():
+        raise ValueError("k_bounds must be dense bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
+    nb, nkv, _, hd = k_bounds.shape
+    if query.dim() == 4 and query.shape[0] == 1:
+        query = query[0]
+    if query.dim() != 3 or query.shape[2] != hd:
+        raise ValueError(f"query must be [users, nq, {hd}], got {tuple(query.shape)}")
+    users, nq = query.shape[0], query.shape[1]
+    if nq % nkv != 0:
+        raise ValueError(f"num_q_heads {nq} is not a multiple of num_kv_heads {nkv}")
+    q, qstride = _token_major(query, nq, hd, "query")
+    _i32(page_table, "page_table")
+    _i32(cur_pos, "cur_pos")
+    if page_table.dim() != 2 or page_table.shape[0] < users or page_table.stride(1) != 1 \
+            or not cur_pos.is_contiguous() or cur_pos.numel() != users:
+        raise ValueError("page_table needs a dense row, and cur_pos a dense entry, per user")
+    if keep_first < 0 or keep_last < 1 or keep_first + keep_last > num_pages:
+        raise ValueError("keep_first >= 0 and keep_last >= 1 must fit into num_pages")
+    table = torch.empty((users, nkv, num_pages), dtype=torch.int32, device=query.device)
+    pos = torch.empty((users, nkv), dtype=torch.int32, device=query.device)
+    if users == 0:
+        return table, pos
+    L = _lib.lib()
+    width = page_table.shape[1]
+    with _on_device(query):
+        ws = workspace
+        if ws is None:
+            ws = _scratch(query.device, L.b200attn_select_pages_workspace_bytes(users, nkv, width))
+        _lib.check(
+            "b200attn_select_pages",
+            L.b200attn_select_pages(
+                table.data_ptr(), pos.data_ptr(), q.data_ptr(), qstride, k_bounds.data_ptr(),
+                page_table.data_ptr(), page_table.stride(0), width, cur_pos.data_ptr(), users, nq,
+                nkv, hd, block_size, nb, num_pages, keep_first, keep_last, max_context_len,
+                ws.data_ptr() if ws is not None else None,
+                ws.numel() * ws.element_size() if ws is not None else 0, _stream(query),
+            ),
+        )
+    return table, pos
+
+
+def _decode_blocks(q, qstride, out_t, ostride, k_cache, v_cache, k_scale, v_scale, page_table,
+                   cur_pos, scale, num_splits, max_context_len, workspace, sliding_window, sinks,
+                   geometry) -> None:
+    """paged_decode over block-scaled caches and / or a page list per KV head."""
+    users, nq, nb, nkv, bs, hd = geometry
+    _one_device(q, out_t, k_cache, v_cache, page_table, cur_pos, sinks, workspace)
+    head_stride = 0
+    if page_table.dim() == 3:
+        if tuple(page_table.shape[:2]) != (users, nkv) or page_table.stride(2) != 1:
+            raise ValueError("a page list per KV head must be dense [users, num_kv_heads, pages]")
+        if tuple(cur_pos.shape) != (users, nkv):
+            raise ValueError("with a page list per KV head cur_pos must be [users, num_kv_heads]")
+        if sliding_window > 0:
+            raise ValueError("a list of chosen pages has no sliding window")
+        head_stride = page_table.stride(1)
+        if head_stride < page_table.shape[2]:
+            raise ValueError("the page lists of the KV heads must not overlap")
+    elif page_table.dim() != 2 or page_table.shape[0] < users or cur_pos.numel() != users:
+        raise ValueError("page_table needs a row, and cur_pos an entry, per user")
+    width = page_table.shape[-1]
+    L = _lib.lib()
+    with _on_device(q):
+        if num_splits == 0:
+            ctx = max_context_len if max_context_len > 0 else width * bs
+            if head_stride:
+                ctx = min(ctx, width * bs)
+            if sliding_window > 0:
+                ctx = min(ctx, sliding_window + 64)
+            pick = L.b200attn_decode_blocks_auto_splits if k_scale is not None \
+                else L.b200attn_decode_auto_splits
+            num_splits = pick(users, nkv, hd, ctx)
+        need = L.b200attn_decode_workspace_bytes(users, nq, hd, num_splits)
+        ws = workspace if workspace is not None else _scratch(q.device, need)
+        _lib.check(
+            "b200attn_paged_decode_blocks",
+            L.b200attn_paged_decode_blocks(
+                out_t.data_ptr(), ostride, q.data_ptr(), qstride, k_cache.data_ptr(),
+                v_cache.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                v_scale.data_ptr() if v_scale is not None else None, _cache_dtype(k_cache),
+                page_table.data_ptr(), page_table.stride(0), head_stride, width,
+                cur_pos.data_ptr(), users, nq, nkv, hd, bs, nb, float(scale), int(sliding_window),
+                sinks.data_ptr() if sinks is not None else None, max_context_len, num_splits,
+                ws.data_ptr() if ws is not None else None,
+                ws.numel() * ws.element_size() if ws is not None else 0, _stream(q),
+            ),
+        )
+
+
 def paged_decode(
     query: torch.Tensor,
     k_cache: torch.Tensor,
@@ -295,6 +676,8 @@ def paged_decode(
     new_key: Optional[torch.Tensor] = None,
     new_value: Optional[torch.Tensor] = None,
     wrap_negative_positions: bool = True,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Paged GQA decode attention: `tt.paged_scaled_dot_product_attention_decode` with
     is_causal=True and cur_pos_tensor (custom_ops.py:1198-1331).  `query`: [users, nq, hd]
@@ -305,9 +688,14 @@ def paged_decode(
     With `new_key` / `new_value` ([users, nkv, hd] bf16) the same launch first writes those rows
     into the caches at `cur_pos`, i.e. it is `paged_update_cache` + decode in one kernel;
     `wrap_negative_positions=False` skips rows with a negative position instead of wrapping them
-    the way the reference's CPU indexing does."""
+    the way the reference's CPU indexing does.
+    `k_scale` / `v_scale` (fp32 [num_blocks, num_kv_heads]): int8 or e4m3 caches with a scale per
+    page and KV head, as `paged_write` fills them.  A `page_table` [users, nkv, pages] with a
+    `cur_pos` [users, nkv] gives every KV head its own list of pages, `cur_pos` counting within the
+    list: what `select_pages` returns (no `sliding_window` then).  Neither form takes `new_key`."""
     _need_cuda(query, k_cache, v_cache, page_table, cur_pos, out, new_key, new_value)
-    nb, nkv, bs, hd = _check_cache(k_cache, v_cache)
+    scaled = _check_scales(k_scale, v_scale, k_cache)
+    nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
     orig_shape = query.shape
     if query.dim() == 4:
         if query.shape[0] != 1:
@@ -330,7 +718,9 @@ def paged_decode(
     ostride = out_t.stride(0) if users > 1 else max(out_t.stride(0), nq * hd)
     _i32(page_table, "page_table")
     _i32(cur_pos, "cur_pos")
-    if page_table.stride(1) != 1 or not cur_pos.is_contiguous() or cur_pos.numel() != users:
+    blocks = scaled or page_table.dim() == 3
+    if not cur_pos.is_contiguous() or page_table.stride(-1) != 1 or (not blocks and
+                                                                    cur_pos.numel() != users):
         raise ValueError("page_table rows must be dense and cur_pos must hold one entry per user")
     if scale is None:
         scale = hd ** -0.5
@@ -341,6 +731,16 @@ def paged_decode(
             raise ValueError("sinks must be a dense float32 tensor with one entry per q head")
     if num_splits == 0:
         num_splits = _env_num_splits()
+    if blocks:
+        if new_key is not None or new_value is not None:
+            raise ValueError("new_key / new_value go with unscaled caches and one page list per "
+                             "user; use paged_write first")
+        if users:
+            _decode_blocks(q, qstride if users > 1 else max(qstride, nq * hd), out_t, ostride,
+                           k_cache, v_cache, k_scale, v_scale, page_table, cur_pos, scale,
+                           num_splits, max_context_len, workspace, sliding_window, sinks,
+                           (users, nq, nb, nkv, bs, hd))
+        return out if out is not None else out_t.reshape(orig_shape)
     if num_splits == 0:
         ctx = max_context_len if max_context_len > 0 else page_table.shape[1] * bs
         if sliding_window > 0:
@@ -389,13 +789,17 @@ def prefill(
     out: Optional[torch.Tensor] = None,
     cu_q: Optional[torch.Tensor] = None,
     sliding_window: int = 0,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Causal varlen prefill (`tt.scaled_dot_product_attention`, custom_ops.py:635-742) when
     `page_table` is None and `k_src`/`v_src` are the fresh [tokens, nkv, hd] K/V of the same
     tokens; chunked prefill over the paged cache
     (`tt.chunked_scaled_dot_product_attention`, custom_ops.py:1334-1443) when `page_table` is
     given and `k_src`/`v_src` are the caches.  `query`: [tokens, nq, hd] with sequence s owning
-    rows cu_q[s]:cu_q[s+1]; `q_start[s]` is the absolute position of its first row."""
+    rows cu_q[s]:cu_q[s+1]; `q_start[s]` is the absolute position of its first row.
+    `k_scale` / `v_scale`: paged int8 or e4m3 caches with a scale per page and KV head
+    (`paged_write`)."""
     _need_cuda(query, k_src, v_src, page_table, q_start, out, cu_q)
     if cu_q_host.is_cuda or cu_q_host.dtype != torch.int32 or not cu_q_host.is_contiguous():
         raise ValueError("cu_q_host must be a dense int32 CPU tensor")
@@ -405,8 +809,12 @@ def prefill(
     total_q, nq, hd = query.shape
     q, qstride = _token_major(query, nq, hd, "query")
     paged = page_table is not None
+    scaled = False
+    if not paged and (k_scale is not None or v_scale is not None):
+        raise ValueError("k_scale / v_scale go with a paged cache")
     if paged:
-        nb, nkv, bs, _hd = _check_cache(k_src, v_src)
+        scaled = _check_scales(k_scale, v_scale, k_src)
+        nb, nkv, bs, _hd = _check_cache(k_src, v_src, scaled)
         if _hd != hd:
             raise ValueError("cache head_size differs from query head_size")
         _i32(page_table, "page_table")
@@ -437,7 +845,11 @@ def prefill(
     if cu_q is None:
         cu_q = cu_q_host.to(query.device, non_blocking=True)
     _i32(cu_q, "cu_q")
-    if paged and k_src.dtype == torch.float8_e4m3fn:
+    if scaled:
+        _one_device(query, k_src, v_src, page_table, q_start, cu_q, out)
+        k, v, factors, page_table, nb = _widen_scaled_pages(k_src, v_src, k_scale, v_scale,
+                                                            page_table, cu_q, q_start, num_seqs)
+    elif paged and k_src.dtype == torch.float8_e4m3fn:
         # The tcgen05 kernel takes 16-bit tiles: widen the pages this batch reads into a bf16
         # scratch pool laid out [sequence][page slot] and attend over that through the identity
         # page table.  e4m3 -> bf16 is exact, so the kernel sees the cache's own values.
@@ -454,6 +866,20 @@ def prefill(
     if scale is None:
         scale = hd ** -0.5
     L = _lib.lib()
+    if scaled:
+        with _on_device(query):
+            _lib.check(
+                "b200attn_prefill_scaled",
+                L.b200attn_prefill_scaled(
+                    out_t.data_ptr(), ostride, q.data_ptr(),
+                    qstride if total_q > 1 else max(qstride, nq * hd), k.data_ptr(), v.data_ptr(),
+                    factors.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+                    page_table.shape[1], cu_q.data_ptr(), cu_q_host.data_ptr(),
+                    q_start.data_ptr() if q_start is not None else None, num_seqs, total_q, nq,
+                    nkv, hd, bs, nb, float(scale), int(sliding_window), _stream(query),
+                ),
+            )
+        return out if out is not None else out_t
     _lib.check(
         "b200attn_prefill_ex",
         L.b200attn_prefill_ex(
@@ -505,6 +931,48 @@ def _widen_fp8_pages(k_cache, v_cache, page_table, cu_q, q_start, num_seqs):
         ),
     )
     return k_pool, v_pool, ident, k_pool.shape[0]
+
+
+_scaled_scratch: dict[tuple, tuple] = {}
+
+
+def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_start, num_seqs):
+    """_widen_fp8_pages for a block-scaled cache pair: (k_pool, v_pool, the pages' factors, identity
+    page table, pool size).  Under stream capture the pool belongs to the graph being captured."""
+    nb, nkv, bs, hd = k_cache.shape
+    width = page_table.shape[1]
+    pages = max(num_seqs * width, 1)
+    dev = k_cache.device
+    with _on_device(k_cache):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        capturing = torch.cuda.is_current_stream_capturing()
+        key = (dev.index or 0, stream, nkv, bs, hd)
+        have = None if capturing else _scaled_scratch.get(key)
+        if have is None or have[0].shape[0] < pages:
+            grow = pages
+            if have is not None:
+                grow = max(pages, 2 * have[0].shape[0])
+            have = (torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
+                    torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
+                    torch.empty((grow, nkv, 2), dtype=torch.float32, device=dev), {})
+            if not capturing:
+                _scaled_scratch[key] = have
+        k_pool, v_pool, factors, tables = have
+        ident = tables.get((num_seqs, width))
+        if ident is None:
+            ident = torch.arange(num_seqs * width, dtype=torch.int32, device=dev)
+            ident = tables[(num_seqs, width)] = ident.reshape(num_seqs, width)
+        _lib.check(
+            "b200attn_dequant_pages_scaled",
+            _lib.lib().b200attn_dequant_pages_scaled(
+                k_pool.data_ptr(), v_pool.data_ptr(), factors.data_ptr(), k_cache.data_ptr(),
+                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _cache_dtype(k_cache),
+                page_table.data_ptr(), page_table.stride(0), width, cu_q.data_ptr(),
+                q_start.data_ptr() if q_start is not None else None, num_seqs, nkv, hd, bs, nb,
+                stream,
+            ),
+        )
+    return k_pool, v_pool, factors, ident, k_pool.shape[0]
 
 
 def read_error_word(device: Optional[torch.device] = None) -> int:

@@ -12,10 +12,14 @@
 
 #include "decode.cuh"
 #include "decode_fp8.cuh"
+#include "decode_scaled.cuh"
 #include "kv_scatter.cuh"
+#include "paged_write.cuh"
 #include "prefill.cuh"
+#include "qk_norm_rope.cuh"
 #include "rope_scatter.cuh"
 #include "rowlinear_ar.cuh"
+#include "select_pages.cuh"
 #include "step_metadata.cuh"
 
 namespace b200attn {
@@ -284,11 +288,73 @@ static int launch_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, const
   return static_cast<int>(e);
 }
 
-template <int HD, int BS, bool WIN>
+template <int HD, int BS, int FMT, int NG>
+static int launch_decode_scaled(const CUtensorMap& tk, const CUtensorMap& tv,
+                                const DecodeScaledParams& p, int num_users, cudaStream_t s) {
+  constexpr int kStages = 6;
+  using L = DecodeScaledSmem<HD, BS, kStages>;
+  auto kern = paged_decode_scaled_kernel<HD, BS, FMT, NG, kStages>;
+  static bool smem_allowed[kMaxDevices] = {};
+  cudaError_t e = allow_dynamic_smem(kern, L::kTotalBytes, smem_allowed);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  dim3 grid(p.d.num_splits, p.d.num_kv_heads, num_users);
+  kern<<<grid, kDecThreads, L::kTotalBytes, s>>>(tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (p.d.num_splits > 1 && !p.d.tickets) {
+    dim3 cgrid(p.d.num_q_heads, num_users);
+    decode_combine_kernel<HD><<<cgrid, HD, 0, s>>>(p.d);
+    e = cudaGetLastError();
+  }
+  return static_cast<int>(e);
+}
+
+// query heads per KV head: one MMA column group up to 8, two up to 16
+template <int HD, int BS, int FMT>
+static int launch_decode_scaled_ng(const CUtensorMap& tk, const CUtensorMap& tv,
+                                   const DecodeScaledParams& p, int num_users, cudaStream_t s) {
+  return p.d.group <= 8 ? launch_decode_scaled<HD, BS, FMT, 1>(tk, tv, p, num_users, s)
+                        : launch_decode_scaled<HD, BS, FMT, 2>(tk, tv, p, num_users, s);
+}
+
+template <int HD, int BS>
+static int launch_decode_scaled_fmt(int fmt, const CUtensorMap& tk, const CUtensorMap& tv,
+                                    const DecodeScaledParams& p, int num_users, cudaStream_t s) {
+  return fmt == kPageInt8 ? launch_decode_scaled_ng<HD, BS, kPageInt8>(tk, tv, p, num_users, s)
+                          : launch_decode_scaled_ng<HD, BS, kPageE4m3>(tk, tv, p, num_users, s);
+}
+
+template <int HD, int BS>
+static void launch_paged_write(int fmt, dim3 grid, const PagedWriteParams& p, cudaStream_t s) {
+  if (fmt == kPageInt8)
+    paged_write_kernel<HD, BS, kPageInt8><<<grid, kPwThreads, 0, s>>>(p);
+  else if (fmt == kPageE4m3)
+    paged_write_kernel<HD, BS, kPageE4m3><<<grid, kPwThreads, 0, s>>>(p);
+  else
+    paged_write_kernel<HD, BS, kPageBf16><<<grid, kPwThreads, 0, s>>>(p);
+}
+
+template <int HD, int BS>
+static void launch_dequant_scaled(int fmt, dim3 grid, const DequantScaledParams& p, cudaStream_t s) {
+  if (fmt == kPageInt8)
+    dequant_scaled_kernel<HD, BS, kPageInt8><<<grid, 128, 0, s>>>(p);
+  else
+    dequant_scaled_kernel<HD, BS, kPageE4m3><<<grid, 128, 0, s>>>(p);
+}
+
+template <int HD, int BS>
+static void launch_select_pages(int group, dim3 grid, const SelectPagesParams& p, cudaStream_t s) {
+  if (group <= 8)
+    select_pages_kernel<HD, BS, 1><<<grid, kSelThreads, 0, s>>>(p);
+  else
+    select_pages_kernel<HD, BS, 2><<<grid, kSelThreads, 0, s>>>(p);
+}
+
+template <int HD, int BS, bool WIN, bool SCALED>
 static int launch_prefill_win(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const PrefillParams& p, int sm_count, cudaStream_t s) {
   using L = PrefillSmem<HD>;
-  auto kern = prefill_tcgen05_kernel<HD, BS, WIN>;
+  auto kern = prefill_tcgen05_kernel<HD, BS, WIN, SCALED>;
   static bool smem_allowed[kMaxDevices] = {};
   cudaError_t e = allow_dynamic_smem(kern, L::kTotalBytes, smem_allowed);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -298,13 +364,16 @@ static int launch_prefill_win(const CUtensorMap& tq, const CUtensorMap& tk, cons
   return static_cast<int>(cudaGetLastError());
 }
 
-// The sliding-window variant is a separate instantiation, so full causal attention carries none
-// of its masking or bookkeeping.
+// The sliding-window and the block-scaled variants are separate instantiations, so plain causal
+// attention carries none of their masking or bookkeeping.
 template <int HD, int BS>
 static int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                           const PrefillParams& p, int sm_count, cudaStream_t s) {
-  return p.window > 0 ? launch_prefill_win<HD, BS, true>(tq, tk, tv, p, sm_count, s)
-                      : launch_prefill_win<HD, BS, false>(tq, tk, tv, p, sm_count, s);
+  if (p.page_factors)
+    return p.window > 0 ? launch_prefill_win<HD, BS, true, true>(tq, tk, tv, p, sm_count, s)
+                        : launch_prefill_win<HD, BS, false, true>(tq, tk, tv, p, sm_count, s);
+  return p.window > 0 ? launch_prefill_win<HD, BS, true, false>(tq, tk, tv, p, sm_count, s)
+                      : launch_prefill_win<HD, BS, false, false>(tq, tk, tv, p, sm_count, s);
 }
 
 template <int NB, int S, int W>
@@ -687,17 +756,19 @@ int b200attn_paged_decode_ex(void* out, int64_t out_row_stride, const void* q,
                                     workspace_bytes, stream);
 }
 
-int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
-                               int64_t q_row_stride, void* k_cache, void* v_cache,
-                               const void* k_new, const void* v_new, int64_t new_token_stride,
-                               int wrap_negative_positions, const int32_t* page_table,
-                               int64_t page_table_stride, int page_table_width,
-                               const int32_t* cur_pos, int num_users, int num_q_heads,
-                               int num_kv_heads, int head_size, int block_size,
-                               int64_t num_blocks, float scale, int sliding_window,
-                               const float* sinks, int cache_dtype, int max_context_len,
-                               int num_splits, void* workspace, size_t workspace_bytes,
-                               void* stream) {
+// What paged_decode_step and paged_decode_blocks share.  k_scale / v_scale: the caches are 8-bit
+// with a scale per page and KV head; per_head: page_table and cur_pos have a row per KV head.
+static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                      void* k_cache, void* v_cache, const float* k_scale, const float* v_scale,
+                      const void* k_new, const void* v_new, int64_t new_token_stride,
+                      int wrap_negative_positions, const int32_t* page_table,
+                      int64_t page_table_stride, int64_t page_table_head_stride, int per_head,
+                      int page_table_width, const int32_t* cur_pos, int num_users,
+                      int num_q_heads, int num_kv_heads, int head_size, int block_size,
+                      int64_t num_blocks, float scale, int sliding_window, const float* sinks,
+                      int cache_dtype, int max_context_len, int num_splits, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const bool scaled = k_scale != nullptr;
   if ((k_new == nullptr) != (v_new == nullptr)) return B200ATTN_ERR_NULL_POINTER;
   if (k_new) {
     if (!aligned16(k_new) || !aligned16(v_new) || new_token_stride % 8 != 0)
@@ -706,10 +777,10 @@ int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
       return B200ATTN_ERR_BAD_ARGUMENT;
   }
   if (sliding_window < 0 || !(scale > 0.f)) return B200ATTN_ERR_BAD_ARGUMENT;
-  if (cache_dtype != B200ATTN_CACHE_BF16 && cache_dtype != B200ATTN_CACHE_FP8_E4M3)
-    return B200ATTN_ERR_BAD_ARGUMENT;
   const bool fp8 = cache_dtype == B200ATTN_CACHE_FP8_E4M3;
-  if (fp8 && head_size != 128) return B200ATTN_ERR_UNSUPPORTED;
+  if (scaled ? !fp8 && cache_dtype != B200ATTN_CACHE_INT8 : !fp8 && cache_dtype != B200ATTN_CACHE_BF16)
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  if (fp8 && !scaled && head_size != 128) return B200ATTN_ERR_UNSUPPORTED;
   if (!out || !q || !k_cache || !v_cache || !page_table || !cur_pos)
     return B200ATTN_ERR_NULL_POINTER;
   if (num_users < 0 || num_q_heads <= 0 || page_table_width <= 0 || num_splits < 0)
@@ -734,14 +805,21 @@ int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
   if (sliding_window > 0 && max_context_len > sliding_window + kDecTile)
     max_context_len = sliding_window + kDecTile;       // what a user streams at most
   if (num_splits == 0)
-    num_splits = b200attn_decode_auto_splits(num_users, num_kv_heads, head_size, max_context_len);
+    num_splits = scaled ? b200attn_decode_blocks_auto_splits(num_users, num_kv_heads, head_size,
+                                                             max_context_len)
+                        : b200attn_decode_auto_splits(num_users, num_kv_heads, head_size,
+                                                      max_context_len);
   const size_t need = b200attn_decode_workspace_bytes(num_users, num_q_heads, head_size, num_splits);
   if (num_splits > 1 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return B200ATTN_ERR_WORKSPACE;
 
   CUtensorMap tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * num_kv_heads * block_size;
-  if (fp8) {
+  if (scaled) {    // rows of 128 bytes: one token of head size 128, two of head size 64
+    const uint32_t box = static_cast<uint32_t>(block_size * head_size / 128);
+    if (int rc = make_map_u8(&tk, k_cache, rows * head_size / 128, box)) return rc;
+    if (int rc = make_map_u8(&tv, v_cache, rows * head_size / 128, box)) return rc;
+  } else if (fp8) {
     if (int rc = make_map_u8(&tk, k_cache, rows, block_size)) return rc;
     if (int rc = make_map_u8(&tv, v_cache, rows, block_size)) return rc;
   } else {
@@ -774,6 +852,9 @@ int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
   p.cache_fp8 = fp8 ? 1 : 0;
   p.wrap_negative = wrap_negative_positions ? 1 : 0;
   p.err_word = dev->err_word;
+  p.per_head = per_head;
+  p.page_table_head_stride = page_table_head_stride;
+  p.keep_nan = scaled ? 1 : 0;
   if (num_splits > 1) {
     const size_t rows_p = static_cast<size_t>(num_users) * num_q_heads * num_splits;
     size_t o_bytes = rows_p * head_size * sizeof(float);
@@ -788,6 +869,15 @@ int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
     p.part_ml = reinterpret_cast<float2*>(ws + kDecTicketBytes + o_bytes);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (scaled) {
+    const DecodeScaledParams sp{p, k_scale, v_scale};
+    const int fmt = fp8 ? kPageE4m3 : kPageInt8;
+    if (head_size == 128)
+      return block_size == 64 ? launch_decode_scaled_fmt<128, 64>(fmt, tk, tv, sp, num_users, s)
+                              : launch_decode_scaled_fmt<128, 32>(fmt, tk, tv, sp, num_users, s);
+    return block_size == 64 ? launch_decode_scaled_fmt<64, 64>(fmt, tk, tv, sp, num_users, s)
+                            : launch_decode_scaled_fmt<64, 32>(fmt, tk, tv, sp, num_users, s);
+  }
   if (fp8)
     return block_size == 64 ? launch_decode_fp8<64, 6>(tk, tv, p, num_users, s)
                             : launch_decode_fp8<32, 6>(tk, tv, p, num_users, s);
@@ -795,6 +885,332 @@ int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
   if (head_size == 128 && block_size == 32) return launch_decode<128, 32, 3>(tk, tv, p, num_users, s);
   if (head_size == 64 && block_size == 64) return launch_decode<64, 64, 4>(tk, tv, p, num_users, s);
   return launch_decode<64, 32, 4>(tk, tv, p, num_users, s);
+}
+
+int b200attn_paged_decode_step(void* out, int64_t out_row_stride, const void* q,
+                               int64_t q_row_stride, void* k_cache, void* v_cache,
+                               const void* k_new, const void* v_new, int64_t new_token_stride,
+                               int wrap_negative_positions, const int32_t* page_table,
+                               int64_t page_table_stride, int page_table_width,
+                               const int32_t* cur_pos, int num_users, int num_q_heads,
+                               int num_kv_heads, int head_size, int block_size,
+                               int64_t num_blocks, float scale, int sliding_window,
+                               const float* sinks, int cache_dtype, int max_context_len,
+                               int num_splits, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  return decode_any(out, out_row_stride, q, q_row_stride, k_cache, v_cache, nullptr, nullptr, k_new,
+                    v_new, new_token_stride, wrap_negative_positions, page_table,
+                    page_table_stride, 0, 0, page_table_width, cur_pos, num_users, num_q_heads,
+                    num_kv_heads, head_size, block_size, num_blocks, scale, sliding_window, sinks,
+                    cache_dtype, max_context_len, num_splits, workspace, workspace_bytes, stream);
+}
+
+int b200attn_paged_decode_blocks(void* out, int64_t out_row_stride, const void* q,
+                                 int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                 const float* k_scale, const float* v_scale, int cache_dtype,
+                                 const int32_t* page_table, int64_t page_table_stride,
+                                 int64_t page_table_head_stride, int page_table_width,
+                                 const int32_t* cur_pos, int num_users, int num_q_heads,
+                                 int num_kv_heads, int head_size, int block_size,
+                                 int64_t num_blocks, float scale, int sliding_window,
+                                 const float* sinks, int max_context_len, int num_splits,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  if ((k_scale == nullptr) != (v_scale == nullptr)) return B200ATTN_ERR_NULL_POINTER;
+  if (page_table_head_stride < 0 || page_table_stride < 0) return B200ATTN_ERR_BAD_ARGUMENT;
+  // a list of chosen pages has no positions a window could be taken of
+  if (page_table_head_stride > 0 && sliding_window > 0) return B200ATTN_ERR_UNSUPPORTED;
+  return decode_any(out, out_row_stride, q, q_row_stride, const_cast<void*>(k_cache),
+                    const_cast<void*>(v_cache), k_scale, v_scale, nullptr, nullptr, 0, 1,
+                    page_table, page_table_stride, page_table_head_stride,
+                    page_table_head_stride > 0 ? 1 : 0, page_table_width, cur_pos, num_users,
+                    num_q_heads, num_kv_heads, head_size, block_size, num_blocks, scale,
+                    sliding_window, sinks, cache_dtype, max_context_len, num_splits, workspace,
+                    workspace_bytes, stream);
+}
+
+int b200attn_decode_blocks_auto_splits(int num_users, int num_kv_heads, int head_size,
+                                       int max_context_len) {
+  return b200attn_decode_auto_splits(num_users, num_kv_heads, head_size, max_context_len);
+}
+
+// ------------------------------------------------------- norms + rotation, block-scaled writes
+int b200attn_qk_norm_rope_kv_scatter_slots(
+    void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, const void* q,
+    int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+    const void* q_weight, const void* k_weight, int weight_f32, float eps,
+    const int64_t* positions, const float* inv_freq, int rotary_dim, int is_neox_style,
+    void* k_cache, void* v_cache, int cache_dtype, const int64_t* slot_mapping, int num_tokens,
+    int num_q_heads, int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
+    void* stream) {
+  if (!q_out || !k_out || !q || !k || !q_weight || !k_weight || !positions || !inv_freq)
+    return B200ATTN_ERR_NULL_POINTER;
+  if (slot_mapping && (!v || !k_cache || !v_cache)) return B200ATTN_ERR_NULL_POINTER;
+  if (num_tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || !(eps >= 0.f))
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  if (head_size != 64 && head_size != 128) return B200ATTN_ERR_UNSUPPORTED;
+  if (rotary_dim <= 0 || rotary_dim > head_size || rotary_dim % 16 != 0)
+    return B200ATTN_ERR_UNSUPPORTED;
+  if (slot_mapping) {
+    if (cache_dtype != B200ATTN_CACHE_BF16 && cache_dtype != B200ATTN_CACHE_FP8_E4M3)
+      return B200ATTN_ERR_BAD_ARGUMENT;
+    if (int rc = check_cache_geometry(num_kv_heads, head_size, block_size, num_blocks)) return rc;
+    if (!aligned16(v) || v_stride % 8 || !aligned16(k_cache) || !aligned16(v_cache))
+      return B200ATTN_ERR_MISALIGNED;
+    if (v_stride < static_cast<int64_t>(num_kv_heads) * head_size) return B200ATTN_ERR_BAD_ARGUMENT;
+  }
+  if (!aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) ||
+      !aligned16(q_weight) || !aligned16(k_weight) || q_stride % 8 || k_stride % 8 ||
+      q_out_stride % 8 || k_out_stride % 8)
+    return B200ATTN_ERR_MISALIGNED;
+  const int64_t q_row = static_cast<int64_t>(num_q_heads) * head_size;
+  const int64_t k_row = static_cast<int64_t>(num_kv_heads) * head_size;
+  if (q_stride < q_row || q_out_stride < q_row || k_stride < k_row || k_out_stride < k_row)
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  DeviceInfo* dev;
+  if (int rc = get_device(&dev)) return rc;
+  if (num_tokens == 0) return B200ATTN_OK;
+  QkNormRopeParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_stride;
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.k_stride = k_stride;
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.v_stride = v_stride;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.q_out_stride = q_out_stride;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.k_out_stride = k_out_stride;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.weight_f32 = weight_f32 ? 1 : 0;
+  p.eps = eps;
+  p.positions = positions;
+  p.inv_freq = inv_freq;
+  p.rotary_dim = rotary_dim;
+  p.neox = is_neox_style ? 1 : 0;
+  p.k_cache = static_cast<uint8_t*>(k_cache);
+  p.v_cache = static_cast<uint8_t*>(v_cache);
+  p.cache_fp8 = cache_dtype == B200ATTN_CACHE_FP8_E4M3 ? 1 : 0;
+  p.slot_mapping = slot_mapping;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  p.err_word = dev->err_word;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (head_size == 128)
+    qk_norm_rope_kernel<128><<<static_cast<unsigned>(num_tokens), kNrThreads, 0, s>>>(p);
+  else
+    qk_norm_rope_kernel<64><<<static_cast<unsigned>(num_tokens), kNrThreads, 0, s>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int b200attn_paged_write(void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                         void* k_bounds, int cache_dtype, const void* k_new,
+                         int64_t k_token_stride, const void* v_new, int64_t v_token_stride,
+                         const int32_t* page_table, int64_t page_table_stride,
+                         int page_table_width, const int32_t* cu_q, const int32_t* q_len,
+                         const int32_t* q_start, int num_seqs, int total_tokens,
+                         int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
+                         void* stream) {
+  if (!k_cache || !v_cache || !k_new || !v_new || !page_table || !q_start)
+    return B200ATTN_ERR_NULL_POINTER;
+  if (num_seqs < 0 || total_tokens < 0 || page_table_width <= 0) return B200ATTN_ERR_BAD_ARGUMENT;
+  if (!cu_q && total_tokens != num_seqs) return B200ATTN_ERR_BAD_ARGUMENT;
+  int fmt;
+  if (cache_dtype == B200ATTN_CACHE_BF16) {
+    if (k_scale || v_scale) return B200ATTN_ERR_BAD_ARGUMENT;
+    fmt = kPageBf16;
+  } else if (cache_dtype == B200ATTN_CACHE_FP8_E4M3 || cache_dtype == B200ATTN_CACHE_INT8) {
+    if (!k_scale || !v_scale) return B200ATTN_ERR_NULL_POINTER;
+    fmt = cache_dtype == B200ATTN_CACHE_INT8 ? kPageInt8 : kPageE4m3;
+  } else {
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  }
+  if (int rc = check_cache_geometry(num_kv_heads, head_size, block_size, num_blocks)) return rc;
+  if (num_kv_heads > 65535) return B200ATTN_ERR_TOO_LARGE;
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * head_size;
+  if (k_token_stride < row || v_token_stride < row) return B200ATTN_ERR_BAD_ARGUMENT;
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_new) || !aligned16(v_new) ||
+      (k_bounds && !aligned16(k_bounds)) || k_token_stride % 8 || v_token_stride % 8)
+    return B200ATTN_ERR_MISALIGNED;
+  DeviceInfo* dev;
+  if (int rc = get_device(&dev)) return rc;
+  if (num_seqs == 0 || total_tokens == 0) return B200ATTN_OK;
+  PagedWriteParams p{};
+  p.cache[0] = static_cast<uint8_t*>(k_cache);
+  p.cache[1] = static_cast<uint8_t*>(v_cache);
+  p.src[0] = static_cast<const __nv_bfloat16*>(k_new);
+  p.src[1] = static_cast<const __nv_bfloat16*>(v_new);
+  p.src_stride[0] = k_token_stride;
+  p.src_stride[1] = v_token_stride;
+  p.scale[0] = k_scale;
+  p.scale[1] = v_scale;
+  p.bounds = static_cast<__nv_bfloat16*>(k_bounds);
+  p.page_table = page_table;
+  p.page_table_stride = page_table_stride;
+  p.page_table_width = page_table_width;
+  p.cu_q = cu_q;
+  p.q_len = q_len;
+  p.q_start = q_start;
+  p.num_seqs = num_seqs;
+  p.total_tokens = total_tokens;
+  p.num_kv_heads = num_kv_heads;
+  p.num_blocks = num_blocks;
+  p.err_word = dev->err_word;
+  // every page of every sequence has an item (see write_item_base)
+  const int64_t items = cu_q ? total_tokens / block_size + 2 * static_cast<int64_t>(num_seqs)
+                             : num_seqs;
+  if (items > 0x7fffffffLL) return B200ATTN_ERR_TOO_LARGE;
+  const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(num_kv_heads), 2);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (head_size == 128 && block_size == 64) launch_paged_write<128, 64>(fmt, grid, p, s);
+  else if (head_size == 128) launch_paged_write<128, 32>(fmt, grid, p, s);
+  else if (block_size == 64) launch_paged_write<64, 64>(fmt, grid, p, s);
+  else launch_paged_write<64, 32>(fmt, grid, p, s);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, const void* k_cache,
+                                  const void* v_cache, const float* k_scale, const float* v_scale,
+                                  int cache_dtype, const int32_t* page_table,
+                                  int64_t page_table_stride, int page_table_width,
+                                  const int32_t* cu_q, const int32_t* q_start, int num_seqs,
+                                  int num_kv_heads, int head_size, int block_size,
+                                  int64_t num_blocks, void* stream) {
+  if (!k_dst || !v_dst || !factors || !k_cache || !v_cache || !k_scale || !v_scale ||
+      !page_table || !cu_q)
+    return B200ATTN_ERR_NULL_POINTER;
+  if (num_seqs < 0 || page_table_width <= 0) return B200ATTN_ERR_BAD_ARGUMENT;
+  if (cache_dtype != B200ATTN_CACHE_FP8_E4M3 && cache_dtype != B200ATTN_CACHE_INT8)
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  if (int rc = check_cache_geometry(num_kv_heads, head_size, block_size, num_blocks)) return rc;
+  if (!aligned16(k_dst) || !aligned16(v_dst) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      !aligned16(factors))
+    return B200ATTN_ERR_MISALIGNED;
+  if (static_cast<int64_t>(num_seqs) * page_table_width * num_kv_heads * block_size > 0x7fffffffLL)
+    return B200ATTN_ERR_TOO_LARGE;
+  if (num_seqs > 65535) return B200ATTN_ERR_TOO_LARGE;
+  DeviceInfo* dev;
+  if (int rc = get_device(&dev)) return rc;
+  if (num_seqs == 0) return B200ATTN_OK;
+  DequantScaledParams p{};
+  p.src[0] = static_cast<const uint8_t*>(k_cache);
+  p.src[1] = static_cast<const uint8_t*>(v_cache);
+  p.dst[0] = static_cast<__nv_bfloat16*>(k_dst);
+  p.dst[1] = static_cast<__nv_bfloat16*>(v_dst);
+  p.scale[0] = k_scale;
+  p.scale[1] = v_scale;
+  p.factors = reinterpret_cast<float2*>(factors);
+  p.page_table = page_table;
+  p.page_table_stride = page_table_stride;
+  p.page_table_width = page_table_width;
+  p.cu_q = cu_q;
+  p.q_start = q_start;
+  p.num_kv_heads = num_kv_heads;
+  p.num_blocks = num_blocks;
+  p.err_word = dev->err_word;
+  const int fmt = cache_dtype == B200ATTN_CACHE_INT8 ? kPageInt8 : kPageE4m3;
+  const dim3 grid(static_cast<unsigned>(page_table_width) * num_kv_heads,
+                  static_cast<unsigned>(num_seqs), 2);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (head_size == 128 && block_size == 64) launch_dequant_scaled<128, 64>(fmt, grid, p, s);
+  else if (head_size == 128) launch_dequant_scaled<128, 32>(fmt, grid, p, s);
+  else if (block_size == 64) launch_dequant_scaled<64, 64>(fmt, grid, p, s);
+  else launch_dequant_scaled<64, 32>(fmt, grid, p, s);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// ------------------------------------------------------------------------- page selection
+size_t b200attn_select_pages_workspace_bytes(int num_users, int num_kv_heads,
+                                             int page_table_width) {
+  if (num_users <= 0 || num_kv_heads <= 0 || page_table_width <= 0) return 0;
+  const size_t rows = static_cast<size_t>(num_users) * num_kv_heads * page_table_width;
+  return kDecTicketBytes + rows * (sizeof(float2) + sizeof(unsigned long long));
+}
+
+int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
+                          int64_t q_row_stride, const void* k_bounds, const int32_t* page_table,
+                          int64_t page_table_stride, int page_table_width, const int32_t* cur_pos,
+                          int num_users, int num_q_heads, int num_kv_heads, int head_size,
+                          int block_size, int64_t num_blocks, int num_pages, int keep_first,
+                          int keep_last, int max_context_len, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  if (!out_table || !out_pos || !q || !k_bounds || !page_table || !cur_pos)
+    return B200ATTN_ERR_NULL_POINTER;
+  if (num_users < 0 || num_q_heads <= 0 || page_table_width <= 0 || keep_first < 0 ||
+      keep_last < 1 || num_pages < 1 ||
+      static_cast<int64_t>(keep_first) + keep_last > num_pages)
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  if (int rc = check_cache_geometry(num_kv_heads, head_size, block_size, num_blocks)) return rc;
+  if (num_q_heads % num_kv_heads != 0) return B200ATTN_ERR_BAD_ARGUMENT;
+  const int group = num_q_heads / num_kv_heads;
+  if (group > 16) return B200ATTN_ERR_UNSUPPORTED;
+  if (!aligned16(q) || !aligned16(k_bounds) || q_row_stride % 8 != 0)
+    return B200ATTN_ERR_MISALIGNED;
+  if (q_row_stride < static_cast<int64_t>(num_q_heads) * head_size)
+    return B200ATTN_ERR_BAD_ARGUMENT;
+  // the positions within a list, and a context, are 32-bit
+  if (static_cast<int64_t>(num_pages) * block_size > 0x7fffffffLL ||
+      static_cast<int64_t>(page_table_width) * block_size > 0x7fffffffLL)
+    return B200ATTN_ERR_TOO_LARGE;
+  DeviceInfo* dev;
+  if (int rc = get_device(&dev)) return rc;
+  if (num_users == 0) return B200ATTN_OK;
+  if (num_users > 65535 || num_kv_heads > 65535 ||
+      static_cast<size_t>(num_users) * num_kv_heads * sizeof(unsigned int) > kDecTicketBytes)
+    return B200ATTN_ERR_TOO_LARGE;
+  if (!workspace || !aligned16(workspace) ||
+      workspace_bytes < b200attn_select_pages_workspace_bytes(num_users, num_kv_heads, page_table_width))
+    return B200ATTN_ERR_WORKSPACE;
+  SelectPagesParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_row_stride = q_row_stride;
+  p.bounds = static_cast<const __nv_bfloat16*>(k_bounds);
+  p.page_table = page_table;
+  p.page_table_stride = page_table_stride;
+  p.page_table_width = page_table_width;
+  p.cur_pos = cur_pos;
+  p.out_table = out_table;
+  p.out_pos = out_pos;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = group;
+  p.num_blocks = num_blocks;
+  p.num_pages = num_pages;
+  p.keep_first = keep_first;
+  p.keep_last = keep_last;
+  p.max_pages = page_table_width;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const size_t rows = static_cast<size_t>(num_users) * num_kv_heads * page_table_width;
+  p.tickets = reinterpret_cast<unsigned int*>(ws);
+  p.exact = reinterpret_cast<unsigned long long*>(ws + kDecTicketBytes);
+  p.score = reinterpret_cast<float2*>(ws + kDecTicketBytes + rows * sizeof(unsigned long long));
+  p.err_word = dev->err_word;
+  // pages the longest context can have (only the launch geometry goes by it)
+  int pages = page_table_width;
+  if (max_context_len > 0 && (max_context_len - 1) / block_size + 1 < pages)
+    pages = (max_context_len - 1) / block_size + 1;
+  p.slice = 128;
+  const int64_t slices = (static_cast<int64_t>(pages) + p.slice - 1) / p.slice;
+  const dim3 grid(static_cast<unsigned>(slices), static_cast<unsigned>(num_kv_heads),
+                  static_cast<unsigned>(num_users));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (head_size == 128 && block_size == 64) launch_select_pages<128, 64>(group, grid, p, s);
+  else if (head_size == 128) launch_select_pages<128, 32>(group, grid, p, s);
+  else if (block_size == 64) launch_select_pages<64, 64>(group, grid, p, s);
+  else launch_select_pages<64, 32>(group, grid, p, s);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// Identity of the stream capture `stream` is in, 0 when it is not capturing.
+int b200attn_capture_id(uint64_t* id_out, void* stream) {
+  if (!id_out) return B200ATTN_ERR_NULL_POINTER;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id);
+  *id_out = e == cudaSuccess && status == cudaStreamCaptureStatusActive ? id : 0;
+  return static_cast<int>(e);
 }
 
 // ------------------------------------------------------------------------------- prefill
@@ -812,14 +1228,14 @@ int b200attn_prefill(void* out, int64_t out_row_stride, const void* q, int64_t q
                              num_kv_heads, head_size, block_size, num_blocks, scale, 0, stream);
 }
 
-int b200attn_prefill_ex(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
-                        const void* k_src, const void* v_src, int kv_is_paged,
-                        int64_t kv_token_stride, const int32_t* page_table,
-                        int64_t page_table_stride, int page_table_width, const int32_t* cu_q,
-                        const int32_t* cu_q_host, const int32_t* q_start, int num_seqs,
-                        int total_q, int num_q_heads, int num_kv_heads, int head_size,
-                        int block_size, int64_t num_blocks, float scale, int sliding_window,
-                        void* stream) {
+// What prefill_ex and prefill_scaled share.
+static int prefill_any(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                       const void* k_src, const void* v_src, const float* page_factors,
+                       int kv_is_paged, int64_t kv_token_stride, const int32_t* page_table,
+                       int64_t page_table_stride, int page_table_width, const int32_t* cu_q,
+                       const int32_t* cu_q_host, const int32_t* q_start, int num_seqs, int total_q,
+                       int num_q_heads, int num_kv_heads, int head_size, int block_size,
+                       int64_t num_blocks, float scale, int sliding_window, void* stream) {
   if (sliding_window < 0 || !(scale > 0.f)) return B200ATTN_ERR_BAD_ARGUMENT;
   if (!out || !q || !k_src || !v_src || !cu_q || !cu_q_host) return B200ATTN_ERR_NULL_POINTER;
   if (num_seqs < 0 || total_q < 0 || num_q_heads <= 0 || num_kv_heads <= 0)
@@ -893,6 +1309,7 @@ int b200attn_prefill_ex(void* out, int64_t out_row_stride, const void* q, int64_
   if (tag == 0) tag = ++g_pf_launch_seq;      // 0 marks a clear counter word
   p.sched_tag = tag;
   p.sched = dev->pf_sched + tag % kPfSchedSlots;
+  p.page_factors = reinterpret_cast<const float2*>(page_factors);
 #ifdef B200ATTN_PF_TRACE
   p.trace = g_pf_trace;
 #endif
@@ -901,6 +1318,36 @@ int b200attn_prefill_ex(void* out, int64_t out_row_stride, const void* q, int64_
   if (head_size == 128) return launch_prefill<128, 32>(tq, tk, tv, p, dev->sm_count, s);
   if (block_size == 64) return launch_prefill<64, 64>(tq, tk, tv, p, dev->sm_count, s);
   return launch_prefill<64, 32>(tq, tk, tv, p, dev->sm_count, s);
+}
+
+int b200attn_prefill_ex(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                        const void* k_src, const void* v_src, int kv_is_paged,
+                        int64_t kv_token_stride, const int32_t* page_table,
+                        int64_t page_table_stride, int page_table_width, const int32_t* cu_q,
+                        const int32_t* cu_q_host, const int32_t* q_start, int num_seqs,
+                        int total_q, int num_q_heads, int num_kv_heads, int head_size,
+                        int block_size, int64_t num_blocks, float scale, int sliding_window,
+                        void* stream) {
+  return prefill_any(out, out_row_stride, q, q_row_stride, k_src, v_src, nullptr, kv_is_paged,
+                     kv_token_stride, page_table, page_table_stride, page_table_width, cu_q,
+                     cu_q_host, q_start, num_seqs, total_q, num_q_heads, num_kv_heads, head_size,
+                     block_size, num_blocks, scale, sliding_window, stream);
+}
+
+int b200attn_prefill_scaled(void* out, int64_t out_row_stride, const void* q,
+                            int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                            const float* factors, const int32_t* page_table,
+                            int64_t page_table_stride, int page_table_width, const int32_t* cu_q,
+                            const int32_t* cu_q_host, const int32_t* q_start, int num_seqs,
+                            int total_q, int num_q_heads, int num_kv_heads, int head_size,
+                            int block_size, int64_t num_blocks, float scale, int sliding_window,
+                            void* stream) {
+  if (!factors) return B200ATTN_ERR_NULL_POINTER;
+  if (!aligned16(factors)) return B200ATTN_ERR_MISALIGNED;
+  return prefill_any(out, out_row_stride, q, q_row_stride, k_pool, v_pool, factors, 1, 0,
+                     page_table, page_table_stride, page_table_width, cu_q, cu_q_host, q_start,
+                     num_seqs, total_q, num_q_heads, num_kv_heads, head_size, block_size,
+                     num_blocks, scale, sliding_window, stream);
 }
 
 #ifdef B200ATTN_PF_TRACE

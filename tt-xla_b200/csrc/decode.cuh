@@ -51,7 +51,19 @@ struct DecodeParams {
   int cache_fp8;       // 1: the caches hold e4m3
   int wrap_negative;   // 1: a negative position wraps like the reference's CPU indexing, 0: skip
   int* err_word;
+  int per_head;        // 1: page_table is [users, nkv, width] and cur_pos [users, nkv]: a page list
+                       // (and the position within the list) of its own for every KV head
+  int64_t page_table_head_stride;
+  int keep_nan;        // 1: a row whose sum is NaN comes out as NaN, 0: as zeros
 };
+
+__device__ __forceinline__ int decode_cur_pos(const DecodeParams& p, int user, int kvh) {
+  return p.cur_pos[p.per_head ? static_cast<int64_t>(user) * p.num_kv_heads + kvh : user];
+}
+__device__ __forceinline__ const int32_t* decode_page_row(const DecodeParams& p, int user, int kvh) {
+  return p.page_table + static_cast<int64_t>(user) * p.page_table_stride +
+         kvh * p.page_table_head_stride;
+}
 
 // The decode step's cache write, done by the one warp that is about to stream the tile holding
 // the new token: user u's K / V rows of KV head `kvh` go to position cur_pos[u], addressed
@@ -187,7 +199,7 @@ __device__ __forceinline__ void decode_split_finish(const DecodeParams& p, int u
     const int head = kvh * G + r;
     if (p.sinks) acc *= apply_sink(m, l, p.sinks[head] * 1.4426950408889634f);
     p.out[static_cast<int64_t>(user) * p.out_row_stride + head * HD + d] =
-        __float2bfloat16(l > 0.f ? acc / l : 0.f);
+        __float2bfloat16(l > 0.f || (p.keep_nan && l != l) ? acc / l : 0.f);
   }
   if (tid == 0) *ticket = 0u;              // leave the counter as the next launch expects it
 }
@@ -225,7 +237,7 @@ paged_decode_splitkv_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  const int ctx = p.cur_pos[user] + 1;  // keys 0 .. cur_pos
+  const int ctx = decode_cur_pos(p, user, kvh) + 1;  // keys 0 .. cur_pos
   const int lo = (p.window > 0 && ctx > p.window) ? ctx - p.window : 0;   // first key attended
   const int n_tiles = ctx > 0 ? (ctx + kDecTile - 1) / kDecTile : 0;
   const int t_lo = lo / kDecTile;
@@ -277,7 +289,7 @@ paged_decode_splitkv_kernel(const __grid_constant__ CUtensorMap tm_k,
     // the split that streams the last tile writes the new token's rows first
     if (p.k_new && t_end == n_tiles) decode_write_new_token<HD, BS>(p, user, kvh, lane);
     const int n_pages = (ctx + BS - 1) / BS;
-    const int32_t* pt = p.page_table + static_cast<int64_t>(user) * p.page_table_stride;
+    const int32_t* pt = decode_page_row(p, user, kvh);
     const int first_page = t_begin * L::kPages;
     // Each lane keeps one page id of a 32-page window; the next window is fetched early.
     int win_base = first_page;
@@ -547,7 +559,7 @@ __global__ void __launch_bounds__(HD) decode_combine_kernel(const DecodeParams p
   }
   if (p.sinks) acc *= apply_sink(m, l, p.sinks[head] * 1.4426950408889634f);
   p.out[static_cast<int64_t>(user) * p.out_row_stride + head * HD + d] =
-      __float2bfloat16(l > 0.f ? acc / l : 0.f);
+      __float2bfloat16(l > 0.f || (p.keep_nan && l != l) ? acc / l : 0.f);
 }
 
 }  // namespace b200attn

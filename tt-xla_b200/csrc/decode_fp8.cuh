@@ -86,7 +86,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  const int ctx = p.cur_pos[user] + 1;  // keys 0 .. cur_pos
+  const int ctx = decode_cur_pos(p, user, kvh) + 1;  // keys 0 .. cur_pos
   const int lo = (p.window > 0 && ctx > p.window) ? ctx - p.window : 0;   // first key attended
   const int n_tiles = ctx > 0 ? (ctx + kDecTile - 1) / kDecTile : 0;
   const int t_lo = lo / kDecTile;
@@ -138,7 +138,7 @@ paged_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k,
     // the split that streams the last tile writes the new token's rows first
     if (p.k_new && t_end == n_tiles) decode_write_new_token<HD, BS>(p, user, kvh, lane);
     const int n_pages = (ctx + BS - 1) / BS;
-    const int32_t* pt = p.page_table + static_cast<int64_t>(user) * p.page_table_stride;
+    const int32_t* pt = decode_page_row(p, user, kvh);
     int win_base = t_begin * L::kPages;
     auto fetch = [&](int base) {
       const int idx = min(min(base + lane, n_pages - 1), p.page_table_width - 1);

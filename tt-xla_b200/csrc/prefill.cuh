@@ -97,6 +97,9 @@ struct PrefillParams {
   int* err_word;
   unsigned long long* sched;   // this launch's counter word: (tag << 32) | next item
   uint32_t sched_tag;          // unique per launch on a device, never 0
+  // SCALED: (K factor, log2 of the V factor) per page and KV head of the pool a block-scaled cache
+  // was widened into: [num_seqs * page_table_width, num_kv_heads]
+  const float2* page_factors;
 #ifdef B200ATTN_PF_TRACE
   unsigned long long* trace;   // [CTA][role 0..5][8] cycles spent per wait site (debug builds only)
 #endif
@@ -282,7 +285,11 @@ __device__ __forceinline__ void setmaxnreg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-template <int HD, int BS, bool WIN>
+// SCALED: K and V come from dequant_scaled_kernel's pool, whose pages hold code * 2^e, exact in bf16;
+// what is left of a page's scale is a factor in [1, 2) that is applied here in fp32.  The K factor
+// multiplies the scores (in the FMA that scales them anyway), the V factor enters the exponent of
+// the weights, and the row sum takes it out again per 32-key chunk (a chunk lies in one page).
+template <int HD, int BS, bool WIN, bool SCALED>
 __global__ void __launch_bounds__(kPfThreads, 1)
 prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
@@ -713,6 +720,15 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
       if (!take_item(item_no, it)) break;
       const int ip = item_no & 1;
       const int q_pos = it.first_pos + row;
+      // SCALED: the factors of the item's KV head, and its last page (the producers repeat it too)
+      const float2* factors = nullptr;
+      int last_page = 0;
+      if constexpr (SCALED) {
+        factors = p.page_factors +
+                  static_cast<int64_t>(it.seq) * p.page_table_width * p.num_kv_heads +
+                  it.head / p.group;
+        last_page = min((it.first_pos + it.rows_valid - 1) / BS, p.page_table_width - 1);
+      }
       float l_run = 0.f, m_last = -INFINITY;   // this group's row sum, relative to m_last
       for (int jr = 0; jr < it.n_tiles; ++jr) {
         const uint32_t t = t0 + jr;
@@ -720,6 +736,13 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
         const uint32_t b = t % 3u;                       // S / P buffer of the tile
         const uint32_t s_addr = tmem_base + b * kPfN + lane_addr;
         const int j = it.j0 + jr;                        // absolute KV tile
+        float2 fac[SCALED ? kPagesPerTile : 1];          // loaded while S is being computed
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int pg = 0; pg < kPagesPerTile; ++pg)
+            fac[pg] = __ldg(factors + static_cast<int64_t>(min(j * kPagesPerTile + pg, last_page)) *
+                                          p.num_kv_heads);
+        }
         PF_TRACE_BEGIN();
         pf_wait(&s_full[b], (t / 3u) & 1, abort_flag);
         PF_TRACE_END(0);
@@ -782,6 +805,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
           for (int kx = 3; kx + 1 < 32; kx += 2)
             mx[c] = max3(mx[c], __uint_as_float(sreg[c][kx]), __uint_as_float(sreg[c][kx + 1]));
           mx[c] = fmaxf(mx[c], __uint_as_float(sreg[c][31]));
+          if constexpr (SCALED) mx[c] *= fac[c * 32 / BS].x;
         }
         const float mx_s = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
 #ifdef B200ATTN_PF_TRACE
@@ -816,14 +840,23 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
         const float m_sub = (WIN && m_new == -INFINITY) ? 0.f : m_new;
         const uint64_t negm2 = pack_f32x2(-m_sub, -m_sub);
         uint64_t sum2[2] = {0ull, 0ull};
+        float sum_scaled = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t preg[16];
+          uint64_t mul2 = scale2, add2 = negm2;
+          if constexpr (SCALED) {
+            const float2 f = fac[c * 32 / BS];
+            const float mul = p.scale_log2 * f.x, add = f.y - m_sub;
+            mul2 = pack_f32x2(mul, mul);
+            add2 = pack_f32x2(add, add);
+            sum2[0] = sum2[1] = 0ull;
+          }
 #pragma unroll
           for (int kx = 0; kx < 32; kx += 2) {
             const uint64_t x2 = fma_f32x2(
-                pack_f32x2(__uint_as_float(sreg[c][kx]), __uint_as_float(sreg[c][kx + 1])), scale2,
-                negm2);
+                pack_f32x2(__uint_as_float(sreg[c][kx]), __uint_as_float(sreg[c][kx + 1])), mul2,
+                add2);
             float x0, x1, e0, e1;
             unpack_f32x2(x2, x0, x1);
             if (kPfPolyEvery > 0 && ((kx >> 1) % (kPfPolyEvery > 0 ? kPfPolyEvery : 1)) ==
@@ -837,6 +870,12 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
             preg[kx >> 1] = pack_bf16x2(e0, e1);
           }
           tmem_st_32x16(s_addr + c * 16, preg);
+          if constexpr (SCALED) {
+            float a0, a1, b0, b1;
+            unpack_f32x2(sum2[0], a0, a1);
+            unpack_f32x2(sum2[1], b0, b1);
+            sum_scaled += ((a0 + a1) + (b0 + b1)) * fast_exp2(-fac[c * 32 / BS].y);
+          }
         }
         {
           float a0, a1, b0, b1;
@@ -844,7 +883,7 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
           unpack_f32x2(sum2[1], b0, b1);
           // this group's sum is relative to the max at ITS previous tile
           const float f = (m_last == -INFINITY) ? 0.f : fast_exp2(m_last - m_new);
-          l_run = l_run * f + ((a0 + a1) + (b0 + b1));
+          l_run = l_run * f + (SCALED ? sum_scaled : (a0 + a1) + (b0 + b1));
           m_last = m_new;
         }
 #ifdef B200ATTN_PF_TRACE
