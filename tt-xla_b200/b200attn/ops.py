@@ -94,24 +94,36 @@ def _i32(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+# Raw handle of a device's current stream, and the current device, without building Python objects:
+# the ops below are a few microseconds long on the GPU.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the CUDA device all tensors are on; raises when they are not."""
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            _need_cuda(first, t)
             raise ValueError(f"all tensors must be on {first.device}, got one on {t.device}")
+    if index < 0:
+        _need_cuda(first)
+    return index
 
 
 class _on_device:
-    """Makes a tensor's device current for a call into the library (which works on the current
-    device); free of charge when it already is."""
+    """Makes a device current for a call into the library (which works on the current device); free
+    of charge when it already is."""
 
     __slots__ = ("index", "previous")
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
+    def __init__(self, index: int):
+        self.index = index
         self.previous = -1
 
     def __enter__(self):
-        current = torch.cuda.current_device()
+        current = _current_device()
         if current != self.index:
             self.previous = current
             torch.cuda.set_device(self.index)
@@ -124,16 +136,15 @@ class _on_device:
 
 def _check_scales(k_scale, v_scale, k_cache: torch.Tensor) -> bool:
     """True when the caches are block-scaled; the scales are dense fp32 [num_blocks, num_kv_heads]."""
-    if (k_scale is None) != (v_scale is None):
-        raise ValueError("k_scale and v_scale go together")
-    if k_scale is None:
+    if k_scale is None and v_scale is None:
         return False
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32 or tuple(t.shape) != tuple(k_cache.shape[:2]) \
-                or not t.is_contiguous():
-            raise ValueError(f"{name} must be a dense float32 tensor [num_blocks, num_kv_heads]")
-    _need_cuda(k_scale, v_scale)
-    _one_device(k_cache, k_scale, v_scale)
+    if k_scale is None or v_scale is None:
+        raise ValueError("k_scale and v_scale go together")
+    shape = k_cache.shape[:2]
+    if k_scale.shape != shape or v_scale.shape != shape or k_scale.dtype != torch.float32 \
+            or v_scale.dtype != torch.float32 or not k_scale.is_contiguous() \
+            or not v_scale.is_contiguous():
+        raise ValueError("k_scale / v_scale must be dense float32 [num_blocks, num_kv_heads]")
     return True
 
 
@@ -305,15 +316,17 @@ def rope_kv_scatter_slots(
     )
 
 
-def _spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory between the first and the last element of two 2-D row tensors meets."""
-    def span(t):
-        lo = t.data_ptr()
-        return lo, lo + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-    if a.numel() == 0 or b.numel() == 0:
+def _rows_meet(a: tuple, b: tuple, tokens: int) -> bool:
+    """Whether two sets of `tokens` rows, each (pointer, row stride, row width) in bytes, share
+    memory.  Exact for equal strides (columns of one buffer), else by the memory between their
+    first and last byte."""
+    (a0, a_step, a_width), (b0, b_step, b_width) = a, b
+    if b0 >= a0 + (tokens - 1) * a_step + a_width or a0 >= b0 + (tokens - 1) * b_step + b_width:
         return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if a_step == b_step:
+        gap = (b0 - a0) % a_step
+        return gap < a_width or a_step - gap < b_width
+    return True
 
 
 def qk_norm_rope_kv_scatter_slots(
@@ -343,80 +356,73 @@ def qk_norm_rope_kv_scatter_slots(
     input or overlaps none of the inputs.  Pairs are (i, i + rotary_dim/2) for `is_neox_style`,
     (2i, 2i + 1) otherwise.  Caches: bf16 or unscaled e4m3 (`paged_write` fills block-scaled
     ones).  Returns (out_query, out_key)."""
-    _need_cuda(query, key, value, positions, inv_freq, q_weight, k_weight, k_cache, v_cache,
-               slot_mapping, out_query, out_key)
-    _one_device(query, key, value, positions, inv_freq, q_weight, k_weight, k_cache, v_cache,
-                slot_mapping, out_query, out_key)
+    oq = query if out_query is None else out_query
+    ok = key if out_key is None else out_key
+    index = _device_of(query, key, positions, inv_freq, q_weight, k_weight, out_query, out_key,
+                       value, slot_mapping, k_cache, v_cache)
     tokens = positions.numel()
     if query.dim() != 2 or key.dim() != 2 or query.shape[0] != tokens or key.shape[0] != tokens:
         raise ValueError("query / key must be [tokens, heads*head_size] with one row per position")
-    if query.shape[1] % head_size or key.shape[1] % head_size:
+    q_width, k_width = query.shape[1], key.shape[1]
+    if q_width % head_size or k_width % head_size:
         raise ValueError("query / key rows must hold whole heads")
-    outs = []
-    for name, x, out in (("query", query, out_query), ("key", key, out_key)):
-        out = x if out is None else out
-        if out.shape != x.shape:
-            raise ValueError(f"out_{name} must have {name}'s shape")
-        for t in (x, out):
-            if t.dtype != torch.bfloat16 or t.stride(1) != 1:
-                raise ValueError(f"{name} must be bfloat16 with dense rows")
-        outs.append(out)
-    for i, out in enumerate(outs):
-        own_input = (query, key)[i]
-        if out.data_ptr() != own_input.data_ptr() or (tokens > 1 and
-                                                      out.stride(0) != own_input.stride(0)):
-            for x in (query, key, value):
-                if x is not None and x.dim() == 2 and _spans_overlap(out, x):
-                    raise ValueError("an output must be its input or overlap none of the inputs")
-            if _spans_overlap(out, outs[1 - i]):
-                raise ValueError("the outputs must not overlap")
-    nq, nkv = query.shape[1] // head_size, key.shape[1] // head_size
+    if oq.shape != query.shape or ok.shape != key.shape:
+        raise ValueError("out_query / out_key must have query's / key's shape")
+    bf16 = torch.bfloat16
+    strides = []
+    for t in (oq, ok, query, key):
+        row, column = t.stride()
+        if t.dtype != bf16 or column != 1:
+            raise ValueError("query, key and the outputs must be bfloat16 with dense rows")
+        strides.append(row if tokens > 1 else t.shape[1])
     if positions.dtype != torch.int64 or not positions.is_contiguous():
         raise ValueError("positions must be a dense int64 tensor")
     if inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2 \
             or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be dense float32 [rotary_dim / 2]")
-    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (torch.bfloat16, torch.float32):
+    w_dtype = q_weight.dtype
+    if w_dtype != k_weight.dtype or w_dtype not in (bf16, torch.float32):
         raise ValueError("q_weight / k_weight must both be bfloat16 or both be float32")
-    for w in (q_weight, k_weight):
-        if w.numel() != head_size or not w.is_contiguous():
-            raise ValueError("q_weight / k_weight must be dense [head_size]")
-    nb = bs = 0
+    if q_weight.numel() != head_size or k_weight.numel() != head_size \
+            or not q_weight.is_contiguous() or not k_weight.is_contiguous():
+        raise ValueError("q_weight / k_weight must be dense [head_size]")
+    nkv = k_width // head_size
+    nb = bs = v_stride = v_ptr = kc_ptr = vc_ptr = slot_ptr = kind = 0
     if slot_mapping is not None:
         if k_cache is None or v_cache is None or value is None:
             raise ValueError("slot_mapping needs k_cache, v_cache and value")
         nb, nkv_c, bs, hd_c = _check_cache(k_cache, v_cache)
         if nkv_c != nkv or hd_c != head_size:
             raise ValueError("cache geometry differs from key geometry")
-        if value.shape != key.shape or value.dtype != torch.bfloat16 or value.stride(1) != 1:
+        if value.shape != key.shape or value.dtype != bf16 or value.stride(1) != 1:
             raise ValueError("value must match key")
         if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < tokens \
                 or not slot_mapping.is_contiguous():
             raise ValueError("slot_mapping must be dense int64 with one entry per token")
+        v_stride = value.stride(0) if tokens > 1 else k_width
+        v_ptr, kc_ptr, vc_ptr = value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        slot_ptr, kind = slot_mapping.data_ptr(), _cache_dtype(k_cache)
     if tokens == 0:
-        return outs[0], outs[1]
-
-    def stride(t):
-        return t.stride(0) if tokens > 1 else t.shape[1]
-
-    write = slot_mapping is not None
-    with _on_device(query):
-        _lib.check(
-            "b200attn_qk_norm_rope_kv_scatter_slots",
-            _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
-                outs[0].data_ptr(), stride(outs[0]), outs[1].data_ptr(), stride(outs[1]),
-                query.data_ptr(), stride(query), key.data_ptr(), stride(key),
-                value.data_ptr() if write else None, stride(value) if write else 0,
-                q_weight.data_ptr(), k_weight.data_ptr(),
-                1 if q_weight.dtype == torch.float32 else 0, float(eps), positions.data_ptr(),
-                inv_freq.data_ptr(), rotary_dim, 1 if is_neox_style else 0,
-                k_cache.data_ptr() if write else None, v_cache.data_ptr() if write else None,
-                _cache_dtype(k_cache) if write else CACHE_BF16,
-                slot_mapping.data_ptr() if write else None, tokens, nq, nkv, head_size, bs, nb,
-                _stream(query),
-            ),
-        )
-    return outs[0], outs[1]
+        return oq, ok
+    oq_ptr, ok_ptr, q_ptr, k_ptr = oq.data_ptr(), ok.data_ptr(), query.data_ptr(), key.data_ptr()
+    outs = ((oq_ptr, 2 * strides[0], 2 * q_width), (ok_ptr, 2 * strides[1], 2 * k_width))
+    ins = ((q_ptr, 2 * strides[2], 2 * q_width), (k_ptr, 2 * strides[3], 2 * k_width),
+           (v_ptr, 2 * v_stride, 2 * k_width))
+    for i in (0, 1):
+        if outs[i] != ins[i] and any(_rows_meet(outs[i], x, tokens) for x in ins if x[0]):
+            raise ValueError("an output must be its input or overlap none of the inputs")
+    if _rows_meet(outs[0], outs[1], tokens):
+        raise ValueError("the outputs must not overlap")
+    with _on_device(index):
+        status = _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
+            oq_ptr, strides[0], ok_ptr, strides[1], q_ptr, strides[2], k_ptr, strides[3],
+            v_ptr, v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
+            1 if w_dtype == torch.float32 else 0, eps, positions.data_ptr(), inv_freq.data_ptr(),
+            rotary_dim, 1 if is_neox_style else 0, kc_ptr, vc_ptr, kind, slot_ptr, tokens,
+            q_width // head_size, nkv, head_size, bs, nb, _raw_stream(index))
+    if status:
+        _lib.check("b200attn_qk_norm_rope_kv_scatter_slots", status)
+    return oq, ok
 
 
 def _rows_3d(x: torch.Tensor, nheads: int, hd: int, name: str) -> tuple[torch.Tensor, int]:
@@ -453,52 +459,51 @@ def paged_write(
     the scale NaN, and with it everything read through the page.  `k_bounds` (bf16 [num_blocks,
     num_kv_heads, 2, head_size]) keeps the least and greatest key of each channel for
     `select_pages`.  The sequences of one call must write to different pages."""
-    _need_cuda(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len, k_scale, v_scale,
-               k_bounds)
-    _one_device(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len, k_bounds)
+    index = _device_of(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len, k_scale,
+                       v_scale, k_bounds)
     scaled = _check_scales(k_scale, v_scale, k_cache)
     nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
-    if not scaled and k_cache.dtype != torch.bfloat16:
-        raise ValueError("an 8-bit cache needs k_scale and v_scale here (kv_scatter_slots writes "
-                         "unscaled e4m3)")
-    if not scaled and k_bounds is None:
-        raise ValueError("a bf16 cache without k_bounds is kv_scatter_slots's")
+    if not scaled:
+        if k_cache.dtype != torch.bfloat16:
+            raise ValueError("an 8-bit cache needs k_scale and v_scale here (kv_scatter_slots "
+                             "writes unscaled e4m3)")
+        if k_bounds is None:
+            raise ValueError("a bf16 cache without k_bounds is kv_scatter_slots's")
     if k_bounds is not None and (k_bounds.dtype != torch.bfloat16 or not k_bounds.is_contiguous()
-                                 or tuple(k_bounds.shape) != (nb, nkv, 2, hd)):
+                                 or k_bounds.shape != (nb, nkv, 2, hd)):
         raise ValueError("k_bounds must be dense bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
     key, kstride = _rows_3d(key, nkv, hd, "key")
     value, vstride = _rows_3d(value, nkv, hd, "value")
-    if key.shape != value.shape:
+    rows = key.shape[0]
+    if value.shape[0] != rows:
         raise ValueError("key and value must have the same shape")
-    _i32(page_table, "page_table")
-    _i32(q_start, "q_start")
+    i32 = torch.int32
     seqs = q_start.numel()
-    if page_table.dim() != 2 or page_table.shape[0] < seqs or page_table.stride(1) != 1 \
-            or not q_start.is_contiguous():
-        raise ValueError("page_table needs a dense row, and q_start a dense entry, per sequence")
+    if page_table.dtype != i32 or page_table.dim() != 2 or page_table.shape[0] < seqs \
+            or page_table.stride(1) != 1:
+        raise ValueError("page_table must be int32 with a dense row per sequence")
+    if q_start.dtype != i32 or not q_start.is_contiguous():
+        raise ValueError("q_start must be int32 with a dense entry per sequence")
     if cu_q is None:
-        if key.shape[0] != seqs:
+        if rows != seqs:
             raise ValueError("without cu_q, key / value must hold one row per sequence")
-    elif _i32(cu_q, "cu_q").numel() != seqs + 1 or not cu_q.is_contiguous():
-        raise ValueError("cu_q must hold num_seqs + 1 dense entries")
-    if q_len is not None and (_i32(q_len, "q_len").numel() != seqs or not q_len.is_contiguous()):
-        raise ValueError("q_len must hold one dense entry per sequence")
-    if seqs == 0 or key.shape[0] == 0:
+    elif cu_q.dtype != i32 or cu_q.numel() != seqs + 1 or not cu_q.is_contiguous():
+        raise ValueError("cu_q must be int32 with num_seqs + 1 dense entries")
+    if q_len is not None and (q_len.dtype != i32 or q_len.numel() != seqs
+                              or not q_len.is_contiguous()):
+        raise ValueError("q_len must be int32 with a dense entry per sequence")
+    if seqs == 0 or rows == 0:
         return
-    with _on_device(k_cache):
-        _lib.check(
-            "b200attn_paged_write",
-            _lib.lib().b200attn_paged_write(
-                k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if scaled else None,
-                v_scale.data_ptr() if scaled else None,
-                k_bounds.data_ptr() if k_bounds is not None else None, _cache_dtype(k_cache),
-                key.data_ptr(), kstride, value.data_ptr(), vstride, page_table.data_ptr(),
-                page_table.stride(0), page_table.shape[1],
-                cu_q.data_ptr() if cu_q is not None else None,
-                q_len.data_ptr() if q_len is not None else None, q_start.data_ptr(), seqs,
-                key.shape[0], nkv, hd, bs, nb, _stream(k_cache),
-            ),
-        )
+    with _on_device(index):
+        status = _lib.lib().b200attn_paged_write(
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if scaled else 0,
+            v_scale.data_ptr() if scaled else 0, 0 if k_bounds is None else k_bounds.data_ptr(),
+            _cache_dtype(k_cache), key.data_ptr(), kstride, value.data_ptr(), vstride,
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+            0 if cu_q is None else cu_q.data_ptr(), 0 if q_len is None else q_len.data_ptr(),
+            q_start.data_ptr(), seqs, rows, nkv, hd, bs, nb, _raw_stream(index))
+    if status:
+        _lib.check("b200attn_paged_write", status)
 
 
 def decode_auto_splits(users: int, nkv: int, hd: int, max_context_len: int) -> int:
@@ -528,21 +533,24 @@ def _workspace(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
 _capture_workspaces: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
 
 
-def _scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
-    """Scratch of the block-scaled and page-list ops, `device` current.  Eager calls take the
-    per-stream workspace.  Calls under stream capture take one that belongs to the graph being
-    captured (from its memory pool, its counters zeroed by a node of the graph), so that graphs
-    captured on the same stream may be replayed side by side on others."""
-    if nbytes == 0 or not torch.cuda.is_current_stream_capturing():
-        return _workspace(device, nbytes)
-    stream = torch.cuda.current_stream(device).cuda_stream
+def _scratch(index: int, stream: int, nbytes: int) -> Optional[torch.Tensor]:
+    """Scratch of the block-scaled and page-list ops on the (current) device `index`.  Eager calls
+    take the stream's workspace.  Calls under stream capture take one that belongs to the graph
+    being captured (from its memory pool, its counters zeroed by a node of the graph), so that
+    graphs captured on the same stream may be replayed side by side on others."""
+    if nbytes == 0:
+        return None
+    key = (index, stream)
+    if not torch.cuda.is_current_stream_capturing():
+        ws = _workspaces.get(key)
+        return ws if ws is not None and ws.numel() >= nbytes else \
+            _workspace(torch.device("cuda", index), nbytes)
     capture = ctypes.c_uint64(0)
     _lib.check("b200attn_capture_id",
                _lib.lib().b200attn_capture_id(ctypes.byref(capture), stream))
-    key = (device.index or 0, stream)
     have = _capture_workspaces.get(key)
     if have is None or have[0] != capture.value or have[1].numel() < nbytes:
-        ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", index))
         ws[:TICKET_BYTES].zero_()
         have = (capture.value, ws)
         _capture_workspaces[key] = have
@@ -568,8 +576,7 @@ def select_pages(
     keeps them; `page_table` [users, width] and `cur_pos` [users] as for `paged_decode`.
     Returns (table [users, nkv, num_pages], pos [users, nkv]): hand them to `paged_decode` as
     `page_table` and `cur_pos`.  `max_context_len` only shapes the launch."""
-    _need_cuda(query, k_bounds, page_table, cur_pos)
-    _one_device(query, k_bounds, page_table, cur_pos, workspace)
+    index = _device_of(query, k_bounds, page_table, cur_pos, workspace)
     if k_bounds.dim() != 4 or k_bounds.shape[2] != 2 or k_bounds.dtype != torch.bfloat16 \
             or not k_bounds.is_contiguous():
         raise ValueError("k_bounds must be dense bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
@@ -578,86 +585,114 @@ def select_pages(
         query = query[0]
     if query.dim() != 3 or query.shape[2] != hd:
         raise ValueError(f"query must be [users, nq, {hd}], got {tuple(query.shape)}")
-    users, nq = query.shape[0], query.shape[1]
+    users, nq, _ = query.shape
     if nq % nkv != 0:
         raise ValueError(f"num_q_heads {nq} is not a multiple of num_kv_heads {nkv}")
     q, qstride = _token_major(query, nq, hd, "query")
-    _i32(page_table, "page_table")
-    _i32(cur_pos, "cur_pos")
-    if page_table.dim() != 2 or page_table.shape[0] < users or page_table.stride(1) != 1 \
-            or not cur_pos.is_contiguous() or cur_pos.numel() != users:
-        raise ValueError("page_table needs a dense row, and cur_pos a dense entry, per user")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < users \
+            or page_table.stride(1) != 1:
+        raise ValueError("page_table must be int32 with a dense row per user")
+    if cur_pos.dtype != torch.int32 or not cur_pos.is_contiguous() or cur_pos.numel() != users:
+        raise ValueError("cur_pos must be int32 with a dense entry per user")
     if keep_first < 0 or keep_last < 1 or keep_first + keep_last > num_pages:
         raise ValueError("keep_first >= 0 and keep_last >= 1 must fit into num_pages")
-    table = torch.empty((users, nkv, num_pages), dtype=torch.int32, device=query.device)
-    pos = torch.empty((users, nkv), dtype=torch.int32, device=query.device)
+    table = cur_pos.new_empty((users, nkv, num_pages))
+    pos = cur_pos.new_empty((users, nkv))
     if users == 0:
         return table, pos
     L = _lib.lib()
     width = page_table.shape[1]
-    with _on_device(query):
+    with _on_device(index):
+        stream = _raw_stream(index)
         ws = workspace
         if ws is None:
-            ws = _scratch(query.device, L.b200attn_select_pages_workspace_bytes(users, nkv, width))
-        _lib.check(
-            "b200attn_select_pages",
-            L.b200attn_select_pages(
-                table.data_ptr(), pos.data_ptr(), q.data_ptr(), qstride, k_bounds.data_ptr(),
-                page_table.data_ptr(), page_table.stride(0), width, cur_pos.data_ptr(), users, nq,
-                nkv, hd, block_size, nb, num_pages, keep_first, keep_last, max_context_len,
-                ws.data_ptr() if ws is not None else None,
-                ws.numel() * ws.element_size() if ws is not None else 0, _stream(query),
-            ),
-        )
+            ws = _scratch(index, stream, L.b200attn_select_pages_workspace_bytes(users, nkv, width))
+        status = L.b200attn_select_pages(
+            table.data_ptr(), pos.data_ptr(), q.data_ptr(), qstride, k_bounds.data_ptr(),
+            page_table.data_ptr(), page_table.stride(0), width, cur_pos.data_ptr(), users, nq, nkv,
+            hd, block_size, nb, num_pages, keep_first, keep_last, max_context_len, ws.data_ptr(),
+            ws.numel() * ws.element_size(), stream)
+    if status:
+        _lib.check("b200attn_select_pages", status)
     return table, pos
 
 
-def _decode_blocks(q, qstride, out_t, ostride, k_cache, v_cache, k_scale, v_scale, page_table,
-                   cur_pos, scale, num_splits, max_context_len, workspace, sliding_window, sinks,
-                   geometry) -> None:
+def _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out, num_splits,
+                   max_context_len, workspace, sliding_window, sinks, k_scale, v_scale):
     """paged_decode over block-scaled caches and / or a page list per KV head."""
-    users, nq, nb, nkv, bs, hd = geometry
-    _one_device(q, out_t, k_cache, v_cache, page_table, cur_pos, sinks, workspace)
+    index = _device_of(query, k_cache, v_cache, page_table, cur_pos, k_scale, v_scale, out, sinks,
+                       workspace)
+    scaled = _check_scales(k_scale, v_scale, k_cache)
+    nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
+    shape = query.shape
+    if query.dim() == 4 and shape[0] == 1:
+        query = query[0]
+    if query.dim() != 3 or query.shape[2] != hd:
+        raise ValueError(f"query must be [users, nq, {hd}], got {tuple(shape)}")
+    users, nq, _ = query.shape
+    if nq % nkv != 0:
+        raise ValueError(f"num_q_heads {nq} is not a multiple of num_kv_heads {nkv}")
+    q, qstride = _token_major(query, nq, hd, "query")
+    if out is None:
+        out_t = q.new_empty((users, nq, hd))
+    else:
+        out_t = out.reshape(users, nq, hd) if out.dim() != 3 else out
+        if out_t.shape != q.shape or out_t.dtype != torch.bfloat16 or out_t.stride(2) != 1 \
+                or out_t.stride(1) != hd:
+            raise ValueError("out must be a dense-row bfloat16 tensor of query's shape")
+        if out_t.data_ptr() != out.data_ptr():
+            raise ValueError("out must be viewable as [users, nq, hd] without a copy")
+    ostride = out_t.stride(0) if users > 1 else max(out_t.stride(0), nq * hd)
+    if page_table.dtype != torch.int32 or cur_pos.dtype != torch.int32:
+        raise ValueError("page_table and cur_pos must be int32")
+    if page_table.stride(-1) != 1 or not cur_pos.is_contiguous():
+        raise ValueError("page_table rows and cur_pos must be dense")
+    width = page_table.shape[-1]
     head_stride = 0
     if page_table.dim() == 3:
-        if tuple(page_table.shape[:2]) != (users, nkv) or page_table.stride(2) != 1:
-            raise ValueError("a page list per KV head must be dense [users, num_kv_heads, pages]")
-        if tuple(cur_pos.shape) != (users, nkv):
+        if page_table.shape[0] != users or page_table.shape[1] != nkv:
+            raise ValueError("a page list per KV head must be [users, num_kv_heads, pages]")
+        if cur_pos.shape != (users, nkv):
             raise ValueError("with a page list per KV head cur_pos must be [users, num_kv_heads]")
         if sliding_window > 0:
             raise ValueError("a list of chosen pages has no sliding window")
-        head_stride = page_table.stride(1)
-        if head_stride < page_table.shape[2]:
+        head_stride = page_table.stride(1) if nkv > 1 else max(page_table.stride(1), width)
+        if head_stride < width:
             raise ValueError("the page lists of the KV heads must not overlap")
+        max_context_len = min(max_context_len, width * bs)
     elif page_table.dim() != 2 or page_table.shape[0] < users or cur_pos.numel() != users:
         raise ValueError("page_table needs a row, and cur_pos an entry, per user")
-    width = page_table.shape[-1]
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nq
+                              or not sinks.is_contiguous()):
+        raise ValueError("sinks must be a dense float32 tensor with one entry per q head")
+    if users == 0:
+        return out if out is not None else out_t.reshape(shape)
     L = _lib.lib()
-    with _on_device(q):
+    with _on_device(index):
+        stream = _raw_stream(index)
+        if num_splits == 0:
+            num_splits = _env_num_splits()
         if num_splits == 0:
             ctx = max_context_len if max_context_len > 0 else width * bs
-            if head_stride:
-                ctx = min(ctx, width * bs)
             if sliding_window > 0:
                 ctx = min(ctx, sliding_window + 64)
-            pick = L.b200attn_decode_blocks_auto_splits if k_scale is not None \
-                else L.b200attn_decode_auto_splits
+            pick = L.b200attn_decode_blocks_auto_splits if scaled else L.b200attn_decode_auto_splits
             num_splits = pick(users, nkv, hd, ctx)
-        need = L.b200attn_decode_workspace_bytes(users, nq, hd, num_splits)
-        ws = workspace if workspace is not None else _scratch(q.device, need)
-        _lib.check(
-            "b200attn_paged_decode_blocks",
-            L.b200attn_paged_decode_blocks(
-                out_t.data_ptr(), ostride, q.data_ptr(), qstride, k_cache.data_ptr(),
-                v_cache.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
-                v_scale.data_ptr() if v_scale is not None else None, _cache_dtype(k_cache),
-                page_table.data_ptr(), page_table.stride(0), head_stride, width,
-                cur_pos.data_ptr(), users, nq, nkv, hd, bs, nb, float(scale), int(sliding_window),
-                sinks.data_ptr() if sinks is not None else None, max_context_len, num_splits,
-                ws.data_ptr() if ws is not None else None,
-                ws.numel() * ws.element_size() if ws is not None else 0, _stream(q),
-            ),
-        )
+        ws = workspace
+        if ws is None and num_splits > 1:
+            ws = _scratch(index, stream, L.b200attn_decode_workspace_bytes(users, nq, hd, num_splits))
+        status = L.b200attn_paged_decode_blocks(
+            out_t.data_ptr(), ostride, q.data_ptr(), qstride, k_cache.data_ptr(),
+            v_cache.data_ptr(), k_scale.data_ptr() if scaled else 0,
+            v_scale.data_ptr() if scaled else 0, _cache_dtype(k_cache), page_table.data_ptr(),
+            page_table.stride(0), head_stride, width, cur_pos.data_ptr(), users, nq, nkv, hd, bs,
+            nb, hd ** -0.5 if scale is None else scale, sliding_window,
+            sinks.data_ptr() if sinks is not None else 0, max_context_len, num_splits,
+            ws.data_ptr() if ws is not None else 0,
+            ws.numel() * ws.element_size() if ws is not None else 0, stream)
+    if status:
+        _lib.check("b200attn_paged_decode_blocks", status)
+    return out if out is not None else out_t.reshape(shape)
 
 
 def paged_decode(
@@ -693,9 +728,14 @@ def paged_decode(
     page and KV head, as `paged_write` fills them.  A `page_table` [users, nkv, pages] with a
     `cur_pos` [users, nkv] gives every KV head its own list of pages, `cur_pos` counting within the
     list: what `select_pages` returns (no `sliding_window` then).  Neither form takes `new_key`."""
+    if k_scale is not None or v_scale is not None or page_table.dim() == 3:
+        if new_key is not None or new_value is not None:
+            raise ValueError("new_key / new_value go with unscaled caches and one page list per "
+                             "user; use paged_write first")
+        return _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out, num_splits,
+                              max_context_len, workspace, sliding_window, sinks, k_scale, v_scale)
     _need_cuda(query, k_cache, v_cache, page_table, cur_pos, out, new_key, new_value)
-    scaled = _check_scales(k_scale, v_scale, k_cache)
-    nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
+    nb, nkv, bs, hd = _check_cache(k_cache, v_cache)
     orig_shape = query.shape
     if query.dim() == 4:
         if query.shape[0] != 1:
@@ -718,9 +758,7 @@ def paged_decode(
     ostride = out_t.stride(0) if users > 1 else max(out_t.stride(0), nq * hd)
     _i32(page_table, "page_table")
     _i32(cur_pos, "cur_pos")
-    blocks = scaled or page_table.dim() == 3
-    if not cur_pos.is_contiguous() or page_table.stride(-1) != 1 or (not blocks and
-                                                                    cur_pos.numel() != users):
+    if page_table.stride(1) != 1 or not cur_pos.is_contiguous() or cur_pos.numel() != users:
         raise ValueError("page_table rows must be dense and cur_pos must hold one entry per user")
     if scale is None:
         scale = hd ** -0.5
@@ -731,16 +769,6 @@ def paged_decode(
             raise ValueError("sinks must be a dense float32 tensor with one entry per q head")
     if num_splits == 0:
         num_splits = _env_num_splits()
-    if blocks:
-        if new_key is not None or new_value is not None:
-            raise ValueError("new_key / new_value go with unscaled caches and one page list per "
-                             "user; use paged_write first")
-        if users:
-            _decode_blocks(q, qstride if users > 1 else max(qstride, nq * hd), out_t, ostride,
-                           k_cache, v_cache, k_scale, v_scale, page_table, cur_pos, scale,
-                           num_splits, max_context_len, workspace, sliding_window, sinks,
-                           (users, nq, nb, nkv, bs, hd))
-        return out if out is not None else out_t.reshape(orig_shape)
     if num_splits == 0:
         ctx = max_context_len if max_context_len > 0 else page_table.shape[1] * bs
         if sliding_window > 0:
@@ -846,7 +874,7 @@ def prefill(
         cu_q = cu_q_host.to(query.device, non_blocking=True)
     _i32(cu_q, "cu_q")
     if scaled:
-        _one_device(query, k_src, v_src, page_table, q_start, cu_q, out)
+        index = _device_of(query, k_src, v_src, page_table, q_start, cu_q, out, k_scale, v_scale)
         k, v, factors, page_table, nb = _widen_scaled_pages(k_src, v_src, k_scale, v_scale,
                                                             page_table, cu_q, q_start, num_seqs)
     elif paged and k_src.dtype == torch.float8_e4m3fn:
@@ -867,7 +895,7 @@ def prefill(
         scale = hd ** -0.5
     L = _lib.lib()
     if scaled:
-        with _on_device(query):
+        with _on_device(index):
             _lib.check(
                 "b200attn_prefill_scaled",
                 L.b200attn_prefill_scaled(
@@ -943,7 +971,7 @@ def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_
     width = page_table.shape[1]
     pages = max(num_seqs * width, 1)
     dev = k_cache.device
-    with _on_device(k_cache):
+    with _on_device(dev.index):
         stream = torch.cuda.current_stream(dev).cuda_stream
         capturing = torch.cuda.is_current_stream_capturing()
         key = (dev.index or 0, stream, nkv, bs, hd)

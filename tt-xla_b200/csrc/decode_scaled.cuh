@@ -9,7 +9,7 @@
 // 64-token tiles full with TMA, and four warps take 16 tokens of a tile each.  What differs:
 //   * the products are transposed: S^T = K Q^T and O^T = V^T P^T, tokens resp. head elements in
 //     the 16 rows of m16n8k16 and the query heads in its 8 columns.  Up to 8 query heads per KV
-//     head then fill an MMA (the other way round 8 of 16 rows would be padding), and the
+//     head then fill an MMA (otherwise half of the 16 rows would be padding), and the
 //     accumulators of 128 x 8 outputs are 32 registers;
 //   * codes become f16 in registers, exactly.  A 16-bit `ldmatrix` hands a thread four consecutive
 //     bytes b0..b3 of a token (K), or 2 elements of 2 tokens (V, transposed).  Bytes 0 and 2 of a
