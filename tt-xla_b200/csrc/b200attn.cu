@@ -22,6 +22,9 @@
 #include "select_pages.cuh"
 #include "step_metadata.cuh"
 
+#ifndef B200ATTN_DS_STAGES
+#define B200ATTN_DS_STAGES 3
+#endif
 namespace b200attn {
 
 static_assert(kDecTicketBytes == B200ATTN_DECODE_TICKET_BYTES, "header and kernels agree");
@@ -291,7 +294,7 @@ static int launch_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, const
 template <int HD, int BS, int FMT, int NG>
 static int launch_decode_scaled(const CUtensorMap& tk, const CUtensorMap& tv,
                                 const DecodeScaledParams& p, int num_users, cudaStream_t s) {
-  constexpr int kStages = 6;
+  constexpr int kStages = HD == 128 ? B200ATTN_DS_STAGES : 6;
   using L = DecodeScaledSmem<HD, BS, kStages>;
   auto kern = paged_decode_scaled_kernel<HD, BS, FMT, NG, kStages>;
   static bool smem_allowed[kMaxDevices] = {};
@@ -322,6 +325,18 @@ static int launch_decode_scaled_fmt(int fmt, const CUtensorMap& tk, const CUtens
                                     const DecodeScaledParams& p, int num_users, cudaStream_t s) {
   return fmt == kPageInt8 ? launch_decode_scaled_ng<HD, BS, kPageInt8>(tk, tv, p, num_users, s)
                           : launch_decode_scaled_ng<HD, BS, kPageE4m3>(tk, tv, p, num_users, s);
+}
+
+// the layout of a head in its lanes (see NrLayout)
+template <int HD>
+static void launch_qk_norm_rope(const QkNormRopeParams& p, int num_tokens, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(num_tokens);
+  if (!p.neox)
+    qk_norm_rope_kernel<HD, kNrAdjacent><<<grid, kNrThreads, 0, s>>>(p);
+  else if (p.rotary_dim == HD)
+    qk_norm_rope_kernel<HD, kNrSplit><<<grid, kNrThreads, 0, s>>>(p);
+  else
+    qk_norm_rope_kernel<HD, kNrShuffle><<<grid, kNrThreads, 0, s>>>(p);
 }
 
 template <int HD, int BS>
@@ -998,10 +1013,8 @@ int b200attn_qk_norm_rope_kv_scatter_slots(
   p.num_blocks = num_blocks;
   p.err_word = dev->err_word;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (head_size == 128)
-    qk_norm_rope_kernel<128><<<static_cast<unsigned>(num_tokens), kNrThreads, 0, s>>>(p);
-  else
-    qk_norm_rope_kernel<64><<<static_cast<unsigned>(num_tokens), kNrThreads, 0, s>>>(p);
+  if (head_size == 128) launch_qk_norm_rope<128>(p, num_tokens, s);
+  else launch_qk_norm_rope<64>(p, num_tokens, s);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1191,7 +1204,12 @@ int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
   int pages = page_table_width;
   if (max_context_len > 0 && (max_context_len - 1) / block_size + 1 < pages)
     pages = (max_context_len - 1) / block_size + 1;
-  p.slice = 128;
+  // about two CTAs per SM; a slice is a multiple of the 128 pages that the warps of a CTA score at
+  // once (one CTA per (user, KV head) needs no second trip of the scores through memory)
+  const int64_t ctas = 2 * static_cast<int64_t>(dev->sm_count);
+  const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
+  const int64_t per_pair = pairs < ctas ? ctas / pairs : 1;
+  p.slice = static_cast<int>(((pages + per_pair - 1) / per_pair + 127) / 128 * 128);
   const int64_t slices = (static_cast<int64_t>(pages) + p.slice - 1) / p.slice;
   const dim3 grid(static_cast<unsigned>(slices), static_cast<unsigned>(num_kv_heads),
                   static_cast<unsigned>(num_users));

@@ -79,6 +79,91 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
 
 constexpr float kScoreSlack = 8.f;   // log2 units a score may pass the running maximum by
 
+// decode_split_finish for this kernel: the same protocol (the split that arrives last merges), with
+// the partial rows read as 16-byte vectors, eight splits in flight per thread: the merge is one CTA
+// reading splits * G * head_size floats, and its time is their latency.
+template <int HD>
+__device__ __forceinline__ void decode_scaled_finish(const DecodeParams& p, int user, int kvh,
+                                                     float* scratch, int tid) {
+  constexpr int kThreads = kDecConsumerWarps * 32;
+  const int S = p.num_splits, G = p.group;
+  float* fac = scratch;                    // [G][S] running max of a split, then its merge factor
+  float* row_m = scratch + 16 * S;         // [G] merged max
+  float* row_l = row_m + 16;               // [G] merged sum
+  volatile int* last_flag = reinterpret_cast<volatile int*>(row_l + 16);
+  unsigned int* ticket = p.tickets + static_cast<int64_t>(user) * p.num_kv_heads + kvh;
+
+  __threadfence();                         // this thread's partial stores, device-wide
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+  if (tid == 0) *last_flag = atomicAdd(ticket, 1u) == static_cast<unsigned int>(S - 1);
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+  if (!*last_flag) return;
+  __threadfence();
+  if (tid == 0) *ticket = 0u;              // leave the counter as the next launch expects it
+
+  const int64_t row0 = (static_cast<int64_t>(user) * p.num_q_heads + kvh * G) * S;
+  const int warp = tid >> 5, lane = tid & 31;
+  for (int r = warp; r < G; r += kDecConsumerWarps) {
+    const float2* ml = p.part_ml + row0 + static_cast<int64_t>(r) * S;
+    float m = -INFINITY, l = 0.f;
+    // two passes over at most kDecMaxSplits pairs: they stay in registers
+    float2 v[kDecMaxSplits / 32];
+#pragma unroll
+    for (int i = 0; i < kDecMaxSplits / 32; ++i) {
+      v[i] = i * 32 + lane < S ? __ldcg(ml + i * 32 + lane) : make_float2(-INFINITY, 0.f);
+      m = fmaxf(m, v[i].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+    for (int i = 0; i < kDecMaxSplits / 32; ++i) {
+      const float f = v[i].x == -INFINITY ? 0.f : fast_exp2(v[i].x - m);   // empty splits: -inf
+      l += f * v[i].y;
+      if (i * 32 + lane < S) fac[r * S + i * 32 + lane] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {
+      row_m[r] = m;
+      row_l[r] = l;
+    }
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+  constexpr int kVec = HD / 4;
+  for (int i = tid; i < G * kVec; i += kThreads) {
+    const int r = i / kVec, d = (i - r * kVec) * 4;
+    const float* src = p.part_o + (row0 + static_cast<int64_t>(r) * S) * HD + d;
+    float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+    for (int s0 = 0; s0 < S; s0 += 8) {
+      float4 x[8];
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // an empty split published no rows: its memory must not be read into the sum
+        f[j] = s0 + j < S ? fac[r * S + s0 + j] : 0.f;
+        x[j] = f[j] != 0.f ? __ldcg(reinterpret_cast<const float4*>(
+                                 src + static_cast<int64_t>(s0 + j) * HD))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        a0 += f[j] * x[j].x;
+        a1 += f[j] * x[j].y;
+        a2 += f[j] * x[j].z;
+        a3 += f[j] * x[j].w;
+      }
+    }
+    float m = row_m[r], l = row_l[r];
+    const int head = kvh * G + r;
+    float by = p.sinks ? apply_sink(m, l, p.sinks[head] * 1.4426950408889634f) : 1.f;
+    by = l > 0.f || l != l ? by / l : 0.f;
+    uint2 y;
+    y.x = pack_bf16x2(a0 * by, a1 * by);
+    y.y = pack_bf16x2(a2 * by, a3 * by);
+    *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(user) * p.out_row_stride + head * HD + d) = y;
+  }
+}
+
 template <int HD, int BS, int FMT, int NG, int STAGES>
 __global__ void __launch_bounds__(kDecThreads)
 paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
@@ -120,7 +205,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
         p.part_ml[row] = make_float2(-INFINITY, 0.f);
       }
       if (p.tickets && threadIdx.x < kDecConsumerWarps * 32)
-        decode_split_finish<HD>(p, user, kvh, reinterpret_cast<float*>(ring), threadIdx.x);
+        decode_scaled_finish<HD>(p, user, kvh, reinterpret_cast<float*>(ring), threadIdx.x);
     } else {
       for (int i = threadIdx.x; i < G * HD; i += blockDim.x) {
         const int r = i / HD, d = i - r * HD;
@@ -318,9 +403,12 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       const float lvs = __log2f(sc.y);
 
       // ---- S^T = K Q^T: rows = 16 tokens, columns = query heads
-      float s[NG][4];
+      // (two accumulators: half the length of the chain of dependent MMAs)
+      float s[NG][4], s2[NG][4];
 #pragma unroll
-      for (int ng = 0; ng < NG; ++ng) s[ng][0] = s[ng][1] = s[ng][2] = s[ng][3] = 0.f;
+      for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[ng][i] = s2[ng][i] = 0.f;
 #pragma unroll
       for (int cp = 0; cp < HD / 32; ++cp) {
         uint32_t b[4];
@@ -333,7 +421,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
           codes_to_f16<FMT>(b[2 * h + 1], a[1], a[3]);
 #pragma unroll
           for (int ng = 0; ng < NG; ++ng)
-            mma_f16_16816(s[ng], a, qf[ng][2 * cp + h][0], qf[ng][2 * cp + h][1]);
+            mma_f16_16816(h ? s2[ng] : s[ng], a, qf[ng][2 * cp + h][0], qf[ng][2 * cp + h][1]);
         }
       }
 
@@ -343,7 +431,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       for (int ng = 0; ng < NG; ++ng) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[ng][i] *= qs[ng][i & 1] * sc.x;
+          s[ng][i] = (s[ng][i] + s2[ng][i]) * (qs[ng][i & 1] * sc.x);
           if (tail) {
             const int j = tok0 + g + (i >> 1) * 8;
             if (j >= ctx || j < lo) s[ng][i] = -INFINITY;
@@ -429,7 +517,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   float* sr = sm + kDecConsumerWarps * 8 * NG;                      // [4][8 NG] max of s - m + log2 vs
   float* sl = sr + kDecConsumerWarps * 8 * NG;                      // [4][8 NG] sum
   static_assert(kDecConsumerWarps * 8 * NG * (kRow + 3) * 4 <= L::kRingBytes, "merge scratch fits");
-  static_assert((32 * kDecMaxSplits + 40) * 4 <= L::kRingBytes, "split merge scratch fits");
+  static_assert((16 * kDecMaxSplits + 40) * 4 <= L::kRingBytes, "split merge scratch fits");
 #pragma unroll
   for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
@@ -473,7 +561,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
   }
   if (p.num_splits > 1 && p.tickets)
-    decode_split_finish<HD>(p, user, kvh, reinterpret_cast<float*>(ring), threadIdx.x);
+    decode_scaled_finish<HD>(p, user, kvh, reinterpret_cast<float*>(ring), threadIdx.x);
 }
 
 }  // namespace b200attn

@@ -11,7 +11,7 @@
 //
 // HBM-bound: each row is read once and written once.  One CTA per token; a head is held by
 // HD / 8 neighbouring lanes (16 bytes each), so the sum of squares is a few shuffles and the
-// rotation partner is a lane of the same warp: no shared memory but the token's cos / sin row.
+// rotation partner is in the same thread or warp: no shared memory but the token's cos / sin row.
 #pragma once
 #include "kv_scatter.cuh"
 
@@ -59,17 +59,66 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4 v, float (&x)[8]) {
 constexpr int kNrThreads = 256;
 constexpr int kNrPrefetch = 3;   // head slices a thread loads before it needs the cos / sin row
 
-template <int HD>
-__global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const QkNormRopeParams p) {
+// How a head lies in its HD / 8 lanes (lane li of the head) and where a rotation partner is:
+//   kNrSplit      NeoX, whole head rotated: elements 4 li .. + 3 and HD/2 + 4 li .. + 3, two 8-byte
+//                 accesses; both halves of a pair are in one thread
+//   kNrShuffle    NeoX, part of the head rotated: elements 8 li .. + 7; the partner is a lane away
+//   kNrAdjacent   interleaved: elements 8 li .. + 7, pairs of neighbours
+// (8192 tokens of 32 + 8 heads of 128: kNrSplit MEASURE_SPLIT us, the same through kNrShuffle
+// MEASURE_SHUFFLE us: eight shuffles per thread and head.)
+enum NrLayout : int { kNrSplit = 0, kNrShuffle = 1, kNrAdjacent = 2 };
+
+template <int HD, int LAYOUT>
+__global__ void __launch_bounds__(kNrThreads, 4) qk_norm_rope_kernel(const QkNormRopeParams p) {
   constexpr int kLanes = HD / 8;                    // lanes per head
   constexpr int kHeadsPerPass = kNrThreads / kLanes;
-  __shared__ float cs[HD / 2];
-  __shared__ float sn[HD / 2];
+  constexpr int kAngles = LAYOUT == kNrShuffle ? 8 : 4;      // that a thread needs
+  __shared__ float4 cs4[HD / 8];
+  __shared__ float4 sn4[HD / 8];
   const int64_t t = blockIdx.x;
   const int half = p.rotary_dim / 2;
-  const int li = threadIdx.x % kLanes;              // this lane's 8 elements: 8 li .. 8 li + 7
+  const int li = threadIdx.x % kLanes;
   const int h0 = threadIdx.x / kLanes;
+  const int nqk = p.num_q_heads + p.num_kv_heads;
+  const int all = nqk + (p.slot_mapping ? p.num_kv_heads : 0);   // q, k and (to be written) v heads
 
+  auto at = [&](const __nv_bfloat16* base, int64_t stride, int head) {
+    return base + t * stride + static_cast<int64_t>(head) * HD;
+  };
+  auto load = [&](int head) -> uint4 {
+    const __nv_bfloat16* src = head < p.num_q_heads ? at(p.q, p.q_stride, head)
+                               : head < nqk ? at(p.k, p.k_stride, head - p.num_q_heads)
+                                            : at(p.v, p.v_stride, head - nqk);
+    if (LAYOUT == kNrSplit) {
+      const uint2 a = *reinterpret_cast<const uint2*>(src + li * 4);
+      const uint2 b = *reinterpret_cast<const uint2*>(src + HD / 2 + li * 4);
+      return make_uint4(a.x, a.y, b.x, b.y);
+    }
+    return *reinterpret_cast<const uint4*>(src + li * 8);
+  };
+  auto store = [&](__nv_bfloat16* dst, const uint4 y) {
+    if (LAYOUT == kNrSplit) {
+      *reinterpret_cast<uint2*>(dst + li * 4) = make_uint2(y.x, y.y);
+      *reinterpret_cast<uint2*>(dst + HD / 2 + li * 4) = make_uint2(y.z, y.w);
+    } else {
+      *reinterpret_cast<uint4*>(dst + li * 8) = y;
+    }
+  };
+  uint4 pre[kNrPrefetch];
+#pragma unroll
+  for (int i = 0; i < kNrPrefetch; ++i) {
+    const int head = h0 + i * kHeadsPerPass;
+    pre[i] = head < all ? load(head) : make_uint4(0u, 0u, 0u, 0u);
+  }
+
+  if (threadIdx.x < half) {
+    const double turns = static_cast<double>(p.positions[t]) *
+                         static_cast<double>(p.inv_freq[threadIdx.x]) * 0.15915494309189535;
+    float s, c;
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+    reinterpret_cast<float*>(sn4)[threadIdx.x] = s;
+    reinterpret_cast<float*>(cs4)[threadIdx.x] = c;
+  }
   int64_t blk = -1;
   int off = 0;
   if (p.slot_mapping) {
@@ -83,62 +132,61 @@ __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const QkNormRo
       }
     }
   }
-  const int nqk = p.num_q_heads + p.num_kv_heads;
-  const int heads = nqk + (blk >= 0 ? p.num_kv_heads : 0);   // q, k and (when written) v heads
-
-  auto load = [&](int head) -> uint4 {
-    const __nv_bfloat16* src;
-    if (head < p.num_q_heads)
-      src = p.q + t * p.q_stride + static_cast<int64_t>(head) * HD;
-    else if (head < nqk)
-      src = p.k + t * p.k_stride + static_cast<int64_t>(head - p.num_q_heads) * HD;
-    else
-      src = p.v + t * p.v_stride + static_cast<int64_t>(head - nqk) * HD;
-    return *reinterpret_cast<const uint4*>(src + li * 8);
-  };
-  uint4 pre[kNrPrefetch];
-#pragma unroll
-  for (int i = 0; i < kNrPrefetch; ++i) {
-    const int head = h0 + i * kHeadsPerPass;
-    pre[i] = head < heads ? load(head) : make_uint4(0u, 0u, 0u, 0u);
-  }
-  float wq[8], wk[8];
-  if (p.weight_f32) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      wq[i] = static_cast<const float*>(p.q_weight)[li * 8 + i];
-      wk[i] = static_cast<const float*>(p.k_weight)[li * 8 + i];
+  auto store_cache = [&](uint8_t* cache, int h, const uint4 y) {
+    const int64_t row = ((blk * p.num_kv_heads + h) * p.block_size + off) * HD;
+    if (!p.cache_fp8) {
+      store(reinterpret_cast<__nv_bfloat16*>(cache) + row, y);
+      return;
     }
-  } else {
-    unpack_bf16x8(*(static_cast<const uint4*>(p.q_weight) + li), wq);
-    unpack_bf16x8(*(static_cast<const uint4*>(p.k_weight) + li), wk);
-  }
-  if (threadIdx.x < half) {
-    const double turns = static_cast<double>(p.positions[t]) *
-                         static_cast<double>(p.inv_freq[threadIdx.x]) * 0.15915494309189535;
-    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn[threadIdx.x], &cs[threadIdx.x]);
-  }
+    const uint2 c = bf16x8_to_e4m3x8(y);
+    if (LAYOUT == kNrSplit) {
+      *reinterpret_cast<uint32_t*>(cache + row + li * 4) = c.x;
+      *reinterpret_cast<uint32_t*>(cache + row + HD / 2 + li * 4) = c.y;
+    } else {
+      *reinterpret_cast<uint2*>(cache + row + li * 8) = c;
+    }
+  };
   __syncthreads();
 
-  // This lane's part in the rotation.  NeoX: lanes [0, r/16) hold the a's, [r/16, r/8) the b's.
+  // This thread's part in the rotation: which angles, and (kNrShuffle) which lane is the partner:
+  // lanes [0, r/16) of a head hold the a's, [r/16, r/8) the b's.
   const int pair_lanes = half / 8;
-  const bool rotates = li < 2 * pair_lanes;
-  const bool second = p.neox && li >= pair_lanes;
+  const bool rotates = LAYOUT == kNrSplit || li < 2 * pair_lanes;
+  const bool second = LAYOUT == kNrShuffle && li >= pair_lanes;
   const int lane = threadIdx.x & 31;
-  const int partner = rotates && p.neox ? (second ? lane - pair_lanes : lane + pair_lanes) : lane;
-  // angle index of element 0: NeoX 8 (li mod r/16), interleaved 4 li
-  const int a0 = rotates ? (p.neox ? (second ? li - pair_lanes : li) * 8 : li * 4) : 0;
+  const int partner = rotates ? (second ? lane - pair_lanes : lane + pair_lanes) : lane;
+  float c[kAngles], s[kAngles];
+#pragma unroll
+  for (int i = 0; i < kAngles; i += 4) {
+    float4 cv = make_float4(1.f, 1.f, 1.f, 1.f), sv = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rotates) {
+      const int v = LAYOUT == kNrShuffle ? (second ? li - pair_lanes : li) * 2 + i / 4 : li;
+      cv = cs4[v];
+      sv = sn4[v];
+    }
+    c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
+    s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
+  }
+  float w[8];
+  bool have_k = false;
+  auto load_weight = [&](const void* weight) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = LAYOUT == kNrSplit ? (i < 4 ? li * 4 + i : HD / 2 + li * 4 + i - 4) : li * 8 + i;
+      w[i] = p.weight_f32 ? __ldg(static_cast<const float*>(weight) + e)
+                          : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(weight) + e));
+    }
+  };
+  load_weight(p.q_weight);
 
   auto process = [&](int head, uint4 raw) {   // every lane of the warp comes here
     if (head >= nqk) {
-      if (head < heads) {
-        const int64_t dst =
-            ((blk * p.num_kv_heads + (head - nqk)) * p.block_size + off) * kLanes + li;
-        if (p.cache_fp8)
-          reinterpret_cast<uint2*>(p.v_cache)[dst] = bf16x8_to_e4m3x8(raw);
-        else
-          reinterpret_cast<uint4*>(p.v_cache)[dst] = raw;
-      }
+      if (head < all && blk >= 0) store_cache(p.v_cache, head - nqk, raw);
+    }
+    const bool is_k = head >= p.num_q_heads;
+    if (is_k && !have_k) {                    // heads come in ascending order: q, then k
+      load_weight(p.k_weight);
+      have_k = true;
     }
     float x[8];
     unpack_bf16x8(raw, x);
@@ -148,55 +196,49 @@ __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const QkNormRo
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float r = rsqrtf(ss * (1.f / HD) + p.eps);
-    const bool is_k = head >= p.num_q_heads;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (is_k ? wk[i] : wq[i]);
-    if (p.neox) {
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+    if (LAYOUT == kNrSplit) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = x[i], b = x[i + 4];
+        x[i] = a * c[i] - b * s[i];
+        x[i + 4] = b * c[i] + a * s[i];
+      }
+    } else if (LAYOUT == kNrShuffle) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float other = __shfl_sync(0xffffffffu, x[i], partner);
-        if (rotates) {
-          const float c = cs[a0 + i], s = sn[a0 + i];
-          x[i] = second ? x[i] * c + other * s : x[i] * c - other * s;
-        }
+        if (rotates) x[i] = second ? x[i] * c[i] + other * s[i] : x[i] * c[i] - other * s[i];
       }
     } else if (rotates) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float c = cs[a0 + i], s = sn[a0 + i];
         const float a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * c - b * s;
-        x[2 * i + 1] = b * c + a * s;
+        x[2 * i] = a * c[i] - b * s[i];
+        x[2 * i + 1] = b * c[i] + a * s[i];
       }
     }
     if (head >= nqk) return;
     const uint4 y = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
                                pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
     if (!is_k) {
-      *reinterpret_cast<uint4*>(p.q_out + t * p.q_out_stride + static_cast<int64_t>(head) * HD +
-                                li * 8) = y;
+      store(p.q_out + t * p.q_out_stride + static_cast<int64_t>(head) * HD, y);
       return;
     }
     const int h = head - p.num_q_heads;
-    *reinterpret_cast<uint4*>(p.k_out + t * p.k_out_stride + static_cast<int64_t>(h) * HD +
-                              li * 8) = y;
-    if (blk >= 0) {
-      const int64_t dst = ((blk * p.num_kv_heads + h) * p.block_size + off) * kLanes + li;
-      if (p.cache_fp8)
-        reinterpret_cast<uint2*>(p.k_cache)[dst] = bf16x8_to_e4m3x8(y);
-      else
-        reinterpret_cast<uint4*>(p.k_cache)[dst] = y;
-    }
+    store(p.k_out + t * p.k_out_stride + static_cast<int64_t>(h) * HD, y);
+    if (blk >= 0) store_cache(p.k_cache, h, y);
   };
 
   // the bound is rounded up to whole warps: all lanes of a warp take the shuffles together
   const int first_of_warp = (threadIdx.x & ~31) / kLanes;
 #pragma unroll
   for (int i = 0; i < kNrPrefetch; ++i)
-    if (first_of_warp + i * kHeadsPerPass < heads) process(h0 + i * kHeadsPerPass, pre[i]);
-  for (int b = kNrPrefetch * kHeadsPerPass; first_of_warp + b < heads; b += kHeadsPerPass) {
+    if (first_of_warp + i * kHeadsPerPass < all) process(h0 + i * kHeadsPerPass, pre[i]);
+  for (int b = kNrPrefetch * kHeadsPerPass; first_of_warp + b < all; b += kHeadsPerPass) {
     const int head = h0 + b;
-    process(head, head < heads ? load(head) : make_uint4(0u, 0u, 0u, 0u));
+    process(head, head < all ? load(head) : make_uint4(0u, 0u, 0u, 0u));
   }
 }
 

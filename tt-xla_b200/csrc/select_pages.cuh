@@ -18,8 +18,10 @@
 // whose fp32 score is within twice that of the border can be on the wrong side of it: these few
 // are summed again in fp64, and the border is drawn among them.
 //
-// One launch: the CTAs of a (user, KV head) each score a slice of the pages; the one that arrives
-// last (a ticket in the workspace) makes the choice.
+// One launch: one CTA per (user, KV head) when these fill the machine, else several that each score
+// a slice of the pages; the one that arrives last (a ticket in the workspace) makes the choice.
+// Choosing is a chain of block-wide counts, so it is a bisection that starts at the highest bit in
+// which the scores differ and ends as soon as the count is right.
 #pragma once
 #include "kv_scatter.cuh"
 
@@ -61,81 +63,66 @@ __device__ __forceinline__ unsigned long long ordered_key(double x) {
 
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelShared = 4096;     // pages whose scores stay in shared memory
 
 struct SelectShared {
-  unsigned int hist[256];
-  unsigned int warp_sum[kSelWarps];
+  float2 score[kSelShared];
+  unsigned int part[2][kSelWarps];   // a block sum, double-buffered: one barrier each
   float warp_err[kSelWarps];
-  unsigned int digit, left, count_sure, count_near;
+  unsigned int warp_lo[kSelWarps], warp_hi[kSelWarps];
+  unsigned int near_list[32];
+  unsigned long long near_key[32];
+  unsigned int near_count;
   int last;
 };
 
-// The k-th largest (k >= 1) of the keys key(i), i in [0, n) with use(i); at least k of them are
-// used.  Eight bits a pass from the top; all threads return the key.  `left` returns how many of
-// the keys equal to it belong to the k largest.
+// Sum over the block, the same for all threads; `turn` alternates the buffer.
+__device__ __forceinline__ unsigned int block_sum(SelectShared& sh, unsigned int v, unsigned int& turn) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  unsigned int* part = sh.part[turn & 1];
+  ++turn;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  unsigned int sum = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) sum += part[w];
+  return sum;
+}
+
+// The k-th largest (k >= 1, at least k keys) of the keys get(i), i in [0, n) with use(i), by
+// bisection from `top` (the highest bit the keys differ in; the bits above are `prefix`).  The
+// barrier per step is what a step costs, so it ends as soon as exactly k keys are at least as large
+// as the candidate: `border` is then such a candidate, not a key.
 template <typename Key, typename Use, typename Get>
-__device__ Key kth_largest(SelectShared& sh, int n, unsigned int k, Use use, Get get,
-                           unsigned int* left) {
-  Key prefix = 0, mask = 0;
-  for (int shift = static_cast<int>(sizeof(Key)) * 8 - 8; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelThreads) sh.hist[i] = 0u;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kSelThreads) {
-      if (!use(i)) continue;
-      const Key v = get(i);
-      if ((v & mask) == prefix) atomicAdd(&sh.hist[(v >> shift) & 255], 1u);
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      // lane l owns digits 255 - 8 l .. 248 - 8 l, from the top
-      unsigned int h[8], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        h[j] = sh.hist[255 - 8 * static_cast<int>(threadIdx.x) - j];
-        sum += h[j];
-      }
-      unsigned int above = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned int up = __shfl_up_sync(0xffffffffu, above, o);
-        if (static_cast<int>(threadIdx.x) >= o) above += up;
-      }
-      above -= sum;
-      if (above < k && k <= above + sum) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (above < k && k <= above + h[j]) {
-            sh.digit = 255 - 8 * threadIdx.x - j;
-            sh.left = k - above;
-          }
-          above += h[j];
-        }
-      }
-    }
-    __syncthreads();
-    prefix |= static_cast<Key>(sh.digit) << shift;
-    mask |= static_cast<Key>(255) << shift;
-    k = sh.left;
-    __syncthreads();
+__device__ Key kth_border(SelectShared& sh, int n, unsigned int k, Key prefix, int top, Use use,
+                          Get get, unsigned int& turn) {
+  for (int bit = top; bit >= 0; --bit) {
+    const Key cand = prefix | (static_cast<Key>(1) << bit);
+    unsigned int c = 0;
+    for (int i = threadIdx.x; i < n; i += kSelThreads) c += use(i) && get(i) >= cand;
+    c = block_sum(sh, c, turn);
+    if (c >= k) prefix = cand;
+    if (c == k) break;
   }
-  *left = k;
   return prefix;
 }
 
 // Exclusive position of each set flag in thread order, and the number of flags (all threads call).
-__device__ __forceinline__ unsigned int block_rank(SelectShared& sh, bool flag, unsigned int* total) {
+__device__ __forceinline__ unsigned int block_rank(SelectShared& sh, bool flag, unsigned int* total,
+                                                   unsigned int& turn) {
   const unsigned int b = __ballot_sync(0xffffffffu, flag);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) sh.warp_sum[warp] = __popc(b);
+  unsigned int* part = sh.part[turn & 1];
+  ++turn;
+  if (lane == 0) part[warp] = __popc(b);
   __syncthreads();
   unsigned int before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kSelWarps; ++w) {
-    const unsigned int c = sh.warp_sum[w];
+    const unsigned int c = part[w];
     before += w < warp ? c : 0u;
     all += c;
   }
-  __syncthreads();
   *total = all;
   return before + __popc(b & ((1u << lane) - 1u));
 }
@@ -192,7 +179,10 @@ __global__ void __launch_bounds__(kSelThreads) select_pages_kernel(const SelectP
   const int num_slices = (n + p.slice - 1) / p.slice;
   const int arrivals = min(num_slices, static_cast<int>(gridDim.x));
   if (static_cast<int>(blockIdx.x) >= num_slices) return;   // beyond the context: takes no ticket
+  // One CTA for all pages keeps the scores to itself; else they go through global memory.
+  const bool shared_scores = n <= kSelShared;
   float2* score = p.score + uh * p.max_pages;
+  float2* put = arrivals == 1 && shared_scores ? sh.score : score;
   const int g = lane >> 2, tq = lane & 3;
   {
     // Q fragments (B operand: columns = query heads 8 ng + g): positive and negative part.  The
@@ -291,70 +281,123 @@ __global__ void __launch_bounds__(kSelThreads) select_pages_kernel(const SelectP
           mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
         }
         if (tq == 0 && rows[r] < end)
-          score[rows[r]] = ok[r] ? make_float2(best, mag * (4.f * HD / 8388608.f))
+          put[rows[r]] = ok[r] ? make_float2(best, mag * (4.f * HD / 8388608.f))
                                  : make_float2(-INFINITY, 0.f);
       }
     }
   }
 
   // ---------------------------------------------------------------- the last CTA chooses
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0)
-    sh.last = atomicAdd(p.tickets + uh, 1u) == static_cast<unsigned int>(arrivals - 1);
-  __syncthreads();
-  if (!sh.last) return;
-  __threadfence();
-  if (threadIdx.x == 0) {
-    p.tickets[uh] = 0u;              // leave the counter as the next launch expects it
-    sh.count_sure = sh.count_near = 0u;
+  if (arrivals > 1) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0)
+      sh.last = atomicAdd(p.tickets + uh, 1u) == static_cast<unsigned int>(arrivals - 1);
+    __syncthreads();
+    if (!sh.last) return;
+    __threadfence();
+    if (threadIdx.x == 0) p.tickets[uh] = 0u;    // leave the counter as the next launch expects it
+    if (shared_scores)
+      for (int i = threadIdx.x; i < n; i += kSelThreads) sh.score[i] = __ldcg(score + i);
   }
   const int e0 = p.keep_first, m = n - p.keep_last - p.keep_first;   // candidates e0 .. e0 + m - 1
   const unsigned int want = static_cast<unsigned int>(p.num_pages - p.keep_first - p.keep_last);
   unsigned long long* exact = p.exact + uh * p.max_pages;
-  const float2* sc = score + e0;
+  auto score_of = [&](int page) { return shared_scores ? sh.score[page] : __ldcg(score + page); };
   constexpr unsigned long long kPicked = ~0ull;
+  unsigned int turn = 0;
 
   float border = INFINITY, width = 0.f;
   bool take_all_near = true;
+  if (threadIdx.x == 0) sh.near_count = 0u;
   __syncthreads();
   if (want > 0) {
     float err = 0.f;
-    for (int i = threadIdx.x; i < m; i += kSelThreads) err = fmaxf(err, __ldcg(sc + i).y);
+    unsigned int lo = ~0u, hi = 0u;
+    for (int i = threadIdx.x; i < m; i += kSelThreads) {
+      const float2 v = score_of(e0 + i);
+      err = fmaxf(err, v.y);
+      const uint32_t key = ordered_key(v.x);
+      lo = min(lo, key);
+      hi = max(hi, key);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
-    if (lane == 0) sh.warp_err[warp] = err;
-    unsigned int left;
-    const uint32_t key = kth_largest<uint32_t>(
-        sh, m, want, [](int) { return true; },
-        [&](int i) { return ordered_key(__ldcg(sc + i).x); }, &left);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      sh.warp_err[warp] = err;
+      sh.warp_lo[warp] = lo;
+      sh.warp_hi[warp] = hi;
+    }
+    __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) err = fmaxf(err, sh.warp_err[w]);
-    border = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    for (int w = 0; w < kSelWarps; ++w) {
+      err = fmaxf(err, sh.warp_err[w]);
+      lo = min(lo, sh.warp_lo[w]);
+      hi = max(hi, sh.warp_hi[w]);
+    }
+    // the keys share the bits above the highest one in which the least and the greatest differ
+    const int top = lo == hi ? -1 : 31 - __clz(lo ^ hi);
+    const uint32_t prefix = lo == hi ? lo : top == 31 ? 0u : lo & ~((2u << top) - 1u);
+    const uint32_t at = kth_border<uint32_t>(
+        sh, m, want, prefix, top, [](int) { return true; },
+        [&](int i) { return ordered_key(score_of(e0 + i).x); }, turn);
+    // the border score: the least of the keys that are >= `at`
+    uint32_t least = ~0u;
+    for (int i = threadIdx.x; i < m; i += kSelThreads) {
+      const uint32_t key = ordered_key(score_of(e0 + i).x);
+      if (key >= at) least = min(least, key);
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    __syncthreads();
+    if (lane == 0) sh.warp_lo[warp] = least;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelWarps; ++w) least = min(least, sh.warp_lo[w]);
+    border = __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
     // both the page's and the border's score may be off by err; the difference is rounded once
     width = 2.f * err * 1.000001f;
     // above: surely among the `want` best; near: may be on either side
-    unsigned int sure = 0, near = 0;
+    auto is_near = [&](int i) {
+      const float s = score_of(e0 + i).x;
+      return s == border || fabsf(s - border) <= width;
+    };
+    unsigned int counts = 0, near_mine = 0;              // sure ones; near ones
     for (int i = threadIdx.x; i < m; i += kSelThreads) {
-      const float s = __ldcg(sc + i).x;
-      const bool is_near = s == border || fabsf(s - border) <= width;
-      sure += !is_near && s > border;
-      near += is_near;
+      const bool n_i = is_near(i);
+      near_mine += n_i;
+      counts += !n_i && score_of(e0 + i).x > border;
+      if (n_i) {
+        const unsigned int slot = atomicAdd(&sh.near_count, 1u);
+        if (slot < 32u) sh.near_list[slot] = static_cast<unsigned int>(i);
+      }
     }
-    sure = __reduce_add_sync(0xffffffffu, sure);
-    near = __reduce_add_sync(0xffffffffu, near);
-    if (lane == 0) {
-      atomicAdd(&sh.count_sure, sure);
-      atomicAdd(&sh.count_near, near);
-    }
-    __syncthreads();
-    const unsigned int open = want - sh.count_sure;      // places for the near ones
-    take_all_near = open == sh.count_near;
-    if (!take_all_near) {
-      auto is_near = [&](int i) {
-        const float s = __ldcg(sc + i).x;
-        return s == border || fabsf(s - border) <= width;
-      };
+    const unsigned int sure = block_sum(sh, counts, turn);
+    const unsigned int near = block_sum(sh, near_mine, turn);
+    const unsigned int open = want - sure;               // places for the near ones
+    take_all_near = open == near;
+    if (!take_all_near && near <= 32u) {
+      // a handful: exact scores, and each one's rank among them
+      for (unsigned int j = warp; j < near; j += kSelWarps) {
+        const int i = static_cast<int>(sh.near_list[j]);
+        const int64_t blk = pt[e0 + i];
+        const bool ok = blk >= 0 && blk < p.num_blocks;
+        const double v = ok ? exact_page_score<HD>(p, user, kvh, blk, lane) : -INFINITY;
+        if (lane == 0) sh.near_key[j] = ordered_key(v);
+      }
+      __syncthreads();
+      if (threadIdx.x < near) {
+        const unsigned long long key = sh.near_key[threadIdx.x];
+        const unsigned int mine = sh.near_list[threadIdx.x];
+        unsigned int rank = 0;
+        for (unsigned int j = 0; j < near; ++j)
+          rank += sh.near_key[j] > key || (sh.near_key[j] == key && sh.near_list[j] < mine);
+        exact[e0 + mine] = rank < open ? kPicked : 0ull;
+      }
+      __syncthreads();
+    } else if (!take_all_near) {
+      // many (equal pages): the same choice by bisection on the exact scores
       for (int i = warp; i < m; i += kSelWarps) {
         if (!is_near(i)) continue;                       // uniform in the warp
         const int64_t blk = pt[e0 + i];
@@ -363,19 +406,21 @@ __global__ void __launch_bounds__(kSelThreads) select_pages_kernel(const SelectP
         if (lane == 0) exact[e0 + i] = ordered_key(v);
       }
       __syncthreads();
-      unsigned int ties;
-      const unsigned long long at = kth_largest<unsigned long long>(
-          sh, m, open, is_near, [&](int i) { return exact[e0 + i]; }, &ties);
-      // mark the chosen ones; of the keys equal to the border's the first `ties`
+      const unsigned long long edge = kth_border<unsigned long long>(
+          sh, m, open, 0ull, 63, is_near, [&](int i) { return exact[e0 + i]; }, turn);
+      unsigned int above = 0;
+      for (int i = threadIdx.x; i < m; i += kSelThreads) above += is_near(i) && exact[e0 + i] > edge;
+      above = block_sum(sh, above, turn);
+      // mark the chosen ones: all above the edge, and of those on it the first `open - above`
       unsigned int before = 0;
       for (int i0 = 0; i0 < m; i0 += kSelThreads) {
         const int i = i0 + threadIdx.x;
         const bool here = i < m && is_near(i);
         const unsigned long long v = here ? exact[e0 + i] : 0ull;
         unsigned int total;
-        const unsigned int rank = before + block_rank(sh, here && v == at, &total);
+        const unsigned int rank = before + block_rank(sh, here && v == edge, &total, turn);
         before += total;
-        if (here) exact[e0 + i] = v > at || (v == at && rank < ties) ? kPicked : 0ull;
+        if (here) exact[e0 + i] = v > edge || (v == edge && rank + above < open) ? kPicked : 0ull;
       }
       __syncthreads();
     }
@@ -387,13 +432,14 @@ __global__ void __launch_bounds__(kSelThreads) select_pages_kernel(const SelectP
     const int i = i0 + threadIdx.x;
     bool take = i < e0 || (i >= n - p.keep_last && i < n);
     if (i >= e0 && i < e0 + m && want > 0) {
-      const float s = __ldcg(score + i).x;
+      const float s = score_of(i).x;
       const bool is_near = s == border || fabsf(s - border) <= width;
       take = is_near ? take_all_near || exact[i] == kPicked : s > border;
     }
+    const int32_t id = i < n ? pt[i] : 0;
     unsigned int total;
-    const unsigned int at = filled + block_rank(sh, take, &total);
-    if (take && at < static_cast<unsigned int>(p.num_pages)) table[at] = pt[i];
+    const unsigned int at = filled + block_rank(sh, take, &total, turn);
+    if (take && at < static_cast<unsigned int>(p.num_pages)) table[at] = id;
     filled += total;
   }
   if (threadIdx.x == 0) p.out_pos[uh] = (p.num_pages - 1) * BS + in_page;
