@@ -24,6 +24,7 @@
 
 #ifndef B200ATTN_DS_STAGES
 #define B200ATTN_DS_STAGES 3
+#define B200ATTN_DS_STAGES64 4
 #endif
 namespace b200attn {
 
@@ -294,7 +295,7 @@ static int launch_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, const
 template <int HD, int BS, int FMT, int NG>
 static int launch_decode_scaled(const CUtensorMap& tk, const CUtensorMap& tv,
                                 const DecodeScaledParams& p, int num_users, cudaStream_t s) {
-  constexpr int kStages = HD == 128 ? B200ATTN_DS_STAGES : 6;
+  constexpr int kStages = HD == 128 ? B200ATTN_DS_STAGES : B200ATTN_DS_STAGES64;
   using L = DecodeScaledSmem<HD, BS, kStages>;
   auto kern = paged_decode_scaled_kernel<HD, BS, FMT, NG, kStages>;
   static bool smem_allowed[kMaxDevices] = {};
@@ -1009,7 +1010,7 @@ int b200attn_qk_norm_rope_kv_scatter_slots(
   p.slot_mapping = slot_mapping;
   p.num_q_heads = num_q_heads;
   p.num_kv_heads = num_kv_heads;
-  p.block_size = block_size;
+  p.log2_block_size = block_size == 64 ? 6 : 5;
   p.num_blocks = num_blocks;
   p.err_word = dev->err_word;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

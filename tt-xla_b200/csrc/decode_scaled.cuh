@@ -6,7 +6,7 @@
 //
 // HBM-bound: a key and value cost 2 * head_size bytes and are read once.  As in the bf16 kernel a
 // CTA owns one KV head of one user (and a slice of the context), a producer warp keeps a ring of
-// 64-token tiles full with TMA, and four warps take 16 tokens of a tile each.  What differs:
+// tiles full with TMA, and four warps take a quarter of a tile each.  What differs:
 //   * the products are transposed: S^T = K Q^T and O^T = V^T P^T, tokens resp. head elements in
 //     the 16 rows of m16n8k16 and the query heads in its 8 columns.  Up to 8 query heads per KV
 //     head then fill an MMA (otherwise half of the 16 rows would be padding), and the
@@ -22,7 +22,10 @@
 //     any size leave the scale its bits): the f16 weights are then at most 2^8 whatever the scales
 //     are, and a page's values keep 11 bits next to pages whose scale is far larger but whose
 //     weight is small.  The row sum uses 2^(s - m), in fp32, unrounded;
-//   * the maxima are raised only when a score passes them by more than 2^8 (one vote per 16
+//   * a tile is 128 tokens, 32 per warp in two halves of 16 that share one page (and its scales),
+//     one vote and one set of waits: with 8-bit keys the issue slots and the length of the chain
+//     load - widen - MMA - softmax - MMA bound a warp, not the bytes;
+//   * the maxima are raised only when a score passes them by more than 2^8 (one vote per 32
 //     tokens instead of six shuffles); until then weights may be up to 2^8, which f16 and the
 //     fp32 sums hold without loss;
 //   * q is scaled by a power of two per head to at most 1 before it is rounded to f16.
@@ -40,14 +43,17 @@ struct DecodeScaledParams {
   const float* v_scale;
 };
 
+constexpr int kDsTile = 128;           // tokens per pipeline stage
+constexpr int kDsWarpTokens = 32;      // of them per consumer warp
+
 template <int HD, int BS, int STAGES>
 struct DecodeScaledSmem {
-  static constexpr int kPages = kDecTile / BS;
+  static constexpr int kPages = kDsTile / BS;
   static constexpr int kBoxBytes = BS * HD;                    // one page of one head
   static constexpr int kTensorBytes = kPages * kBoxBytes;      // K (or V) of one tile
   static constexpr int kStageBytes = 2 * kTensorBytes;
   static constexpr int kRingBytes = STAGES * kStageBytes;
-  static constexpr int kScaleBytes = STAGES * kPages * 8;      // (K scale, V scale) per page
+  static constexpr int kScaleBytes = STAGES * kPages * 8;      // (K scale, log2 of the V scale)
   static constexpr int kBarrierBytes = 2 * STAGES * 8 + 16;
   static constexpr int kTotalBytes = kRingBytes + kScaleBytes + kBarrierBytes + 1024;
 };
@@ -189,8 +195,8 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
 
   const int ctx = decode_cur_pos(p, user, kvh) + 1;  // keys 0 .. cur_pos
   const int lo = (p.window > 0 && ctx > p.window) ? ctx - p.window : 0;   // first key attended
-  const int n_tiles = ctx > 0 ? (ctx + kDecTile - 1) / kDecTile : 0;
-  const int t_lo = lo / kDecTile;
+  const int n_tiles = ctx > 0 ? (ctx + kDsTile - 1) / kDsTile : 0;
+  const int t_lo = lo / kDsTile;
   const int tiles_per_split = (n_tiles - t_lo + p.num_splits - 1) / p.num_splits;
   const int t_begin = t_lo + split * tiles_per_split;
   const int t_end = min(n_tiles, t_begin + tiles_per_split);
@@ -239,7 +245,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     // fetched early, so only the first tiles wait for a page's scales.
     struct Window {
       int id;
-      float ks, vs;
+      float ks, vs;     // K scale, log2 of the V scale
     };
     auto fetch = [&](int base) {
       Window w;
@@ -248,7 +254,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       const bool ok = w.id >= 0 && w.id < p.num_blocks;
       const int64_t at = ok ? static_cast<int64_t>(w.id) * p.num_kv_heads + kvh : kvh;
       w.ks = __ldg(sp.k_scale + at);
-      w.vs = __ldg(sp.v_scale + at);
+      w.vs = __log2f(__ldg(sp.v_scale + at));
       return w;
     };
     int win_base = t_begin * L::kPages;
@@ -260,12 +266,16 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
         nxt = fetch(win_base + 32);
       }
     };
-    // the loads of a tile (the stage's barrier takes their bytes before it is armed ...)
+    // the loads of a tile's pages, not of those past the context (the stage's barrier takes their
+    // bytes before it is armed ...)
+    auto pages_of = [&](int t) { return min(L::kPages, n_pages - t * L::kPages); };
     auto load_tile = [&](int t, int stage) {
+      const int live = pages_of(t);
       uint8_t* kdst = ring + stage * L::kStageBytes;
       uint8_t* vdst = kdst + L::kTensorBytes;
 #pragma unroll
       for (int pg = 0; pg < L::kPages; ++pg) {
+        if (pg >= live) break;
         const int page_idx = t * L::kPages + pg;
         advance(page_idx);
         int64_t blk = __shfl_sync(0xffffffffu, cur.id, page_idx - win_base);
@@ -282,14 +292,16 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     };
     // (... here) and its scales
     auto arm_tile = [&](int t, int stage) {
+      const int live = pages_of(t);
 #pragma unroll
       for (int pg = 0; pg < L::kPages; ++pg) {
+        if (pg >= live) break;
         const int page_idx = t * L::kPages + pg;
         const float ks = __shfl_sync(0xffffffffu, cur.ks, page_idx - win_base);
         const float vs = __shfl_sync(0xffffffffu, cur.vs, page_idx - win_base);
         if (lane == 0) scales[stage * L::kPages + pg] = make_float2(ks, vs);
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], L::kStageBytes);
+      if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], live * 2 * L::kBoxBytes);
     };
     // First fill: all loads go out before anything waits for a scale (all of these pages are in
     // the first window).
@@ -310,6 +322,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   // -------------------------------------------------------------------- consumer warps
   const int g = lane >> 2;
   const int tq = lane & 3;
+  static_assert(kDecConsumerWarps * kDsWarpTokens == kDsTile && BS % kDsWarpTokens == 0, "");
 
   // Q fragments (B operand, columns = query heads 8 ng + g; heads >= G are zero).  Within the
   // 16 elements of k-step ks the thread holds 4tq .. 4tq+3; slots {2tq, 2tq+1} take elements 0
@@ -367,92 +380,112 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   }
 
   // Per-lane ldmatrix addressing inside a tile: token t's head_size bytes start at t * HD; 128-byte
-  // rows, 16-byte chunks XOR-swizzled with the row's low three bits.  Matrix lane / 8: token half
+  // rows, 16-byte chunks XOR-swizzled with the row's low three bits (the two halves of a warp's
+  // tokens are a multiple of 8 rows apart: same swizzle).  Matrix lane / 8: token half of the 16
   // (bit 0) and chunk of a pair (bit 1), for K and for V.
   const int lm = lane >> 3, lr = lane & 7;
-  const int tok = warp * 16 + (lm & 1) * 8 + lr;
+  const int tok = warp * kDsWarpTokens + (lm & 1) * 8 + lr;
   const uint32_t row = static_cast<uint32_t>(tok * HD) >> 7;
-  const uint32_t row_off = row << 7, row_sw = row & 7;
   const uint32_t chunk0 = ((static_cast<uint32_t>(tok * HD) & 127u) >> 4) + (lm >> 1);
+  uint32_t at[HD / 32];
+#pragma unroll
+  for (int cp = 0; cp < HD / 32; ++cp) at[cp] = (row << 7) + (((chunk0 + 2 * cp) ^ (row & 7)) << 4);
+  constexpr uint32_t kHalf = 16 * HD;      // bytes from a warp's first 16 tokens to its second
 
   for (int t = t_begin; t < t_end; ++t) {
     const int it = t - t_begin;
     const int stage = it % STAGES;
     mbar_wait(&full_bar[stage], (it / STAGES) & 1, abort_flag, p.err_word);
-    const uint32_t kbase = smem_u32(ring + stage * L::kStageBytes) + row_off;
+    const uint32_t kbase = smem_u32(ring + stage * L::kStageBytes);
     const uint32_t vbase = kbase + L::kTensorBytes;
-    const int tok0 = t * kDecTile + warp * 16;   // first token of this warp's slice
+    const int tok0 = t * kDsTile + warp * kDsWarpTokens;   // first token of this warp's slice
 
-    if (tok0 < ctx && tok0 + 16 > lo) {       // at least one of this warp's keys is attended
-      const bool tail = (tok0 + 16 > ctx) || (tok0 < lo);
+    if (tok0 < ctx && tok0 + kDsWarpTokens > lo) {  // at least one of this warp's keys is attended
+      const bool tail = (tok0 + kDsWarpTokens > ctx) || (tok0 < lo);
       if (tail && FMT != kPageInt8) {
         // Rows past the context may hold NaN codes: zero them, 0 * NaN would reach the sums.
-        const uint32_t v0 = smem_u32(ring + stage * L::kStageBytes) + L::kTensorBytes;
-        for (int i = lane; i < 16 * (HD / 16); i += 32) {
-          const int r = warp * 16 + i / (HD / 16), c = i % (HD / 16);
-          if (t * kDecTile + r >= ctx) {
+        for (int i = lane; i < kDsWarpTokens * (HD / 16); i += 32) {
+          const int r = warp * kDsWarpTokens + i / (HD / 16), c = i % (HD / 16);
+          if (t * kDsTile + r >= ctx) {
             const uint32_t b = static_cast<uint32_t>(r * HD + c * 16);
-            const uint32_t a = v0 + (b & ~127u) + ((((b >> 4) & 7u) ^ ((b >> 7) & 7u)) << 4);
+            const uint32_t a = vbase + (b & ~127u) + ((((b >> 4) & 7u) ^ ((b >> 7) & 7u)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
           }
         }
         fence_proxy_async_smem();  // the next TMA write to this stage follows generic writes
         __syncwarp();
       }
-      const float2 sc = scales[stage * L::kPages + (warp * 16) / BS];   // 16 tokens: one page
-      const float lvs = __log2f(sc.y);
+      const float2 sc = scales[stage * L::kPages + (warp * kDsWarpTokens) / BS];   // one page
 
       // ---- S^T = K Q^T: rows = 16 tokens, columns = query heads
-      // (two accumulators: half the length of the chain of dependent MMAs)
-      float s[NG][4], s2[NG][4];
+      float s[2][NG][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng)
+          s[u][ng][0] = s[u][ng][1] = s[u][ng][2] = s[u][ng][3] = 0.f;
+#pragma unroll
+      for (int cp = 0; cp < HD / 32; ++cp)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t b[4];
+          ldmatrix_x4(b, kbase + at[cp] + u * kHalf);
+          // b[0]: tokens 0-7, b[1]: tokens 8-15 of chunk 2cp; b[2], b[3]: of chunk 2cp+1
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a[4];
+            codes_to_f16<FMT>(b[2 * h], a[0], a[2]);
+            codes_to_f16<FMT>(b[2 * h + 1], a[1], a[3]);
+#pragma unroll
+            for (int ng = 0; ng < NG; ++ng)
+              mma_f16_16816(s[u][ng], a, qf[ng][2 * cp + h][0], qf[ng][2 * cp + h][1]);
+          }
+        }
+
+      // ---- scores in log2 units; s[u][ng][i]: token 16 u + g + 8 (i / 2), head 8 ng + 2 tq + i % 2
+#pragma unroll
+      for (int ng = 0; ng < NG; ++ng) {
+        const float f[2] = {qs[ng][0] * sc.x, qs[ng][1] * sc.x};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[u][ng][i] *= f[i & 1];
+      }
+      if (tail) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = tok0 + u * 16 + g + (i >> 1) * 8;
+            if (j >= ctx || j < lo)
+#pragma unroll
+              for (int ng = 0; ng < NG; ++ng) s[u][ng][i] = -INFINITY;
+          }
+      }
+      // the exponents' largest: d = s - m of the sum, d + log2 vs - r of the weights
+      bool over = false;
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[ng][i] = s2[ng][i] = 0.f;
-#pragma unroll
-      for (int cp = 0; cp < HD / 32; ++cp) {
-        uint32_t b[4];
-        ldmatrix_x4(b, kbase + (((chunk0 + 2 * cp) ^ row_sw) << 4));
-        // b[0]: tokens 0-7, b[1]: tokens 8-15 of chunk 2cp; b[2], b[3]: of chunk 2cp+1
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a[4];
-          codes_to_f16<FMT>(b[2 * h], a[0], a[2]);
-          codes_to_f16<FMT>(b[2 * h + 1], a[1], a[3]);
-#pragma unroll
-          for (int ng = 0; ng < NG; ++ng)
-            mma_f16_16816(h ? s2[ng] : s[ng], a, qf[ng][2 * cp + h][0], qf[ng][2 * cp + h][1]);
+        for (int j = 0; j < 2; ++j) {
+          const float d = fmaxf(fmaxf(s[0][ng][j], s[0][ng][j + 2]),
+                                fmaxf(s[1][ng][j], s[1][ng][j + 2])) - m[ng][j];
+          over |= d > kScoreSlack || d + sc.y > r[ng][j] + kScoreSlack;
         }
-      }
-
-      // ---- scores in log2 units; s[ng][i]: token g + 8 (i / 2), head 8 ng + 2 tq + i % 2
-      bool over = false;
-#pragma unroll
-      for (int ng = 0; ng < NG; ++ng) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[ng][i] = (s[ng][i] + s2[ng][i]) * (qs[ng][i & 1] * sc.x);
-          if (tail) {
-            const int j = tok0 + g + (i >> 1) * 8;
-            if (j >= ctx || j < lo) s[ng][i] = -INFINITY;
-          }
-          const float d = s[ng][i] - m[ng][i & 1];
-          over |= d > kScoreSlack || d + lvs > r[ng][i & 1] + kScoreSlack;
-        }
-      }
       if (__any_sync(0xffffffffu, over)) {      // raise the maxima
 #pragma unroll
         for (int ng = 0; ng < NG; ++ng) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float mx = fmaxf(s[ng][j], s[ng][j + 2]);
+            float mx = fmaxf(fmaxf(s[0][ng][j], s[0][ng][j + 2]),
+                             fmaxf(s[1][ng][j], s[1][ng][j + 2]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             const float mn = fmaxf(m[ng][j], mx), by = mn - m[ng][j];
             // r seen from the new m; kept finite, so that pages of zero values alone leave it so
             const float was = fmaxf(r[ng][j] - by, -FLT_MAX);
-            const float rn = fmaxf(was, (mx - mn) + lvs);
+            const float rn = fmaxf(was, (mx - mn) + sc.y);
             l[ng][j] *= fast_exp2(-by);
             const float f = fast_exp2(was - rn);
             m[ng][j] = mn;
@@ -466,35 +499,41 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
         }
       }
       // ---- P'^T as B operand: transposed 8x8 blocks, k = tokens, columns = heads
-      uint32_t pb[NG][2];
+      uint32_t pb[2][NG][2];
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng) {
-        float w[4];
+        const float add[2] = {sc.y - r[ng][0], sc.y - r[ng][1]};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float d = s[ng][i] - m[ng][i & 1];
-          l[ng][i & 1] += fast_exp2(d);
-          w[i] = fast_exp2(d + (lvs - r[ng][i & 1]));
+        for (int u = 0; u < 2; ++u) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float d = s[u][ng][i] - m[ng][i & 1];
+            l[ng][i & 1] += fast_exp2(d);
+            w[i] = fast_exp2(d + add[i & 1]);
+          }
+          pb[u][ng][0] = transpose_8x8(pack_f16x2(w[0], w[1]));
+          pb[u][ng][1] = transpose_8x8(pack_f16x2(w[2], w[3]));
         }
-        pb[ng][0] = transpose_8x8(pack_f16x2(w[0], w[1]));
-        pb[ng][1] = transpose_8x8(pack_f16x2(w[2], w[3]));
       }
 
       // ---- O^T += V^T P'^T: rows = the 16 head elements of a chunk (even ones, then odd ones)
 #pragma unroll
-      for (int cp = 0; cp < HD / 32; ++cp) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, vbase + (((chunk0 + 2 * cp) ^ row_sw) << 4));
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a[4];
-          codes_to_f16<FMT>(b[2 * h], a[0], a[1]);
-          codes_to_f16<FMT>(b[2 * h + 1], a[2], a[3]);
+        for (int cp = 0; cp < HD / 32; ++cp) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, vbase + at[cp] + u * kHalf);
 #pragma unroll
-          for (int ng = 0; ng < NG; ++ng)
-            mma_f16_16816(o[ng][2 * cp + h], a, pb[ng][0], pb[ng][1]);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a[4];
+            codes_to_f16<FMT>(b[2 * h], a[0], a[1]);
+            codes_to_f16<FMT>(b[2 * h + 1], a[2], a[3]);
+#pragma unroll
+            for (int ng = 0; ng < NG; ++ng)
+              mma_f16_16816(o[ng][2 * cp + h], a, pb[u][ng][0], pb[u][ng][1]);
+          }
         }
-      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty_bar[stage]);

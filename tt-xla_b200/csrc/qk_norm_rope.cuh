@@ -42,18 +42,16 @@ struct QkNormRopeParams {
   const int64_t* slot_mapping;   // NULL: no cache write
   int num_q_heads;
   int num_kv_heads;
-  int block_size;
+  int log2_block_size;
   int64_t num_blocks;
   int* err_word;
 };
 
-__device__ __forceinline__ void unpack_bf16x8(const uint4 v, float (&x)[8]) {
+__device__ __forceinline__ void unpack_bf16x8_f32x2(const uint4 v, uint64_t (&x)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i)
+    x[i] = pack_f32x2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
 
 constexpr int kNrThreads = 256;
@@ -81,27 +79,30 @@ __global__ void __launch_bounds__(kNrThreads, 4) qk_norm_rope_kernel(const QkNor
   const int h0 = threadIdx.x / kLanes;
   const int nqk = p.num_q_heads + p.num_kv_heads;
   const int all = nqk + (p.slot_mapping ? p.num_kv_heads : 0);   // q, k and (to be written) v heads
+  // this token's rows, at this thread's first element of head 0 (k and v seen from their place in
+  // the order q, k, v, so that a head's offset is its index times HD for all three)
+  constexpr int kEl = LAYOUT == kNrSplit ? 4 : 8;
+  const __nv_bfloat16* q_in = p.q + t * p.q_stride + li * kEl;
+  const __nv_bfloat16* k_in = p.k + t * p.k_stride + li * kEl - p.num_q_heads * HD;
+  const __nv_bfloat16* v_in = p.v + t * p.v_stride + li * kEl - nqk * HD;
+  __nv_bfloat16* q_to = p.q_out + t * p.q_out_stride + li * kEl;
+  __nv_bfloat16* k_to = p.k_out + t * p.k_out_stride + li * kEl - p.num_q_heads * HD;
 
-  auto at = [&](const __nv_bfloat16* base, int64_t stride, int head) {
-    return base + t * stride + static_cast<int64_t>(head) * HD;
-  };
   auto load = [&](int head) -> uint4 {
-    const __nv_bfloat16* src = head < p.num_q_heads ? at(p.q, p.q_stride, head)
-                               : head < nqk ? at(p.k, p.k_stride, head - p.num_q_heads)
-                                            : at(p.v, p.v_stride, head - nqk);
+    const __nv_bfloat16* src = (head < p.num_q_heads ? q_in : head < nqk ? k_in : v_in) + head * HD;
     if (LAYOUT == kNrSplit) {
-      const uint2 a = *reinterpret_cast<const uint2*>(src + li * 4);
-      const uint2 b = *reinterpret_cast<const uint2*>(src + HD / 2 + li * 4);
+      const uint2 a = *reinterpret_cast<const uint2*>(src);
+      const uint2 b = *reinterpret_cast<const uint2*>(src + HD / 2);
       return make_uint4(a.x, a.y, b.x, b.y);
     }
-    return *reinterpret_cast<const uint4*>(src + li * 8);
+    return *reinterpret_cast<const uint4*>(src);
   };
   auto store = [&](__nv_bfloat16* dst, const uint4 y) {
     if (LAYOUT == kNrSplit) {
-      *reinterpret_cast<uint2*>(dst + li * 4) = make_uint2(y.x, y.y);
-      *reinterpret_cast<uint2*>(dst + HD / 2 + li * 4) = make_uint2(y.z, y.w);
+      *reinterpret_cast<uint2*>(dst) = make_uint2(y.x, y.y);
+      *reinterpret_cast<uint2*>(dst + HD / 2) = make_uint2(y.z, y.w);
     } else {
-      *reinterpret_cast<uint4*>(dst + li * 8) = y;
+      *reinterpret_cast<uint4*>(dst) = y;
     }
   };
   uint4 pre[kNrPrefetch];
@@ -119,31 +120,32 @@ __global__ void __launch_bounds__(kNrThreads, 4) qk_norm_rope_kernel(const QkNor
     reinterpret_cast<float*>(sn4)[threadIdx.x] = s;
     reinterpret_cast<float*>(cs4)[threadIdx.x] = c;
   }
-  int64_t blk = -1;
-  int off = 0;
+  // element offset of KV head 0's row of this token's slot in the caches; negative: not written
+  int64_t cache_row = -1;
   if (p.slot_mapping) {
     const int64_t slot = p.slot_mapping[t];
     if (slot >= 0) {
-      blk = slot / p.block_size;
-      off = static_cast<int>(slot - blk * p.block_size);
+      const int64_t blk = slot >> p.log2_block_size;
       if (blk >= p.num_blocks) {
         if (threadIdx.x == 0) atomicExch(p.err_word, kDevBadIndex);
-        blk = -1;
+      } else {
+        const int64_t off = slot & ((1 << p.log2_block_size) - 1);
+        cache_row = (((blk * p.num_kv_heads) << p.log2_block_size) + off) * HD + li * kEl;
       }
     }
   }
   auto store_cache = [&](uint8_t* cache, int h, const uint4 y) {
-    const int64_t row = ((blk * p.num_kv_heads + h) * p.block_size + off) * HD;
+    const int64_t at = cache_row + (static_cast<int64_t>(h * HD) << p.log2_block_size);
     if (!p.cache_fp8) {
-      store(reinterpret_cast<__nv_bfloat16*>(cache) + row, y);
+      store(reinterpret_cast<__nv_bfloat16*>(cache) + at, y);
       return;
     }
     const uint2 c = bf16x8_to_e4m3x8(y);
     if (LAYOUT == kNrSplit) {
-      *reinterpret_cast<uint32_t*>(cache + row + li * 4) = c.x;
-      *reinterpret_cast<uint32_t*>(cache + row + HD / 2 + li * 4) = c.y;
+      *reinterpret_cast<uint32_t*>(cache + at) = c.x;
+      *reinterpret_cast<uint32_t*>(cache + at + HD / 2) = c.y;
     } else {
-      *reinterpret_cast<uint2*>(cache + row + li * 8) = c;
+      *reinterpret_cast<uint2*>(cache + at) = c;
     }
   };
   __syncthreads();
@@ -167,68 +169,96 @@ __global__ void __launch_bounds__(kNrThreads, 4) qk_norm_rope_kernel(const QkNor
     c[i] = cv.x, c[i + 1] = cv.y, c[i + 2] = cv.z, c[i + 3] = cv.w;
     s[i] = sv.x, s[i + 1] = sv.y, s[i + 2] = sv.z, s[i + 3] = sv.w;
   }
-  float w[8];
+  // Two values a register pair and instruction (packed fp32): w2[i] are elements 2 i, 2 i + 1.
+  uint64_t w2[4];
   bool have_k = false;
   auto load_weight = [&](const void* weight) {
+    if (p.weight_f32) {
+      const float* f = static_cast<const float*>(weight) + li * kEl;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = LAYOUT == kNrSplit ? (i < 4 ? li * 4 + i : HD / 2 + li * 4 + i - 4) : li * 8 + i;
-      w[i] = p.weight_f32 ? __ldg(static_cast<const float*>(weight) + e)
-                          : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(weight) + e));
+      for (int i = 0; i < 2; ++i) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(
+            f + (i == 0 ? 0 : LAYOUT == kNrSplit ? HD / 2 : 4)));
+        w2[2 * i] = pack_f32x2(v.x, v.y);
+        w2[2 * i + 1] = pack_f32x2(v.z, v.w);
+      }
+    } else {
+      const __nv_bfloat16* f = static_cast<const __nv_bfloat16*>(weight) + li * kEl;
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(f));
+      const uint2 b = __ldg(reinterpret_cast<const uint2*>(f + (LAYOUT == kNrSplit ? HD / 2 : 4)));
+      unpack_bf16x8_f32x2(make_uint4(a.x, a.y, b.x, b.y), w2);
     }
   };
   load_weight(p.q_weight);
+  uint64_t c2[kAngles / 2], s2[kAngles / 2], n2[kAngles / 2];      // cos, sin, - sin
+#pragma unroll
+  for (int i = 0; i < kAngles / 2; ++i) {
+    c2[i] = pack_f32x2(c[2 * i], c[2 * i + 1]);
+    s2[i] = pack_f32x2(s[2 * i], s[2 * i + 1]);
+    n2[i] = pack_f32x2(-s[2 * i], -s[2 * i + 1]);
+  }
 
   auto process = [&](int head, uint4 raw) {   // every lane of the warp comes here
-    if (head >= nqk) {
-      if (head < all && blk >= 0) store_cache(p.v_cache, head - nqk, raw);
-    }
+    if (head >= nqk && head < all && cache_row >= 0) store_cache(p.v_cache, head - nqk, raw);
     const bool is_k = head >= p.num_q_heads;
     if (is_k && !have_k) {                    // heads come in ascending order: q, then k
       load_weight(p.k_weight);
       have_k = true;
     }
-    float x[8];
-    unpack_bf16x8(raw, x);
-    float ss = 0.f;
+    uint64_t x[4];
+    unpack_bf16x8_f32x2(raw, x);
+    uint64_t sq = mul_f32x2(x[0], x[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+    for (int i = 1; i < 4; ++i) sq = fma_f32x2(x[i], x[i], sq);
+    float ss, ss1;
+    unpack_f32x2(sq, ss, ss1);
+    ss += ss1;
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float r = rsqrtf(ss * (1.f / HD) + p.eps);
+    const uint64_t r2 = pack_f32x2(r, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+    for (int i = 0; i < 4; ++i) x[i] = mul_f32x2(mul_f32x2(x[i], r2), w2[i]);
     if (LAYOUT == kNrSplit) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = x[i], b = x[i + 4];
-        x[i] = a * c[i] - b * s[i];
-        x[i + 4] = b * c[i] + a * s[i];
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t a = x[i], b = x[i + 2];
+        x[i] = fma_f32x2(a, c2[i], mul_f32x2(b, n2[i]));
+        x[i + 2] = fma_f32x2(b, c2[i], mul_f32x2(a, s2[i]));
       }
     } else if (LAYOUT == kNrShuffle) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_sync(0xffffffffu, x[i], partner);
-        if (rotates) x[i] = second ? x[i] * c[i] + other * s[i] : x[i] * c[i] - other * s[i];
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t other = __shfl_sync(0xffffffffu, x[i], partner);
+        if (rotates) x[i] = fma_f32x2(x[i], c2[i], mul_f32x2(other, second ? s2[i] : n2[i]));
       }
     } else if (rotates) {
+      const uint64_t* cp = c2;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * c[i] - b * s[i];
-        x[2 * i + 1] = b * c[i] + a * s[i];
+        float a, b, c0, c1, s0, s1;
+        unpack_f32x2(x[i], a, b);
+        unpack_f32x2(cp[i / 2], c0, c1);
+        unpack_f32x2(s2[i / 2], s0, s1);
+        const float cc = i & 1 ? c1 : c0, sn = i & 1 ? s1 : s0;
+        x[i] = pack_f32x2(a * cc - b * sn, b * cc + a * sn);
       }
     }
     if (head >= nqk) return;
-    const uint4 y = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                               pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      unpack_f32x2(x[i], a, b);
+      y[i] = pack_bf16x2(a, b);
+    }
+    const uint4 yy = make_uint4(y[0], y[1], y[2], y[3]);
     if (!is_k) {
-      store(p.q_out + t * p.q_out_stride + static_cast<int64_t>(head) * HD, y);
+      store(q_to + head * HD, yy);
       return;
     }
-    const int h = head - p.num_q_heads;
-    store(p.k_out + t * p.k_out_stride + static_cast<int64_t>(h) * HD, y);
-    if (blk >= 0) store_cache(p.k_cache, h, y);
+    store(k_to + head * HD, yy);
+    if (cache_row >= 0) store_cache(p.k_cache, head - p.num_q_heads, yy);
   };
 
   // the bound is rounded up to whole warps: all lanes of a warp take the shuffles together

@@ -155,7 +155,7 @@ __device__ double exact_page_score(const SelectPagesParams& p, int user, int kvh
 }
 
 template <int HD, int BS, int NG>
-__global__ void __launch_bounds__(kSelThreads) select_pages_kernel(const SelectPagesParams p) {
+__global__ void __launch_bounds__(kSelThreads, NG == 1 ? 2 : 1) select_pages_kernel(const SelectPagesParams p) {
   __shared__ SelectShared sh;
   const int kvh = blockIdx.y, user = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
