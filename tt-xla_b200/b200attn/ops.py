@@ -9,6 +9,7 @@ to.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -110,28 +111,6 @@ def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
     if index < 0:
         _need_cuda(first)
     return index
-
-
-class _on_device:
-    """Makes a device current for a call into the library (which works on the current device); free
-    of charge when it already is."""
-
-    __slots__ = ("index", "previous")
-
-    def __init__(self, index: int):
-        self.index = index
-        self.previous = -1
-
-    def __enter__(self):
-        current = _current_device()
-        if current != self.index:
-            self.previous = current
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.previous >= 0:
-            torch.cuda.set_device(self.previous)
-        return False
 
 
 def _check_scales(k_scale, v_scale, k_cache: torch.Tensor) -> bool:
@@ -329,6 +308,17 @@ def _rows_meet(a: tuple, b: tuple, tokens: int) -> bool:
     return True
 
 
+def _check_outputs(tokens: int, oq: tuple, ok: tuple, q: tuple, k: tuple, v: tuple) -> None:
+    """Each output is its input or shares no memory with any input, nor with the other output; all
+    as (pointer, row stride, row width) in bytes, v's pointer 0 when it is not read."""
+    for out, own in ((oq, q), (ok, k)):
+        if out != own and (_rows_meet(out, q, tokens) or _rows_meet(out, k, tokens)
+                           or (v[0] and _rows_meet(out, v, tokens))):
+            raise ValueError("an output must be its input or overlap none of the inputs")
+    if _rows_meet(oq, ok, tokens):
+        raise ValueError("the outputs must not overlap")
+
+
 def qk_norm_rope_kv_scatter_slots(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -360,21 +350,29 @@ def qk_norm_rope_kv_scatter_slots(
     ok = key if out_key is None else out_key
     index = _device_of(query, key, positions, inv_freq, q_weight, k_weight, out_query, out_key,
                        value, slot_mapping, k_cache, v_cache)
+    if _current_device() != index:       # the library works on the current device
+        with torch.cuda.device(index):
+            return qk_norm_rope_kv_scatter_slots(
+                query, key, value, positions, inv_freq, rotary_dim, head_size, q_weight, k_weight,
+                eps, k_cache, v_cache, slot_mapping, is_neox_style, out_query, out_key)
     tokens = positions.numel()
     if query.dim() != 2 or key.dim() != 2 or query.shape[0] != tokens or key.shape[0] != tokens:
         raise ValueError("query / key must be [tokens, heads*head_size] with one row per position")
     q_width, k_width = query.shape[1], key.shape[1]
     if q_width % head_size or k_width % head_size:
         raise ValueError("query / key rows must hold whole heads")
-    if oq.shape != query.shape or ok.shape != key.shape:
-        raise ValueError("out_query / out_key must have query's / key's shape")
     bf16 = torch.bfloat16
-    strides = []
-    for t in (oq, ok, query, key):
-        row, column = t.stride()
-        if t.dtype != bf16 or column != 1:
-            raise ValueError("query, key and the outputs must be bfloat16 with dense rows")
-        strides.append(row if tokens > 1 else t.shape[1])
+    if query.dtype != bf16 or key.dtype != bf16 or query.stride(1) != 1 or key.stride(1) != 1:
+        raise ValueError("query / key must be bfloat16 with dense rows")
+    q_stride, k_stride = (query.stride(0), key.stride(0)) if tokens > 1 else (q_width, k_width)
+    oq_stride, ok_stride = q_stride, k_stride
+    if oq is not query or ok is not key:
+        if oq.shape != query.shape or ok.shape != key.shape:
+            raise ValueError("out_query / out_key must have query's / key's shape")
+        if oq.dtype != bf16 or ok.dtype != bf16 or oq.stride(1) != 1 or ok.stride(1) != 1:
+            raise ValueError("out_query / out_key must be bfloat16 with dense rows")
+        if tokens > 1:
+            oq_stride, ok_stride = oq.stride(0), ok.stride(0)
     if positions.dtype != torch.int64 or not positions.is_contiguous():
         raise ValueError("positions must be a dense int64 tensor")
     if inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2 \
@@ -405,21 +403,16 @@ def qk_norm_rope_kv_scatter_slots(
     if tokens == 0:
         return oq, ok
     oq_ptr, ok_ptr, q_ptr, k_ptr = oq.data_ptr(), ok.data_ptr(), query.data_ptr(), key.data_ptr()
-    outs = ((oq_ptr, 2 * strides[0], 2 * q_width), (ok_ptr, 2 * strides[1], 2 * k_width))
-    ins = ((q_ptr, 2 * strides[2], 2 * q_width), (k_ptr, 2 * strides[3], 2 * k_width),
-           (v_ptr, 2 * v_stride, 2 * k_width))
-    for i in (0, 1):
-        if outs[i] != ins[i] and any(_rows_meet(outs[i], x, tokens) for x in ins if x[0]):
-            raise ValueError("an output must be its input or overlap none of the inputs")
-    if _rows_meet(outs[0], outs[1], tokens):
-        raise ValueError("the outputs must not overlap")
-    with _on_device(index):
-        status = _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
-            oq_ptr, strides[0], ok_ptr, strides[1], q_ptr, strides[2], k_ptr, strides[3],
-            v_ptr, v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
-            1 if w_dtype == torch.float32 else 0, eps, positions.data_ptr(), inv_freq.data_ptr(),
-            rotary_dim, 1 if is_neox_style else 0, kc_ptr, vc_ptr, kind, slot_ptr, tokens,
-            q_width // head_size, nkv, head_size, bs, nb, _raw_stream(index))
+    if oq_ptr != q_ptr or ok_ptr != k_ptr or oq_stride != q_stride or ok_stride != k_stride:
+        _check_outputs(tokens, (oq_ptr, 2 * oq_stride, 2 * q_width),
+                       (ok_ptr, 2 * ok_stride, 2 * k_width), (q_ptr, 2 * q_stride, 2 * q_width),
+                       (k_ptr, 2 * k_stride, 2 * k_width), (v_ptr, 2 * v_stride, 2 * k_width))
+    status = _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
+        oq_ptr, oq_stride, ok_ptr, ok_stride, q_ptr, q_stride, k_ptr, k_stride,
+        v_ptr, v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
+        1 if w_dtype == torch.float32 else 0, eps, positions.data_ptr(), inv_freq.data_ptr(),
+        rotary_dim, 1 if is_neox_style else 0, kc_ptr, vc_ptr, kind, slot_ptr, tokens,
+        q_width // head_size, nkv, head_size, bs, nb, _raw_stream(index))
     if status:
         _lib.check("b200attn_qk_norm_rope_kv_scatter_slots", status)
     return oq, ok
@@ -461,6 +454,10 @@ def paged_write(
     `select_pages`.  The sequences of one call must write to different pages."""
     index = _device_of(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len, k_scale,
                        v_scale, k_bounds)
+    if _current_device() != index:       # the library works on the current device
+        with torch.cuda.device(index):
+            return paged_write(k_cache, v_cache, key, value, page_table, q_start, cu_q, q_len,
+                               k_scale, v_scale, k_bounds)
     scaled = _check_scales(k_scale, v_scale, k_cache)
     nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
     if not scaled:
@@ -494,14 +491,13 @@ def paged_write(
         raise ValueError("q_len must be int32 with a dense entry per sequence")
     if seqs == 0 or rows == 0:
         return
-    with _on_device(index):
-        status = _lib.lib().b200attn_paged_write(
-            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if scaled else 0,
-            v_scale.data_ptr() if scaled else 0, 0 if k_bounds is None else k_bounds.data_ptr(),
-            _cache_dtype(k_cache), key.data_ptr(), kstride, value.data_ptr(), vstride,
-            page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-            0 if cu_q is None else cu_q.data_ptr(), 0 if q_len is None else q_len.data_ptr(),
-            q_start.data_ptr(), seqs, rows, nkv, hd, bs, nb, _raw_stream(index))
+    status = _lib.lib().b200attn_paged_write(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if scaled else 0,
+        v_scale.data_ptr() if scaled else 0, 0 if k_bounds is None else k_bounds.data_ptr(),
+        _cache_dtype(k_cache), key.data_ptr(), kstride, value.data_ptr(), vstride,
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+        0 if cu_q is None else cu_q.data_ptr(), 0 if q_len is None else q_len.data_ptr(),
+        q_start.data_ptr(), seqs, rows, nkv, hd, bs, nb, _raw_stream(index))
     if status:
         _lib.check("b200attn_paged_write", status)
 
@@ -557,6 +553,24 @@ def _scratch(index: int, stream: int, nbytes: int) -> Optional[torch.Tensor]:
     return have[1]
 
 
+# Sizes and split counts are pure functions of whole numbers that the library computes.
+@functools.lru_cache(maxsize=4096)
+def _select_bytes(users: int, nkv: int, width: int) -> int:
+    return _lib.lib().b200attn_select_pages_workspace_bytes(users, nkv, width)
+
+
+@functools.lru_cache(maxsize=4096)
+def _blocks_splits(scaled: bool, users: int, nkv: int, hd: int, ctx: int) -> int:
+    L = _lib.lib()
+    pick = L.b200attn_decode_blocks_auto_splits if scaled else L.b200attn_decode_auto_splits
+    return pick(users, nkv, hd, ctx)
+
+
+@functools.lru_cache(maxsize=4096)
+def _decode_bytes(users: int, nq: int, hd: int, splits: int) -> int:
+    return _lib.lib().b200attn_decode_workspace_bytes(users, nq, hd, splits)
+
+
 def select_pages(
     query: torch.Tensor,
     k_bounds: torch.Tensor,
@@ -577,6 +591,10 @@ def select_pages(
     Returns (table [users, nkv, num_pages], pos [users, nkv]): hand them to `paged_decode` as
     `page_table` and `cur_pos`.  `max_context_len` only shapes the launch."""
     index = _device_of(query, k_bounds, page_table, cur_pos, workspace)
+    if _current_device() != index:       # the library works on the current device
+        with torch.cuda.device(index):
+            return select_pages(query, k_bounds, page_table, cur_pos, block_size, num_pages,
+                                keep_first, keep_last, max_context_len, workspace)
     if k_bounds.dim() != 4 or k_bounds.shape[2] != 2 or k_bounds.dtype != torch.bfloat16 \
             or not k_bounds.is_contiguous():
         raise ValueError("k_bounds must be dense bfloat16 [num_blocks, num_kv_heads, 2, head_size]")
@@ -600,18 +618,16 @@ def select_pages(
     pos = cur_pos.new_empty((users, nkv))
     if users == 0:
         return table, pos
-    L = _lib.lib()
     width = page_table.shape[1]
-    with _on_device(index):
-        stream = _raw_stream(index)
-        ws = workspace
-        if ws is None:
-            ws = _scratch(index, stream, L.b200attn_select_pages_workspace_bytes(users, nkv, width))
-        status = L.b200attn_select_pages(
-            table.data_ptr(), pos.data_ptr(), q.data_ptr(), qstride, k_bounds.data_ptr(),
-            page_table.data_ptr(), page_table.stride(0), width, cur_pos.data_ptr(), users, nq, nkv,
-            hd, block_size, nb, num_pages, keep_first, keep_last, max_context_len, ws.data_ptr(),
-            ws.numel() * ws.element_size(), stream)
+    stream = _raw_stream(index)
+    ws = workspace
+    if ws is None:
+        ws = _scratch(index, stream, _select_bytes(users, nkv, width))
+    status = _lib.lib().b200attn_select_pages(
+        table.data_ptr(), pos.data_ptr(), q.data_ptr(), qstride, k_bounds.data_ptr(),
+        page_table.data_ptr(), page_table.stride(0), width, cur_pos.data_ptr(), users, nq, nkv,
+        hd, block_size, nb, num_pages, keep_first, keep_last, max_context_len, ws.data_ptr(),
+        ws.numel() * ws.element_size(), stream)
     if status:
         _lib.check("b200attn_select_pages", status)
     return table, pos
@@ -622,6 +638,11 @@ def _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out, num
     """paged_decode over block-scaled caches and / or a page list per KV head."""
     index = _device_of(query, k_cache, v_cache, page_table, cur_pos, k_scale, v_scale, out, sinks,
                        workspace)
+    if _current_device() != index:       # the library works on the current device
+        with torch.cuda.device(index):
+            return _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out,
+                                  num_splits, max_context_len, workspace, sliding_window, sinks,
+                                  k_scale, v_scale)
     scaled = _check_scales(k_scale, v_scale, k_cache)
     nb, nkv, bs, hd = _check_cache(k_cache, v_cache, scaled)
     shape = query.shape
@@ -667,29 +688,25 @@ def _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out, num
         raise ValueError("sinks must be a dense float32 tensor with one entry per q head")
     if users == 0:
         return out if out is not None else out_t.reshape(shape)
-    L = _lib.lib()
-    with _on_device(index):
-        stream = _raw_stream(index)
-        if num_splits == 0:
-            num_splits = _env_num_splits()
-        if num_splits == 0:
-            ctx = max_context_len if max_context_len > 0 else width * bs
-            if sliding_window > 0:
-                ctx = min(ctx, sliding_window + 64)
-            pick = L.b200attn_decode_blocks_auto_splits if scaled else L.b200attn_decode_auto_splits
-            num_splits = pick(users, nkv, hd, ctx)
-        ws = workspace
-        if ws is None and num_splits > 1:
-            ws = _scratch(index, stream, L.b200attn_decode_workspace_bytes(users, nq, hd, num_splits))
-        status = L.b200attn_paged_decode_blocks(
-            out_t.data_ptr(), ostride, q.data_ptr(), qstride, k_cache.data_ptr(),
-            v_cache.data_ptr(), k_scale.data_ptr() if scaled else 0,
-            v_scale.data_ptr() if scaled else 0, _cache_dtype(k_cache), page_table.data_ptr(),
-            page_table.stride(0), head_stride, width, cur_pos.data_ptr(), users, nq, nkv, hd, bs,
-            nb, hd ** -0.5 if scale is None else scale, sliding_window,
-            sinks.data_ptr() if sinks is not None else 0, max_context_len, num_splits,
-            ws.data_ptr() if ws is not None else 0,
-            ws.numel() * ws.element_size() if ws is not None else 0, stream)
+    stream = _raw_stream(index)
+    if num_splits == 0:
+        num_splits = _env_num_splits()
+    if num_splits == 0:
+        ctx = max_context_len if max_context_len > 0 else width * bs
+        if sliding_window > 0:
+            ctx = min(ctx, sliding_window + 64)
+        num_splits = _blocks_splits(scaled, users, nkv, hd, ctx)
+    ws = workspace
+    if ws is None and num_splits > 1:
+        ws = _scratch(index, stream, _decode_bytes(users, nq, hd, num_splits))
+    status = _lib.lib().b200attn_paged_decode_blocks(
+        out_t.data_ptr(), ostride, q.data_ptr(), qstride, k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr() if scaled else 0, v_scale.data_ptr() if scaled else 0,
+        _cache_dtype(k_cache), page_table.data_ptr(), page_table.stride(0), head_stride, width,
+        cur_pos.data_ptr(), users, nq, nkv, hd, bs, nb, hd ** -0.5 if scale is None else scale,
+        sliding_window, sinks.data_ptr() if sinks is not None else 0, max_context_len, num_splits,
+        ws.data_ptr() if ws is not None else 0,
+        ws.numel() * ws.element_size() if ws is not None else 0, stream)
     if status:
         _lib.check("b200attn_paged_decode_blocks", status)
     return out if out is not None else out_t.reshape(shape)
@@ -840,6 +857,12 @@ def prefill(
     scaled = False
     if not paged and (k_scale is not None or v_scale is not None):
         raise ValueError("k_scale / v_scale go with a paged cache")
+    if paged and k_scale is not None:
+        index = _device_of(query, k_src, v_src, page_table, q_start, cu_q, out, k_scale, v_scale)
+        if _current_device() != index:       # the library works on the current device
+            with torch.cuda.device(index):
+                return prefill(query, k_src, v_src, cu_q_host, scale, page_table, q_start, out,
+                               cu_q, sliding_window, k_scale, v_scale)
     if paged:
         scaled = _check_scales(k_scale, v_scale, k_src)
         nb, nkv, bs, _hd = _check_cache(k_src, v_src, scaled)
@@ -874,7 +897,6 @@ def prefill(
         cu_q = cu_q_host.to(query.device, non_blocking=True)
     _i32(cu_q, "cu_q")
     if scaled:
-        index = _device_of(query, k_src, v_src, page_table, q_start, cu_q, out, k_scale, v_scale)
         k, v, factors, page_table, nb = _widen_scaled_pages(k_src, v_src, k_scale, v_scale,
                                                             page_table, cu_q, q_start, num_seqs)
     elif paged and k_src.dtype == torch.float8_e4m3fn:
@@ -895,18 +917,14 @@ def prefill(
         scale = hd ** -0.5
     L = _lib.lib()
     if scaled:
-        with _on_device(index):
-            _lib.check(
-                "b200attn_prefill_scaled",
-                L.b200attn_prefill_scaled(
-                    out_t.data_ptr(), ostride, q.data_ptr(),
-                    qstride if total_q > 1 else max(qstride, nq * hd), k.data_ptr(), v.data_ptr(),
-                    factors.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                    page_table.shape[1], cu_q.data_ptr(), cu_q_host.data_ptr(),
-                    q_start.data_ptr() if q_start is not None else None, num_seqs, total_q, nq,
-                    nkv, hd, bs, nb, float(scale), int(sliding_window), _stream(query),
-                ),
-            )
+        status = L.b200attn_prefill_scaled(
+            out_t.data_ptr(), ostride, q.data_ptr(),
+            qstride if total_q > 1 else max(qstride, nq * hd), k.data_ptr(), v.data_ptr(),
+            factors.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+            cu_q.data_ptr(), cu_q_host.data_ptr(), q_start.data_ptr() if q_start is not None else 0,
+            num_seqs, total_q, nq, nkv, hd, bs, nb, scale, sliding_window, _raw_stream(index))
+        if status:
+            _lib.check("b200attn_prefill_scaled", status)
         return out if out is not None else out_t
     _lib.check(
         "b200attn_prefill_ex",
@@ -965,41 +983,35 @@ _scaled_scratch: dict[tuple, tuple] = {}
 
 
 def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_start, num_seqs):
-    """_widen_fp8_pages for a block-scaled cache pair: (k_pool, v_pool, the pages' factors, identity
+    """_widen_fp8_pages for a block-scaled cache pair on the current device: (k_pool, v_pool, the pages' factors, identity
     page table, pool size).  Under stream capture the pool belongs to the graph being captured."""
     nb, nkv, bs, hd = k_cache.shape
     width = page_table.shape[1]
     pages = max(num_seqs * width, 1)
     dev = k_cache.device
-    with _on_device(dev.index):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        capturing = torch.cuda.is_current_stream_capturing()
-        key = (dev.index or 0, stream, nkv, bs, hd)
-        have = None if capturing else _scaled_scratch.get(key)
-        if have is None or have[0].shape[0] < pages:
-            grow = pages
-            if have is not None:
-                grow = max(pages, 2 * have[0].shape[0])
-            have = (torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
-                    torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
-                    torch.empty((grow, nkv, 2), dtype=torch.float32, device=dev), {})
-            if not capturing:
-                _scaled_scratch[key] = have
-        k_pool, v_pool, factors, tables = have
-        ident = tables.get((num_seqs, width))
-        if ident is None:
-            ident = torch.arange(num_seqs * width, dtype=torch.int32, device=dev)
-            ident = tables[(num_seqs, width)] = ident.reshape(num_seqs, width)
-        _lib.check(
-            "b200attn_dequant_pages_scaled",
-            _lib.lib().b200attn_dequant_pages_scaled(
-                k_pool.data_ptr(), v_pool.data_ptr(), factors.data_ptr(), k_cache.data_ptr(),
-                v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _cache_dtype(k_cache),
-                page_table.data_ptr(), page_table.stride(0), width, cu_q.data_ptr(),
-                q_start.data_ptr() if q_start is not None else None, num_seqs, nkv, hd, bs, nb,
-                stream,
-            ),
-        )
+    stream = _raw_stream(dev.index)
+    capturing = torch.cuda.is_current_stream_capturing()
+    key = (dev.index, stream, nkv, bs, hd)
+    have = None if capturing else _scaled_scratch.get(key)
+    if have is None or have[0].shape[0] < pages:
+        grow = pages if have is None else max(pages, 2 * have[0].shape[0])
+        have = (torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
+                torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
+                torch.empty((grow, nkv, 2), dtype=torch.float32, device=dev), {})
+        if not capturing:
+            _scaled_scratch[key] = have
+    k_pool, v_pool, factors, tables = have
+    ident = tables.get((num_seqs, width))
+    if ident is None:
+        ident = torch.arange(num_seqs * width, dtype=torch.int32, device=dev)
+        ident = tables[(num_seqs, width)] = ident.reshape(num_seqs, width)
+    _lib.check(
+        "b200attn_dequant_pages_scaled",
+        _lib.lib().b200attn_dequant_pages_scaled(
+            k_pool.data_ptr(), v_pool.data_ptr(), factors.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _cache_dtype(k_cache),
+            page_table.data_ptr(), page_table.stride(0), width, cu_q.data_ptr(),
+            q_start.data_ptr() if q_start is not None else 0, num_seqs, nkv, hd, bs, nb, stream))
     return k_pool, v_pool, factors, ident, k_pool.shape[0]
 
 
