@@ -388,7 +388,10 @@ int b200attn_paged_write(void* k_cache, void* v_cache, float* k_scale, float* v_
  *     between heads, cur_pos is [num_users, num_kv_heads] and counts within the list: the keys
  *     of the list's pages 0 .. cur_pos / block_size are attended, the last page up to
  *     cur_pos % block_size (what b200attn_select_pages writes).  No sliding window then.
- * b200attn_decode_blocks_auto_splits: the split count num_splits = 0 picks for scaled caches. */
+ *   num_splits: for scaled caches 0 cuts the whole batch's context into equal shares, one per CTA
+ *     (num_splits > 0 cuts every (user, KV head) into that many); the workspace then holds
+ *     b200attn_decode_scaled_workspace_bytes of the current device.  For other caches as in
+ *     b200attn_paged_decode. */
 int b200attn_paged_decode_blocks(void* out, int64_t out_row_stride, const void* q,
                                  int64_t q_row_stride, const void* k_cache, const void* v_cache,
                                  const float* k_scale, const float* v_scale, int cache_dtype,
@@ -399,8 +402,8 @@ int b200attn_paged_decode_blocks(void* out, int64_t out_row_stride, const void* 
                                  int64_t num_blocks, float scale, int sliding_window,
                                  const float* sinks, int max_context_len, int num_splits,
                                  void* workspace, size_t workspace_bytes, void* stream);
-int b200attn_decode_blocks_auto_splits(int num_users, int num_kv_heads, int head_size,
-                                       int max_context_len);
+size_t b200attn_decode_scaled_workspace_bytes(int num_users, int num_q_heads, int num_kv_heads,
+                                              int head_size, int num_splits);
 
 /* ------------------------------------------------------------------------------------------
  * Page selection for block-sparse decode attention.

@@ -98,7 +98,7 @@ SIGNATURES = {
          c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64,
          c_float, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p],
     ),
-    "b200attn_decode_blocks_auto_splits": (c_int, [c_int, c_int, c_int, c_int]),
+    "b200attn_decode_scaled_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "b200attn_select_pages_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "b200attn_select_pages": (
         c_int,

@@ -311,6 +311,14 @@ def _rows_meet(a: tuple, b: tuple, tokens: int) -> bool:
 def _check_outputs(tokens: int, oq: tuple, ok: tuple, q: tuple, k: tuple, v: tuple) -> None:
     """Each output is its input or shares no memory with any input, nor with the other output; all
     as (pointer, row stride, row width) in bytes, v's pointer 0 when it is not read."""
+    # the usual case first: outputs on either side of everything else
+    last = tokens - 1
+    lo = min(q[0], k[0], v[0] or q[0])
+    hi = max(q[0] + last * q[1] + q[2], k[0] + last * k[1] + k[2], v[0] + last * v[1] + v[2])
+    oq_end, ok_end = oq[0] + last * oq[1] + oq[2], ok[0] + last * ok[1] + ok[2]
+    if (oq[0] >= hi or oq_end <= lo) and (ok[0] >= hi or ok_end <= lo) and \
+            (oq[0] >= ok_end or ok[0] >= oq_end):
+        return
     for out, own in ((oq, q), (ok, k)):
         if out != own and (_rows_meet(out, q, tokens) or _rows_meet(out, k, tokens)
                            or (v[0] and _rows_meet(out, v, tokens))):
@@ -560,15 +568,18 @@ def _select_bytes(users: int, nkv: int, width: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def _blocks_splits(scaled: bool, users: int, nkv: int, hd: int, ctx: int) -> int:
-    L = _lib.lib()
-    pick = L.b200attn_decode_blocks_auto_splits if scaled else L.b200attn_decode_auto_splits
-    return pick(users, nkv, hd, ctx)
+def _list_splits(users: int, nkv: int, hd: int, ctx: int) -> int:
+    return _lib.lib().b200attn_decode_auto_splits(users, nkv, hd, ctx)
 
 
 @functools.lru_cache(maxsize=4096)
 def _decode_bytes(users: int, nq: int, hd: int, splits: int) -> int:
     return _lib.lib().b200attn_decode_workspace_bytes(users, nq, hd, splits)
+
+
+@functools.lru_cache(maxsize=4096)
+def _scaled_bytes(device: int, users: int, nq: int, nkv: int, hd: int, splits: int) -> int:
+    return _lib.lib().b200attn_decode_scaled_workspace_bytes(users, nq, nkv, hd, splits)
 
 
 def select_pages(
@@ -691,14 +702,16 @@ def _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out, num
     stream = _raw_stream(index)
     if num_splits == 0:
         num_splits = _env_num_splits()
-    if num_splits == 0:
-        ctx = max_context_len if max_context_len > 0 else width * bs
-        if sliding_window > 0:
-            ctx = min(ctx, sliding_window + 64)
-        num_splits = _blocks_splits(scaled, users, nkv, hd, ctx)
     ws = workspace
-    if ws is None and num_splits > 1:
-        ws = _scratch(index, stream, _decode_bytes(users, nq, hd, num_splits))
+    if scaled:
+        if ws is None:
+            ws = _scratch(index, stream, _scaled_bytes(index, users, nq, nkv, hd, num_splits))
+    else:
+        if num_splits == 0:
+            num_splits = _list_splits(users, nkv, hd, max_context_len if max_context_len > 0
+                                      else width * bs)
+        if ws is None and num_splits > 1:
+            ws = _scratch(index, stream, _decode_bytes(users, nq, hd, num_splits))
     status = _lib.lib().b200attn_paged_decode_blocks(
         out_t.data_ptr(), ostride, q.data_ptr(), qstride, k_cache.data_ptr(), v_cache.data_ptr(),
         k_scale.data_ptr() if scaled else 0, v_scale.data_ptr() if scaled else 0,

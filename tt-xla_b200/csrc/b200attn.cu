@@ -22,10 +22,6 @@
 #include "select_pages.cuh"
 #include "step_metadata.cuh"
 
-#ifndef B200ATTN_DS_STAGES
-#define B200ATTN_DS_STAGES 3
-#define B200ATTN_DS_STAGES64 4
-#endif
 namespace b200attn {
 
 static_assert(kDecTicketBytes == B200ATTN_DECODE_TICKET_BYTES, "header and kernels agree");
@@ -294,38 +290,50 @@ static int launch_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, const
 
 template <int HD, int BS, int FMT, int NG>
 static int launch_decode_scaled(const CUtensorMap& tk, const CUtensorMap& tv,
-                                const DecodeScaledParams& p, int num_users, cudaStream_t s) {
-  constexpr int kStages = HD == 128 ? B200ATTN_DS_STAGES : B200ATTN_DS_STAGES64;
-  using L = DecodeScaledSmem<HD, BS, kStages>;
+                                const DecodeScaledParams& p, int num_ctas, cudaStream_t s) {
+  constexpr int kStages = HD == 128 ? (NG == 1 ? 3 : 2) : 4;   // two CTAs per SM
+  using L = DecodeScaledSmem<HD, BS, NG, kStages>;
   auto kern = paged_decode_scaled_kernel<HD, BS, FMT, NG, kStages>;
   static bool smem_allowed[kMaxDevices] = {};
   cudaError_t e = allow_dynamic_smem(kern, L::kTotalBytes, smem_allowed);
   if (e != cudaSuccess) return static_cast<int>(e);
-  dim3 grid(p.d.num_splits, p.d.num_kv_heads, num_users);
-  kern<<<grid, kDecThreads, L::kTotalBytes, s>>>(tk, tv, p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (p.d.num_splits > 1 && !p.d.tickets) {
-    dim3 cgrid(p.d.num_q_heads, num_users);
-    decode_combine_kernel<HD><<<cgrid, HD, 0, s>>>(p.d);
-    e = cudaGetLastError();
-  }
-  return static_cast<int>(e);
+  kern<<<num_ctas, kDecThreads, L::kTotalBytes, s>>>(tk, tv, p);
+  return static_cast<int>(cudaGetLastError());
 }
 
 // query heads per KV head: one MMA column group up to 8, two up to 16
 template <int HD, int BS, int FMT>
 static int launch_decode_scaled_ng(const CUtensorMap& tk, const CUtensorMap& tv,
-                                   const DecodeScaledParams& p, int num_users, cudaStream_t s) {
-  return p.d.group <= 8 ? launch_decode_scaled<HD, BS, FMT, 1>(tk, tv, p, num_users, s)
-                        : launch_decode_scaled<HD, BS, FMT, 2>(tk, tv, p, num_users, s);
+                                   const DecodeScaledParams& p, int num_ctas, cudaStream_t s) {
+  return p.d.group <= 8 ? launch_decode_scaled<HD, BS, FMT, 1>(tk, tv, p, num_ctas, s)
+                        : launch_decode_scaled<HD, BS, FMT, 2>(tk, tv, p, num_ctas, s);
+}
+
+// CTAs of a launch over block-scaled caches.  Equal shares: what is resident at once (kDsCtasPerSm
+// per SM), but at most 64 per pair, as many partials as are worth merging.  64 users of 1024 to
+// 8192 tokens (8 heads of 128): 110 us, against 130 with one CTA per pair and 119 with the best
+// fixed number of splits; three smaller CTAs per SM: 136.  Where one CTA per pair happens to fill
+// the machine with equal work (32 users of 32768) that is 4 % faster (332 us, 349), but the host
+// does not know the lengths.
+constexpr int kDsCtasPerSm = 2;
+static int64_t decode_scaled_ctas(int sm_count, int64_t pairs, int num_splits) {
+  if (num_splits > 0) return pairs * num_splits;
+  const int64_t resident = static_cast<int64_t>(kDsCtasPerSm) * sm_count;
+  return pairs * 64 < resident ? pairs * 64 : resident;
+}
+// Rows of partial results: a share leaves at most two (its first and its last segment).
+static size_t decode_scaled_bytes(int sm_count, int64_t pairs, int group, int head_size,
+                                  int num_splits) {
+  const size_t rows = static_cast<size_t>(decode_scaled_ctas(sm_count, pairs, num_splits)) *
+                      (num_splits > 0 ? 1 : 2) * group;
+  return kDecTicketBytes + rows * (head_size * sizeof(float) + sizeof(float2));
 }
 
 template <int HD, int BS>
 static int launch_decode_scaled_fmt(int fmt, const CUtensorMap& tk, const CUtensorMap& tv,
-                                    const DecodeScaledParams& p, int num_users, cudaStream_t s) {
-  return fmt == kPageInt8 ? launch_decode_scaled_ng<HD, BS, kPageInt8>(tk, tv, p, num_users, s)
-                          : launch_decode_scaled_ng<HD, BS, kPageE4m3>(tk, tv, p, num_users, s);
+                                    const DecodeScaledParams& p, int num_ctas, cudaStream_t s) {
+  return fmt == kPageInt8 ? launch_decode_scaled_ng<HD, BS, kPageInt8>(tk, tv, p, num_ctas, s)
+                          : launch_decode_scaled_ng<HD, BS, kPageE4m3>(tk, tv, p, num_ctas, s);
 }
 
 // the layout of a head in its lanes (see NrLayout)
@@ -820,14 +828,22 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   if (max_context_len <= 0) max_context_len = page_table_width * block_size;
   if (sliding_window > 0 && max_context_len > sliding_window + kDecTile)
     max_context_len = sliding_window + kDecTile;       // what a user streams at most
-  if (num_splits == 0)
-    num_splits = scaled ? b200attn_decode_blocks_auto_splits(num_users, num_kv_heads, head_size,
-                                                             max_context_len)
-                        : b200attn_decode_auto_splits(num_users, num_kv_heads, head_size,
-                                                      max_context_len);
-  const size_t need = b200attn_decode_workspace_bytes(num_users, num_q_heads, head_size, num_splits);
-  if (num_splits > 1 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return B200ATTN_ERR_WORKSPACE;
+  const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
+  size_t need;
+  if (scaled) {
+    // too many pairs for the arrival counters: shares of whole pairs
+    if (pairs * static_cast<int64_t>(sizeof(unsigned int)) > kDecTicketBytes) num_splits = 0;
+    if (decode_scaled_ctas(dev->sm_count, pairs, num_splits) > 0x7fffffffLL)
+      return B200ATTN_ERR_TOO_LARGE;
+    need = decode_scaled_bytes(dev->sm_count, pairs, group, head_size, num_splits);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace)) return B200ATTN_ERR_WORKSPACE;
+  } else {
+    if (num_splits == 0)
+      num_splits = b200attn_decode_auto_splits(num_users, num_kv_heads, head_size, max_context_len);
+    need = b200attn_decode_workspace_bytes(num_users, num_q_heads, head_size, num_splits);
+    if (num_splits > 1 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+      return B200ATTN_ERR_WORKSPACE;
+  }
 
   CUtensorMap tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * num_kv_heads * block_size;
@@ -871,7 +887,14 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   p.per_head = per_head;
   p.page_table_head_stride = page_table_head_stride;
   p.keep_nan = scaled ? 1 : 0;
-  if (num_splits > 1) {
+  if (scaled) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const size_t rows_p = static_cast<size_t>(decode_scaled_ctas(dev->sm_count, pairs, num_splits)) *
+                          (num_splits > 0 ? 1 : 2) * group;
+    p.tickets = reinterpret_cast<unsigned int*>(ws);
+    p.part_o = reinterpret_cast<float*>(ws + kDecTicketBytes);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + rows_p * head_size);
+  } else if (num_splits > 1) {
     const size_t rows_p = static_cast<size_t>(num_users) * num_q_heads * num_splits;
     size_t o_bytes = rows_p * head_size * sizeof(float);
     o_bytes = (o_bytes + 255) & ~static_cast<size_t>(255);
@@ -886,13 +909,15 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (scaled) {
-    const DecodeScaledParams sp{p, k_scale, v_scale};
+    const int whole = pairs * static_cast<int64_t>(sizeof(unsigned int)) > kDecTicketBytes;
+    const DecodeScaledParams sp{p, k_scale, v_scale, static_cast<int>(pairs), whole};
+    const int ctas = static_cast<int>(decode_scaled_ctas(dev->sm_count, pairs, num_splits));
     const int fmt = fp8 ? kPageE4m3 : kPageInt8;
     if (head_size == 128)
-      return block_size == 64 ? launch_decode_scaled_fmt<128, 64>(fmt, tk, tv, sp, num_users, s)
-                              : launch_decode_scaled_fmt<128, 32>(fmt, tk, tv, sp, num_users, s);
-    return block_size == 64 ? launch_decode_scaled_fmt<64, 64>(fmt, tk, tv, sp, num_users, s)
-                            : launch_decode_scaled_fmt<64, 32>(fmt, tk, tv, sp, num_users, s);
+      return block_size == 64 ? launch_decode_scaled_fmt<128, 64>(fmt, tk, tv, sp, ctas, s)
+                              : launch_decode_scaled_fmt<128, 32>(fmt, tk, tv, sp, ctas, s);
+    return block_size == 64 ? launch_decode_scaled_fmt<64, 64>(fmt, tk, tv, sp, ctas, s)
+                            : launch_decode_scaled_fmt<64, 32>(fmt, tk, tv, sp, ctas, s);
   }
   if (fp8)
     return block_size == 64 ? launch_decode_fp8<64, 6>(tk, tv, p, num_users, s)
@@ -944,9 +969,19 @@ int b200attn_paged_decode_blocks(void* out, int64_t out_row_stride, const void* 
                     workspace_bytes, stream);
 }
 
-int b200attn_decode_blocks_auto_splits(int num_users, int num_kv_heads, int head_size,
-                                       int max_context_len) {
-  return b200attn_decode_auto_splits(num_users, num_kv_heads, head_size, max_context_len);
+size_t b200attn_decode_scaled_workspace_bytes(int num_users, int num_q_heads, int num_kv_heads,
+                                              int head_size, int num_splits) {
+  if (num_users <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_size <= 0 ||
+      num_splits < 0)
+    return 0;
+  int sm = 148;
+  DeviceInfo* dev;
+  if (get_device(&dev) == B200ATTN_OK) sm = dev->sm_count;
+  const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
+  const int group = num_q_heads / num_kv_heads;
+  const size_t a = decode_scaled_bytes(sm, pairs, group, head_size, num_splits);
+  const size_t b = decode_scaled_bytes(sm, pairs, group, head_size, 0);
+  return a > b ? a : b;
 }
 
 // ------------------------------------------------------- norms + rotation, block-scaled writes

@@ -5,8 +5,12 @@
 //   out = sum_j 2^(s_j - m) vs(page of j) c'_j / sum_j 2^(s_j - m)
 //
 // HBM-bound: a key and value cost 2 * head_size bytes and are read once.  As in the bf16 kernel a
-// CTA owns one KV head of one user (and a slice of the context), a producer warp keeps a ring of
-// tiles full with TMA, and four warps take a quarter of a tile each.  What differs:
+// CTA works on one KV head of one user at a time, a producer warp keeps a ring of tiles full with
+// TMA, and four warps take a quarter of a tile each.  What differs:
+//   * the launch is one CTA per resident slot and the tiles of all (user, KV head) pairs, end to
+//     end, are dealt to them in equal shares: no wave is partly filled and ragged contexts balance.
+//     A share covers the end of one pair, whole pairs and the start of another; the ring runs on
+//     across them.  A pair that several CTAs share is merged by the one that finishes last;
 //   * the products are transposed: S^T = K Q^T and O^T = V^T P^T, tokens resp. head elements in
 //     the 16 rows of m16n8k16 and the query heads in its 8 columns.  Up to 8 query heads per KV
 //     head then fill an MMA (otherwise half of the 16 rows would be padding), and the
@@ -38,15 +42,17 @@
 namespace b200attn {
 
 struct DecodeScaledParams {
-  DecodeParams d;
+  DecodeParams d;            // num_splits == 0: equal shares; part_o / part_ml: [slot][G] rows
   const float* k_scale;      // [num_blocks, num_kv_heads]
   const float* v_scale;
+  int num_pairs;             // users * KV heads
+  int whole_pairs;           // equal shares rounded to pairs (more pairs than arrival counters)
 };
 
 constexpr int kDsTile = 128;           // tokens per pipeline stage
 constexpr int kDsWarpTokens = 32;      // of them per consumer warp
 
-template <int HD, int BS, int STAGES>
+template <int HD, int BS, int NG, int STAGES>
 struct DecodeScaledSmem {
   static constexpr int kPages = kDsTile / BS;
   static constexpr int kBoxBytes = BS * HD;                    // one page of one head
@@ -55,7 +61,14 @@ struct DecodeScaledSmem {
   static constexpr int kRingBytes = STAGES * kStageBytes;
   static constexpr int kScaleBytes = STAGES * kPages * 8;      // (K scale, log2 of the V scale)
   static constexpr int kBarrierBytes = 2 * STAGES * 8 + 16;
-  static constexpr int kTotalBytes = kRingBytes + kScaleBytes + kBarrierBytes + 1024;
+  static constexpr int kRow = HD + 4;                          // padded: fewer bank conflicts
+  // merge of the warps, two at a time: rows of 8 NG heads and their (max, scale max, sum)
+  static constexpr int kMergeBytes = 2 * 8 * NG * (kRow + 4) * 4;
+  static constexpr int kMergeOff = kRingBytes + kScaleBytes + kBarrierBytes;
+  static constexpr int kPlanOff = kMergeOff + kMergeBytes;     // the CTA's share; block scan
+  static constexpr int kTotalBytes = kPlanOff + 128 + 1024;
+  static_assert(kMergeOff % 16 == 0 && kPlanOff % 16 == 0, "vector access");
+  static_assert((8 * NG * (32 + 2) + 1) * 4 <= kMergeBytes, "the merge of partials fits");
 };
 
 // Four codes in a word -> f16 pairs (bytes 0, 2) and (bytes 1, 3), exact.
@@ -85,47 +98,115 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
 
 constexpr float kScoreSlack = 8.f;   // log2 units a score may pass the running maximum by
 
-// decode_split_finish for this kernel: the same protocol (the split that arrives last merges), with
-// the partial rows read as 16-byte vectors, eight splits in flight per thread: the merge is one CTA
-// reading splits * G * head_size floats, and its time is their latency.
-template <int HD>
-__device__ __forceinline__ void decode_scaled_finish(const DecodeParams& p, int user, int kvh,
-                                                     float* scratch, int tid) {
+// A run of tiles of one (user, KV head) pair that one CTA works on.
+struct DsSegment {
+  int user, kvh, ctx, lo;    // keys lo .. ctx - 1 are attended
+  int t_begin, t_end;        // tiles
+  int n_tiles;               // of the pair in all
+  int64_t pair_pos;          // where the pair's tiles start among all pairs' tiles
+};
+
+// First attended key and tiles of a pair.
+__device__ __forceinline__ int ds_pair_tiles(const DecodeParams& p, int user, int kvh, int* ctx_out,
+                                             int* lo_out) {
+  const int ctx = decode_cur_pos(p, user, kvh) + 1;
+  const int lo = (p.window > 0 && ctx > p.window) ? ctx - p.window : 0;
+  *ctx_out = ctx;
+  *lo_out = lo;
+  return ctx > 0 ? (ctx + kDsTile - 1) / kDsTile - lo / kDsTile : 0;
+}
+
+// The CTA's share of the work, walked segment by segment by every warp for itself.
+struct DsShare {
+  int64_t pos, end;          // tiles [pos, end) of all pairs' tiles
+  int pair, offset;          // the pair that pos lies in, and the tile within it
+  int64_t total;             // tiles of all pairs
+  int shares;                // CTAs that have a share
+
+  // Next segment; false at the end of the share.  Empty pairs are passed over.
+  __device__ __forceinline__ bool next(const DecodeScaledParams& sp, DsSegment& s) {
+    const DecodeParams& p = sp.d;
+    while (pos < end && pair < sp.num_pairs) {
+      s.user = pair / p.num_kv_heads;
+      s.kvh = pair - s.user * p.num_kv_heads;
+      s.n_tiles = ds_pair_tiles(p, s.user, s.kvh, &s.ctx, &s.lo);
+      const int first = offset, left = s.n_tiles - first;
+      if (sp.whole_pairs && first > 0) {       // the pair belongs to the share it starts in
+        pos += left;
+        ++pair;
+        offset = 0;
+        continue;
+      }
+      const int n = sp.whole_pairs ? left : static_cast<int>(min(static_cast<int64_t>(left), end - pos));
+      s.pair_pos = pos - first;
+      s.t_begin = s.lo / kDsTile + first;
+      s.t_end = s.t_begin + n;
+      pos += n;
+      offset = 0;
+      ++pair;
+      if (n > 0) return true;
+    }
+    return false;
+  }
+};
+
+// Share of CTA c of n over `total` tiles: [c total / n, (c + 1) total / n).
+__device__ __forceinline__ int64_t ds_share_start(int64_t total, int shares, int c) {
+  return static_cast<int64_t>(c) * total / shares;
+}
+// The share that tile x lies in (the inverse of the above).
+__device__ __forceinline__ int ds_share_of(int64_t total, int shares, int64_t x) {
+  return static_cast<int>(((x + 1) * shares - 1) / total);
+}
+
+// Where the partials of a shared pair lie: the i-th in slot first (i = 0) or base + i * step.
+struct DsSlots {
+  int64_t first, base;
+  int step, count;
+  __device__ __forceinline__ int64_t operator()(int i) const { return i == 0 ? first : base + i * step; }
+};
+
+// End of a segment that is not its pair's only one: the partial rows are in global memory, written
+// by warp 0.  Whoever of the pair's CTAs arrives last (a ticket) finds all of them published and
+// merges them; nobody waits.  The merge is one CTA reading count * G * head_size floats and its time
+// is their latency: every thread keeps several 16-byte loads in flight for each of the vectors it
+// owns.  Called by the consumer threads; `scratch` is shared memory of kMergeBytes.
+template <int HD, int NG>
+__device__ __forceinline__ void ds_finish(const DecodeParams& p, int user, int kvh,
+                                          const DsSlots& slots, float* scratch, int tid) {
   constexpr int kThreads = kDecConsumerWarps * 32;
-  const int S = p.num_splits, G = p.group;
-  float* fac = scratch;                    // [G][S] running max of a split, then its merge factor
-  float* row_m = scratch + 16 * S;         // [G] merged max
-  float* row_l = row_m + 16;               // [G] merged sum
-  volatile int* last_flag = reinterpret_cast<volatile int*>(row_l + 16);
+  constexpr int kChunk = 32;               // partials whose weights are held at once
+  constexpr int kVec = HD / 4;
+  constexpr int kItems = 8 * NG * kVec / kThreads;       // vectors per thread
+  constexpr int kBatch = kItems > 2 ? 4 : 8;             // loads in flight for each
+  const int G = p.group, count = slots.count;
+  float* weight = scratch;                 // [8 NG][kChunk]
+  float* row_m = weight + 8 * NG * kChunk;               // [8 NG] merged max
+  float* row_l = row_m + 8 * NG;                         // [8 NG] merged sum
+  volatile int* last_flag = reinterpret_cast<volatile int*>(row_l + 8 * NG);
   unsigned int* ticket = p.tickets + static_cast<int64_t>(user) * p.num_kv_heads + kvh;
 
-  __threadfence();                         // this thread's partial stores, device-wide
-  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-  if (tid == 0) *last_flag = atomicAdd(ticket, 1u) == static_cast<unsigned int>(S - 1);
+  if (tid < 32) {
+    __threadfence();                       // this lane's partial stores, device-wide
+    __syncwarp();
+    if (tid == 0) {
+      *last_flag = atomicAdd(ticket, 1u) == static_cast<unsigned int>(count - 1);
+      __threadfence();
+    }
+  }
   asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
   if (!*last_flag) return;
-  __threadfence();
   if (tid == 0) *ticket = 0u;              // leave the counter as the next launch expects it
 
-  const int64_t row0 = (static_cast<int64_t>(user) * p.num_q_heads + kvh * G) * S;
   const int warp = tid >> 5, lane = tid & 31;
   for (int r = warp; r < G; r += kDecConsumerWarps) {
-    const float2* ml = p.part_ml + row0 + static_cast<int64_t>(r) * S;
     float m = -INFINITY, l = 0.f;
-    // two passes over at most kDecMaxSplits pairs: they stay in registers
-    float2 v[kDecMaxSplits / 32];
-#pragma unroll
-    for (int i = 0; i < kDecMaxSplits / 32; ++i) {
-      v[i] = i * 32 + lane < S ? __ldcg(ml + i * 32 + lane) : make_float2(-INFINITY, 0.f);
-      m = fmaxf(m, v[i].x);
-    }
+    for (int i = lane; i < count; i += 32) m = fmaxf(m, __ldcg(p.part_ml + slots(i) * G + r).x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-    for (int i = 0; i < kDecMaxSplits / 32; ++i) {
-      const float f = v[i].x == -INFINITY ? 0.f : fast_exp2(v[i].x - m);   // empty splits: -inf
-      l += f * v[i].y;
-      if (i * 32 + lane < S) fac[r * S + i * 32 + lane] = f;
+    for (int i = lane; i < count; i += 32) {
+      const float2 v = __ldcg(p.part_ml + slots(i) * G + r);
+      l += (v.x == -INFINITY ? 0.f : fast_exp2(v.x - m)) * v.y;   // -inf: attended nothing
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -134,47 +215,69 @@ __device__ __forceinline__ void decode_scaled_finish(const DecodeParams& p, int 
       row_l[r] = l;
     }
   }
-  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-  constexpr int kVec = HD / 4;
-  for (int i = tid; i < G * kVec; i += kThreads) {
-    const int r = i / kVec, d = (i - r * kVec) * 4;
-    const float* src = p.part_o + (row0 + static_cast<int64_t>(r) * S) * HD + d;
-    float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-    for (int s0 = 0; s0 < S; s0 += 8) {
-      float4 x[8];
-      float f[8];
+  float acc[kItems][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // an empty split published no rows: its memory must not be read into the sum
-        f[j] = s0 + j < S ? fac[r * S + s0 + j] : 0.f;
-        x[j] = f[j] != 0.f ? __ldcg(reinterpret_cast<const float4*>(
-                                 src + static_cast<int64_t>(s0 + j) * HD))
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < kItems; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
+  for (int s0 = 0; s0 < count; s0 += kChunk) {
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    for (int i = tid; i < 8 * NG * kChunk; i += kThreads) {
+      const int r = i / kChunk, j = s0 + i % kChunk;
+      float w = 0.f;                       // also for a partial that attended nothing
+      if (r < G && j < count) {
+        const float m = __ldcg(p.part_ml + slots(j) * G + r).x;
+        if (m != -INFINITY) w = fast_exp2(m - row_m[r]);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a0 += f[j] * x[j].x;
-        a1 += f[j] * x[j].y;
-        a2 += f[j] * x[j].z;
-        a3 += f[j] * x[j].w;
-      }
+      weight[i] = w;
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    const int n = min(kChunk, count - s0);
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += kBatch) {
+      float4 x[kItems][kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int64_t row = slots(s0 + min(j0 + j, n - 1)) * G;
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+          const int i = tid + k * kThreads, r = min(i / kVec, G - 1), d = (i % kVec) * 4;
+          x[k][j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (row + r) * HD + d));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+          const int r = min((tid + k * kThreads) / kVec, G - 1);
+          const float w = j0 + j < n ? weight[r * kChunk + j0 + j] : 0.f;
+          if (w != 0.f) {                  // what a zero weight stands for may be no row at all
+            acc[k][0] += w * x[k][j].x;
+            acc[k][1] += w * x[k][j].y;
+            acc[k][2] += w * x[k][j].z;
+            acc[k][3] += w * x[k][j].w;
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int i = tid + k * kThreads, r = i / kVec, d = (i % kVec) * 4;
+    if (r >= G) break;
     float m = row_m[r], l = row_l[r];
     const int head = kvh * G + r;
     float by = p.sinks ? apply_sink(m, l, p.sinks[head] * 1.4426950408889634f) : 1.f;
     by = l > 0.f || l != l ? by / l : 0.f;
     uint2 y;
-    y.x = pack_bf16x2(a0 * by, a1 * by);
-    y.y = pack_bf16x2(a2 * by, a3 * by);
+    y.x = pack_bf16x2(acc[k][0] * by, acc[k][1] * by);
+    y.y = pack_bf16x2(acc[k][2] * by, acc[k][3] * by);
     *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(user) * p.out_row_stride + head * HD + d) = y;
   }
 }
 
 template <int HD, int BS, int FMT, int NG, int STAGES>
-__global__ void __launch_bounds__(kDecThreads)
+__global__ void __launch_bounds__(kDecThreads, 2)
 paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const DecodeScaledParams sp) {
-  using L = DecodeScaledSmem<HD, BS, STAGES>;
+  using L = DecodeScaledSmem<HD, BS, NG, STAGES>;
   const DecodeParams& p = sp.d;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -183,44 +286,15 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(ring + L::kRingBytes + L::kScaleBytes);
   uint64_t* empty_bar = full_bar + STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty_bar + STAGES);
+  int64_t* plan = reinterpret_cast<int64_t*>(ring + L::kPlanOff);   // [0..4] warp sums, [5] total
+  int* plan_at = reinterpret_cast<int*>(plan + 6);                  // pair and offset of the start
 
   // A CTA of this launch just gave up on a wait: do not repeat the timeout per CTA.
   if (timeout_drain_window(p.err_word)) return;
 
-  const int split = blockIdx.x;
-  const int kvh = blockIdx.y;
-  const int user = blockIdx.z;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-
-  const int ctx = decode_cur_pos(p, user, kvh) + 1;  // keys 0 .. cur_pos
-  const int lo = (p.window > 0 && ctx > p.window) ? ctx - p.window : 0;   // first key attended
-  const int n_tiles = ctx > 0 ? (ctx + kDsTile - 1) / kDsTile : 0;
-  const int t_lo = lo / kDsTile;
-  const int tiles_per_split = (n_tiles - t_lo + p.num_splits - 1) / p.num_splits;
-  const int t_begin = t_lo + split * tiles_per_split;
-  const int t_end = min(n_tiles, t_begin + tiles_per_split);
   const int G = p.group;
-
-  if (t_begin >= t_end) {
-    // Nothing for this split: publish an empty partial (or zeros when it is the only split).
-    if (p.num_splits > 1) {
-      if (threadIdx.x < G) {
-        const int64_t row = (static_cast<int64_t>(user) * p.num_q_heads + kvh * G + threadIdx.x) *
-                                p.num_splits + split;
-        p.part_ml[row] = make_float2(-INFINITY, 0.f);
-      }
-      if (p.tickets && threadIdx.x < kDecConsumerWarps * 32)
-        decode_scaled_finish<HD>(p, user, kvh, reinterpret_cast<float*>(ring), threadIdx.x);
-    } else {
-      for (int i = threadIdx.x; i < G * HD; i += blockDim.x) {
-        const int r = i / HD, d = i - r * HD;
-        p.out[static_cast<int64_t>(user) * p.out_row_stride + (kvh * G + r) * HD + d] =
-            __float2bfloat16(0.f);
-      }
-    }
-    return;
-  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -230,7 +304,80 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     *abort_flag = 0;
     mbar_fence_init();
   }
+  // ---- this CTA's share of the tiles
+  DsShare share;
+  if (p.num_splits > 0) {
+    // every pair cut into num_splits (or as many as it has tiles): one segment
+    share.pair = blockIdx.x / p.num_splits;
+    const int split = blockIdx.x - share.pair * p.num_splits;
+    int ctx, lo;
+    const int user = share.pair / p.num_kv_heads;
+    const int n = ds_pair_tiles(p, user, share.pair - user * p.num_kv_heads, &ctx, &lo);
+    share.total = n;
+    share.shares = min(p.num_splits, n);
+    share.pos = split < share.shares ? ds_share_start(n, share.shares, split) : 0;
+    share.end = split < share.shares ? ds_share_start(n, share.shares, split + 1) : 0;
+    share.offset = static_cast<int>(share.pos);
+  } else {
+    // all pairs' tiles in equal shares: a prefix sum over the pairs finds the start of this one
+    const int per = (sp.num_pairs + kDecThreads - 1) / kDecThreads;
+    const int first = min(sp.num_pairs, static_cast<int>(threadIdx.x) * per);
+    const int last = min(sp.num_pairs, first + per);
+    int64_t mine = 0;
+    int ctx, lo;
+    for (int q = first; q < last; ++q)
+      mine += ds_pair_tiles(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) plan[warp] = incl;
+    __syncthreads();
+    int64_t before = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kDecThreads / 32; ++w) {
+      if (w < warp) before += plan[w];
+      total += plan[w];
+    }
+    share.total = total;
+    share.shares = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+    const int c = blockIdx.x;
+    const bool has = c < share.shares;
+    share.pos = has ? ds_share_start(total, share.shares, c) : 0;
+    share.end = has ? ds_share_start(total, share.shares, c + 1) : 0;
+    if (has && share.pos >= before && share.pos < before + mine) {
+      int q = first;
+      for (;; ++q) {
+        const int n = ds_pair_tiles(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
+        if (share.pos < before + n) break;
+        before += n;
+      }
+      plan_at[0] = q;
+      plan_at[1] = static_cast<int>(share.pos - before);
+    }
+    __syncthreads();
+    share.pair = plan_at[0];
+    share.offset = plan_at[1];
+  }
+  // rows of pairs without context are zeros
+  {
+    const int step = p.num_splits > 0 ? sp.num_pairs : static_cast<int>(gridDim.x);
+    int q = p.num_splits > 0 ? (blockIdx.x % p.num_splits == 0 ? blockIdx.x / p.num_splits
+                                                               : sp.num_pairs)
+                             : blockIdx.x;
+    for (; q < sp.num_pairs; q += step) {
+      int ctx, lo;
+      const int user = q / p.num_kv_heads, kvh = q - user * p.num_kv_heads;
+      if (ds_pair_tiles(p, user, kvh, &ctx, &lo) > 0) continue;
+      for (int i = threadIdx.x; i < G * HD; i += kDecThreads)
+        p.out[static_cast<int64_t>(user) * p.out_row_stride + kvh * G * HD + i] = __float2bfloat16(0.f);
+    }
+  }
   __syncthreads();
+  if (share.pos >= share.end) return;
+  DsSegment seg;
 
   if (warp == kDecConsumerWarps) {
     // ------------------------------------------------------------------ producer warp
@@ -239,82 +386,87 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       prefetch_tensormap(&tm_v);
     }
     const uint64_t policy = l2_policy_evict_first();
-    const int n_pages = (ctx + BS - 1) / BS;
-    const int32_t* pt = decode_page_row(p, user, kvh);
     // Each lane keeps the id and the scales of one page of a 32-page window; the next window is
-    // fetched early, so only the first tiles wait for a page's scales.
+    // fetched early, so only the first tiles of a segment wait for a page's scales.
     struct Window {
       int id;
       float ks, vs;     // K scale, log2 of the V scale
     };
-    auto fetch = [&](int base) {
-      Window w;
-      const int idx = min(min(base + lane, n_pages - 1), p.page_table_width - 1);
-      w.id = pt[idx];
-      const bool ok = w.id >= 0 && w.id < p.num_blocks;
-      const int64_t at = ok ? static_cast<int64_t>(w.id) * p.num_kv_heads + kvh : kvh;
-      w.ks = __ldg(sp.k_scale + at);
-      w.vs = __log2f(__ldg(sp.v_scale + at));
-      return w;
-    };
-    int win_base = t_begin * L::kPages;
-    Window cur = fetch(win_base), nxt = fetch(win_base + 32);
-    auto advance = [&](int page_idx) {
-      if (page_idx - win_base >= 32) {
-        win_base += 32;
-        cur = nxt;
-        nxt = fetch(win_base + 32);
-      }
-    };
-    // the loads of a tile's pages, not of those past the context (the stage's barrier takes their
-    // bytes before it is armed ...)
-    auto pages_of = [&](int t) { return min(L::kPages, n_pages - t * L::kPages); };
-    auto load_tile = [&](int t, int stage) {
-      const int live = pages_of(t);
-      uint8_t* kdst = ring + stage * L::kStageBytes;
-      uint8_t* vdst = kdst + L::kTensorBytes;
-#pragma unroll
-      for (int pg = 0; pg < L::kPages; ++pg) {
-        if (pg >= live) break;
-        const int page_idx = t * L::kPages + pg;
-        advance(page_idx);
-        int64_t blk = __shfl_sync(0xffffffffu, cur.id, page_idx - win_base);
-        if (blk < 0 || blk >= p.num_blocks) {
-          if (lane == 0) atomicExch(p.err_word, kDevBadIndex);
-          blk = 0;
+    uint32_t it = 0;    // tiles since the start of the share
+    while (share.next(sp, seg)) {
+      const int kvh = seg.kvh;
+      const int n_pages = (seg.ctx + BS - 1) / BS;
+      const int32_t* pt = decode_page_row(p, seg.user, kvh);
+      auto fetch = [&](int base) {
+        Window w;
+        const int idx = min(min(base + lane, n_pages - 1), p.page_table_width - 1);
+        w.id = pt[idx];
+        const bool ok = w.id >= 0 && w.id < p.num_blocks;
+        const int64_t at = ok ? static_cast<int64_t>(w.id) * p.num_kv_heads + kvh : kvh;
+        w.ks = __ldg(sp.k_scale + at);
+        w.vs = __log2f(__ldg(sp.v_scale + at));
+        return w;
+      };
+      int win_base = seg.t_begin * L::kPages;
+      Window cur = fetch(win_base), nxt = fetch(win_base + 32);
+      // the loads of a tile's pages, not of those past the context (the stage's barrier takes their
+      // bytes before it is armed ...)
+      auto pages_of = [&](int t) { return min(L::kPages, n_pages - t * L::kPages); };
+      auto load_tile = [&](int t, int stage) {
+        const int live = pages_of(t);
+        uint8_t* kdst = ring + stage * L::kStageBytes;
+        uint8_t* vdst = kdst + L::kTensorBytes;
+        if (t * L::kPages - win_base >= 32) {     // windows start at a tile and hold whole tiles
+          win_base += 32;
+          cur = nxt;
+          nxt = fetch(win_base + 32);
         }
-        if (lane == 0) {
-          const int32_t y = static_cast<int32_t>((blk * p.num_kv_heads + kvh) * (BS * HD / 128));
-          tma_load_2d(kdst + pg * L::kBoxBytes, &tm_k, &full_bar[stage], 0, y, policy);
-          tma_load_2d(vdst + pg * L::kBoxBytes, &tm_v, &full_bar[stage], 0, y, policy);
-        }
-      }
-    };
-    // (... here) and its scales
-    auto arm_tile = [&](int t, int stage) {
-      const int live = pages_of(t);
 #pragma unroll
-      for (int pg = 0; pg < L::kPages; ++pg) {
-        if (pg >= live) break;
-        const int page_idx = t * L::kPages + pg;
-        const float ks = __shfl_sync(0xffffffffu, cur.ks, page_idx - win_base);
-        const float vs = __shfl_sync(0xffffffffu, cur.vs, page_idx - win_base);
-        if (lane == 0) scales[stage * L::kPages + pg] = make_float2(ks, vs);
+        for (int pg = 0; pg < L::kPages; ++pg) {
+          if (pg >= live) break;
+          const int page_idx = t * L::kPages + pg;
+          int64_t blk = __shfl_sync(0xffffffffu, cur.id, page_idx - win_base);
+          if (blk < 0 || blk >= p.num_blocks) {
+            if (lane == 0) atomicExch(p.err_word, kDevBadIndex);
+            blk = 0;
+          }
+          if (lane == 0) {
+            const int32_t y = static_cast<int32_t>((blk * p.num_kv_heads + kvh) * (BS * HD / 128));
+            tma_load_2d(kdst + pg * L::kBoxBytes, &tm_k, &full_bar[stage], 0, y, policy);
+            tma_load_2d(vdst + pg * L::kBoxBytes, &tm_v, &full_bar[stage], 0, y, policy);
+          }
+        }
+      };
+      // (... here) and its scales
+      auto arm_tile = [&](int t, int stage) {
+        const int live = pages_of(t);
+#pragma unroll
+        for (int pg = 0; pg < L::kPages; ++pg) {
+          if (pg >= live) break;
+          const int page_idx = t * L::kPages + pg;
+          const float ks = __shfl_sync(0xffffffffu, cur.ks, page_idx - win_base);
+          const float vs = __shfl_sync(0xffffffffu, cur.vs, page_idx - win_base);
+          if (lane == 0) scales[stage * L::kPages + pg] = make_float2(ks, vs);
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], live * 2 * L::kBoxBytes);
+      };
+      static_assert(32 % L::kPages == 0, "a window holds whole tiles");
+      static_assert(STAGES * L::kPages <= 32, "the first fill stays in one window");
+      int t = seg.t_begin;
+      if (it == 0) {
+        // first fill: all loads go out before anything waits for a scale
+        const int first = min(seg.t_end, t + STAGES);
+        for (int j = t; j < first; ++j) load_tile(j, j - t);
+        for (int j = t; j < first; ++j) arm_tile(j, j - t);
+        it = first - t;
+        t = first;
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full_bar[stage], live * 2 * L::kBoxBytes);
-    };
-    // First fill: all loads go out before anything waits for a scale (all of these pages are in
-    // the first window).
-    static_assert(STAGES * L::kPages <= 32, "the first fill stays in one window");
-    const int first = min(t_end, t_begin + STAGES);
-    for (int t = t_begin; t < first; ++t) load_tile(t, t - t_begin);
-    for (int t = t_begin; t < first; ++t) arm_tile(t, t - t_begin);
-    for (int t = first; t < t_end; ++t) {
-      const int it = t - t_begin;
-      const int stage = it % STAGES;
-      mbar_wait(&empty_bar[stage], ((it / STAGES) & 1) ^ 1, abort_flag, p.err_word);
-      load_tile(t, stage);
-      arm_tile(t, stage);
+      for (; t < seg.t_end; ++t, ++it) {
+        const int stage = it % STAGES;
+        mbar_wait(&empty_bar[stage], ((it / STAGES) & 1) ^ 1, abort_flag, p.err_word);
+        load_tile(t, stage);
+        arm_tile(t, stage);
+      }
     }
     return;  // consumers wait on every full barrier, so no copy is in flight at kernel end
   }
@@ -324,6 +476,24 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   const int tq = lane & 3;
   static_assert(kDecConsumerWarps * kDsWarpTokens == kDsTile && BS % kDsWarpTokens == 0, "");
 
+  // Per-lane ldmatrix addressing inside a tile: token t's head_size bytes start at t * HD; 128-byte
+  // rows, 16-byte chunks XOR-swizzled with the row's low three bits (the two halves of a warp's
+  // tokens are a multiple of 8 rows apart: same swizzle).  Matrix lane / 8: token half of the 16
+  // (bit 0) and chunk of a pair (bit 1), for K and for V.
+  const int lm = lane >> 3, lr = lane & 7;
+  const int tok = warp * kDsWarpTokens + (lm & 1) * 8 + lr;
+  const uint32_t row = static_cast<uint32_t>(tok * HD) >> 7;
+  const uint32_t chunk0 = ((static_cast<uint32_t>(tok * HD) & 127u) >> 4) + (lm >> 1);
+  uint32_t at[HD / 32];
+#pragma unroll
+  for (int cp = 0; cp < HD / 32; ++cp) at[cp] = (row << 7) + (((chunk0 + 2 * cp) ^ (row & 7)) << 4);
+  constexpr uint32_t kHalf = 16 * HD;      // bytes from a warp's first 16 tokens to its second
+
+  float* mo = reinterpret_cast<float*>(ring + L::kMergeOff);       // [2][8 NG heads][kRow]
+  float4* ms = reinterpret_cast<float4*>(mo + 2 * 8 * NG * L::kRow);   // [2][8 NG] m, r, l
+  uint32_t it = 0;                  // tiles since the start of the share
+  int segments = 0;
+  while (share.next(sp, seg)) {
   // Q fragments (B operand, columns = query heads 8 ng + g; heads >= G are zero).  Within the
   // 16 elements of k-step ks the thread holds 4tq .. 4tq+3; slots {2tq, 2tq+1} take elements 0
   // and 2 of these, slots {2tq+8, 2tq+9} elements 1 and 3: the order codes_to_f16 gives.
@@ -334,8 +504,8 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     const int head = ng * 8 + g;
     uint2 raw[HD / 16];
     uint32_t top = 0;
-    const __nv_bfloat16* qrow = p.q + static_cast<int64_t>(user) * p.q_row_stride +
-                                (static_cast<int64_t>(kvh) * G + head) * HD;
+    const __nv_bfloat16* qrow = p.q + static_cast<int64_t>(seg.user) * p.q_row_stride +
+                                (static_cast<int64_t>(seg.kvh) * G + head) * HD;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
       raw[ks] = head < G ? *reinterpret_cast<const uint2*>(qrow + ks * 16 + tq * 4)
@@ -379,25 +549,12 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     }
   }
 
-  // Per-lane ldmatrix addressing inside a tile: token t's head_size bytes start at t * HD; 128-byte
-  // rows, 16-byte chunks XOR-swizzled with the row's low three bits (the two halves of a warp's
-  // tokens are a multiple of 8 rows apart: same swizzle).  Matrix lane / 8: token half of the 16
-  // (bit 0) and chunk of a pair (bit 1), for K and for V.
-  const int lm = lane >> 3, lr = lane & 7;
-  const int tok = warp * kDsWarpTokens + (lm & 1) * 8 + lr;
-  const uint32_t row = static_cast<uint32_t>(tok * HD) >> 7;
-  const uint32_t chunk0 = ((static_cast<uint32_t>(tok * HD) & 127u) >> 4) + (lm >> 1);
-  uint32_t at[HD / 32];
-#pragma unroll
-  for (int cp = 0; cp < HD / 32; ++cp) at[cp] = (row << 7) + (((chunk0 + 2 * cp) ^ (row & 7)) << 4);
-  constexpr uint32_t kHalf = 16 * HD;      // bytes from a warp's first 16 tokens to its second
-
-  for (int t = t_begin; t < t_end; ++t) {
-    const int it = t - t_begin;
+  for (int t = seg.t_begin; t < seg.t_end; ++t, ++it) {
     const int stage = it % STAGES;
     mbar_wait(&full_bar[stage], (it / STAGES) & 1, abort_flag, p.err_word);
     const uint32_t kbase = smem_u32(ring + stage * L::kStageBytes);
     const uint32_t vbase = kbase + L::kTensorBytes;
+    const int ctx = seg.ctx, lo = seg.lo;
     const int tok0 = t * kDsTile + warp * kDsWarpTokens;   // first token of this warp's slice
 
     if (tok0 < ctx && tok0 + kDsWarpTokens > lo) {  // at least one of this warp's keys is attended
@@ -548,59 +705,97 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       l[ng][j] += __shfl_xor_sync(0xffffffffu, l[ng][j], 8);
       l[ng][j] += __shfl_xor_sync(0xffffffffu, l[ng][j], 16);
     }
-  // All consumer warps are past their last full-barrier wait: the ring is free to reuse.
-  asm volatile("bar.sync 1, %0;" ::"n"(kDecConsumerWarps * 32));
-  constexpr int kRow = HD + 4;                                      // padded: fewer bank conflicts
-  float* so = reinterpret_cast<float*>(ring);                       // [4 warps][8 NG heads][kRow]
-  float* sm = so + kDecConsumerWarps * 8 * NG * kRow;               // [4][8 NG] max of s
-  float* sr = sm + kDecConsumerWarps * 8 * NG;                      // [4][8 NG] max of s - m + log2 vs
-  float* sl = sr + kDecConsumerWarps * 8 * NG;                      // [4][8 NG] sum
-  static_assert(kDecConsumerWarps * 8 * NG * (kRow + 3) * 4 <= L::kRingBytes, "merge scratch fits");
-  static_assert((16 * kDecMaxSplits + 40) * 4 <= L::kRingBytes, "split merge scratch fits");
+  // Warps 2 and 3 hand their rows to warps 0 and 1, then warp 1 to warp 0 (the ring is busy with
+  // the next segment's tiles, so the rows of two warps are what there is room for).
+  auto heads_do = [&](int from, auto f) {
 #pragma unroll
-  for (int ng = 0; ng < NG; ++ng)
+    for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int head = warp * 8 * NG + ng * 8 + 2 * tq + j;
+      for (int j = 0; j < 2; ++j) f(from * 8 * NG + ng * 8 + 2 * tq + j, ng, j);
+  };
+#pragma unroll 1
+  for (int half = kDecConsumerWarps / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) {
+      heads_do(warp - half, [&](int head, int ng, int j) {
 #pragma unroll
-      for (int c = 0; c < HD / 16; ++c)
-        *reinterpret_cast<float2*>(so + head * kRow + c * 16 + 2 * g) =
-            make_float2(o[ng][c][j], o[ng][c][j + 2]);
-      if (g == 0) {
-        sm[head] = m[ng][j];
-        sr[head] = r[ng][j];
-        sl[head] = l[ng][j];
-      }
+        for (int c = 0; c < HD / 16; ++c)
+          *reinterpret_cast<float2*>(mo + head * L::kRow + c * 16 + 2 * g) =
+              make_float2(o[ng][c][j], o[ng][c][j + 2]);
+        if (g == 0) ms[head] = make_float4(m[ng][j], r[ng][j], l[ng][j], 0.f);
+      });
     }
-  asm volatile("bar.sync 1, %0;" ::"n"(kDecConsumerWarps * 32));
-
-  for (int i = threadIdx.x; i < G * HD; i += kDecConsumerWarps * 32) {
-    const int r = i / HD, d = i - r * HD;
-    float mm = -FLT_MAX;
+    asm volatile("bar.sync 1, %0;" ::"n"(kDecConsumerWarps * 32) : "memory");
+    if (warp < half) {
+      heads_do(warp, [&](int head, int ng, int j) {
+        const float4 other = ms[head];
+        // a warp that attended no key has m = -FLT_MAX and a zero sum: factor 0 (or 1 when both)
+        const float mn = fmaxf(m[ng][j], other.x);
+        const float fa = fast_exp2(m[ng][j] - mn), fb = fast_exp2(other.x - mn);
+        const float ra = fmaxf(r[ng][j] + (m[ng][j] - mn), -FLT_MAX);
+        const float rb = fmaxf(other.y + (other.x - mn), -FLT_MAX);
+        const float rn = fmaxf(ra, rb);
+        const float ga = fast_exp2(ra - rn), gb = fast_exp2(rb - rn);
+        m[ng][j] = mn;
+        r[ng][j] = rn;
+        l[ng][j] = l[ng][j] * fa + other.z * fb;
 #pragma unroll
-    for (int w = 0; w < kDecConsumerWarps; ++w) mm = fmaxf(mm, sm[w * 8 * NG + r]);
-    float acc = 0.f, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDecConsumerWarps; ++w) {
-      const int at = w * 8 * NG + r;
-      if (sm[at] == -FLT_MAX && sl[at] == 0.f) continue;   // no key of this warp was attended
-      ll += fast_exp2(sm[at] - mm) * sl[at];
-      acc += exp2f((sm[at] - mm) + sr[at]) * so[at * kRow + d];   // 2^r gives the V scales back
+        for (int c = 0; c < HD / 16; ++c) {
+          const float2 x = *reinterpret_cast<const float2*>(mo + head * L::kRow + c * 16 + 2 * g);
+          o[ng][c][j] = o[ng][c][j] * ga + x.x * gb;
+          o[ng][c][j + 2] = o[ng][c][j + 2] * ga + x.y * gb;
+        }
+      });
     }
-    const int head = kvh * G + r;
-    if (p.num_splits == 1) {
-      if (p.sinks) acc *= apply_sink(mm, ll, p.sinks[head] * 1.4426950408889634f);
-      p.out[static_cast<int64_t>(user) * p.out_row_stride + head * HD + d] =
-          __float2bfloat16(ll > 0.f || ll != ll ? acc / ll : 0.f);
-    } else {
-      const int64_t prow =
-          (static_cast<int64_t>(user) * p.num_q_heads + head) * p.num_splits + split;
-      p.part_o[prow * HD + d] = acc;
-      if (d == 0) p.part_ml[prow] = make_float2(mm == -FLT_MAX && ll == 0.f ? -INFINITY : mm, ll);
-    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kDecConsumerWarps * 32) : "memory");
   }
-  if (p.num_splits > 1 && p.tickets)
-    decode_scaled_finish<HD>(p, user, kvh, reinterpret_cast<float*>(ring), threadIdx.x);
+  // warp 0 holds the segment's rows: 2^r gives the V scales back
+  const bool whole = seg.t_end - seg.t_begin == seg.n_tiles;
+  const int64_t my_slot = p.num_splits > 0 ? blockIdx.x
+                                           : 2 * static_cast<int64_t>(blockIdx.x) + (segments > 0);
+  ++segments;
+  if (warp == 0) {
+    heads_do(0, [&](int, int ng, int j) {
+      const int h = ng * 8 + 2 * tq + j;
+      if (h >= G) return;
+      float mm = m[ng][j], ll = l[ng][j], by = exp2f(r[ng][j]);
+      if (r[ng][j] == -FLT_MAX) by = ll != ll ? NAN : 0.f;      // nothing but zero values
+      if (whole) {
+        const int head = seg.kvh * G + h;
+        if (p.sinks) by *= apply_sink(mm, ll, p.sinks[head] * 1.4426950408889634f);
+        by = ll > 0.f || ll != ll ? by / ll : 0.f;
+        __nv_bfloat16* dst = p.out + static_cast<int64_t>(seg.user) * p.out_row_stride + head * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+          *reinterpret_cast<uint32_t*>(dst + c * 16 + 2 * g) =
+              pack_bf16x2(o[ng][c][j] * by, o[ng][c][j + 2] * by);
+      } else {
+        float* dst = p.part_o + (my_slot * G + h) * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+          *reinterpret_cast<float2*>(dst + c * 16 + 2 * g) =
+              make_float2(o[ng][c][j] * by, o[ng][c][j + 2] * by);
+        if (g == 0)
+          p.part_ml[my_slot * G + h] = make_float2(mm == -FLT_MAX && ll == 0.f ? -INFINITY : mm, ll);
+      }
+    });
+  }
+  if (!whole) {
+    DsSlots slots;
+    if (p.num_splits > 0) {
+      const int64_t pair = static_cast<int64_t>(seg.user) * p.num_kv_heads + seg.kvh;
+      slots = DsSlots{pair * p.num_splits, pair * p.num_splits, 1, share.shares};
+    } else {
+      // a share's first segment has slot 2 c, its last 2 c + 1
+      const int c0 = ds_share_of(share.total, share.shares, seg.pair_pos);
+      const int c1 = ds_share_of(share.total, share.shares, seg.pair_pos + seg.n_tiles - 1);
+      const bool inside = ds_share_start(share.total, share.shares, c0) < seg.pair_pos;
+      slots = DsSlots{2 * static_cast<int64_t>(c0) + (inside ? 1 : 0), 2 * static_cast<int64_t>(c0),
+                      2, c1 - c0 + 1};
+    }
+    ds_finish<HD, NG>(p, seg.user, seg.kvh, slots, reinterpret_cast<float*>(mo), threadIdx.x);
+    asm volatile("bar.sync 1, %0;" ::"n"(kDecConsumerWarps * 32) : "memory");   // mo is free again
+  }
+  }
 }
 
 }  // namespace b200attn
