@@ -1,0 +1,142 @@
+"""Refusals of the block-scaled / page-list / norm entry points, and the shapes that
+allocate_kv_caches makes for them: no GPU needed, nothing is launched."""
+import pytest
+import torch
+
+from b200attn import _lib, sharding
+
+OK, NULL, UNSUPPORTED, MISALIGNED, WORKSPACE, BAD, NO_DEVICE = 0, -1, -2, -3, -4, -5, -6
+BF16, FP8, INT8 = 0, 1, 2
+
+
+@pytest.fixture()
+def L(built_library):
+    return _lib.lib()
+
+
+def _call(fn, args, **changes):
+    args = dict(args)
+    for name, value in changes.items():
+        assert name in args, name
+        args[name] = value
+    return fn(*args.values())
+
+
+WRITE = dict(k=16, v=16, ks=16, vs=16, bounds=None, kind=INT8, kn=16, kstride=256, vn=16,
+             vstride=256, table=16, tstride=4, width=4, cu=None, qlen=None, start=16, seqs=2,
+             tokens=2, nkv=2, hd=128, bs=32, nb=8, stream=None)
+
+
+@pytest.mark.parametrize("changes,status", [
+    (dict(k=None), NULL), (dict(start=None), NULL), (dict(ks=None), NULL), (dict(table=None), NULL),
+    (dict(kind=BF16), BAD), (dict(kind=7), BAD), (dict(seqs=-1), BAD), (dict(width=0), BAD),
+    (dict(tokens=3), BAD), (dict(kstride=128), BAD), (dict(nkv=0), BAD), (dict(nb=0), BAD),
+    (dict(hd=96), UNSUPPORTED), (dict(bs=16), UNSUPPORTED), (dict(kn=8), MISALIGNED),
+    (dict(vstride=260), MISALIGNED), (dict(bounds=4), MISALIGNED),
+])
+def test_paged_write_refusals(L, changes, status):
+    assert _call(L.b200attn_paged_write, WRITE, **changes) == status
+
+
+DECODE = dict(out=16, ostride=1024, q=16, qstride=1024, k=16, v=16, ks=16, vs=16, kind=INT8,
+              table=16, tstride=4, hstride=0, width=4, pos=16, users=2, nq=8, nkv=2, hd=128, bs=32,
+              nb=8, scale=1.0, window=0, sinks=None, ctx=0, splits=0, ws=None, wsbytes=0,
+              stream=None)
+
+
+@pytest.mark.parametrize("changes,status", [
+    (dict(vs=None), NULL), (dict(q=None), NULL), (dict(kind=BF16), BAD), (dict(kind=9), BAD),
+    (dict(ks=None, vs=None, kind=INT8), BAD), (dict(ks=None, vs=None, kind=FP8, hd=64), UNSUPPORTED),
+    (dict(hstride=4, window=8), UNSUPPORTED), (dict(hstride=-4), BAD), (dict(scale=0.0), BAD),
+    (dict(nq=34, qstride=8192, ostride=8192), UNSUPPORTED), (dict(nq=7), BAD),
+    (dict(splits=-1), BAD), (dict(splits=300), -8), (dict(qstride=512), BAD), (dict(q=8), MISALIGNED),
+    (dict(window=-1), BAD),
+])
+def test_paged_decode_blocks_refusals(L, changes, status):
+    assert _call(L.b200attn_paged_decode_blocks, DECODE, **changes) == status
+
+
+SELECT = dict(table_out=16, pos_out=16, q=16, qstride=1024, bounds=16, table=16, tstride=8, width=8,
+              pos=16, users=2, nq=8, nkv=2, hd=128, bs=64, nb=8, pages=4, first=1, last=1, ctx=0,
+              ws=None, wsbytes=0, stream=None)
+
+
+@pytest.mark.parametrize("changes,status", [
+    (dict(q=None), NULL), (dict(bounds=None), NULL), (dict(pages=0), BAD), (dict(last=0), BAD),
+    (dict(first=-1), BAD), (dict(first=3, last=2), BAD), (dict(nq=9), BAD), (dict(width=0), BAD),
+    (dict(nq=40, qstride=8192), UNSUPPORTED), (dict(hd=32), UNSUPPORTED), (dict(bs=128), UNSUPPORTED),
+    (dict(bounds=8), MISALIGNED), (dict(qstride=512), BAD), (dict(pages=1 << 30, first=0), -8),
+    (dict(first=2 ** 31 - 1, last=2 ** 31 - 1), BAD),
+])
+def test_select_pages_refusals(L, changes, status):
+    assert _call(L.b200attn_select_pages, SELECT, **changes) == status
+
+
+NORM = dict(oq=16, oqs=512, ok=16, oks=128, q=16, qs=512, k=16, ks=128, v=16, vs=128, wq=16, wk=16,
+            f32=0, eps=1e-6, pos=16, inv=16, rotary=64, neox=1, kc=16, vc=16, kind=BF16, slots=16,
+            tokens=3, nq=8, nkv=2, hd=64, bs=32, nb=4, stream=None)
+
+
+@pytest.mark.parametrize("changes,status", [
+    (dict(oq=None), NULL), (dict(wk=None), NULL), (dict(kc=None), NULL), (dict(v=None), NULL),
+    (dict(eps=-1.0), BAD), (dict(eps=float("nan")), BAD), (dict(rotary=24), UNSUPPORTED),
+    (dict(rotary=80), UNSUPPORTED), (dict(rotary=0), UNSUPPORTED), (dict(hd=80), UNSUPPORTED),
+    (dict(kind=INT8), BAD), (dict(bs=48), UNSUPPORTED), (dict(tokens=-1), BAD), (dict(qs=504), BAD),
+    (dict(qs=516), MISALIGNED), (dict(wq=8), MISALIGNED), (dict(vs=64), BAD),
+])
+def test_qk_norm_rope_refusals(L, changes, status):
+    assert _call(L.b200attn_qk_norm_rope_kv_scatter_slots, NORM, **changes) == status
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU behaviour")
+def test_nothing_runs_without_a_device(L):
+    for fn, args in ((L.b200attn_paged_write, WRITE), (L.b200attn_paged_decode_blocks, DECODE),
+                     (L.b200attn_select_pages, SELECT),
+                     (L.b200attn_qk_norm_rope_kv_scatter_slots, NORM)):
+        assert fn(*args.values()) == NO_DEVICE
+
+
+def test_workspace_sizes(L):
+    small = L.b200attn_decode_scaled_workspace_bytes(2, 8, 2, 128, 0)
+    assert small >= 65536 + 2 * 2 * 64 * 4 * (128 * 4 + 8)
+    # more users do not grow it beyond the launch's CTAs; explicit splits do
+    assert L.b200attn_decode_scaled_workspace_bytes(4096, 8, 2, 128, 0) == \
+        L.b200attn_decode_scaled_workspace_bytes(1024, 8, 2, 128, 0)
+    assert L.b200attn_decode_scaled_workspace_bytes(1024, 8, 2, 128, 8) >= \
+        65536 + 1024 * 2 * 8 * 4 * (128 * 4 + 8)
+    assert L.b200attn_decode_scaled_workspace_bytes(0, 8, 2, 128, 0) == 0
+    assert L.b200attn_select_pages_workspace_bytes(3, 2, 100) == 65536 + 600 * 16
+
+
+def test_allocated_caches():
+    def shapes(**kw):
+        pair = sharding.allocate_kv_caches(2, 6, 4, 32, 64, tp_size=2, **kw)["layers.1.attn"]
+        return [None if t is None else (tuple(t.shape), t.dtype) for t in pair]
+
+    scale = ((6, 2), torch.float32)
+    bounds = ((6, 2, 2, 64), torch.bfloat16)
+    rows = (6, 2, 32, 64)
+    assert shapes() == [(rows, torch.bfloat16)] * 2
+    assert shapes(dtype=torch.int8) == [(rows, torch.int8)] * 2 + [scale] * 2
+    assert shapes(dtype=torch.float8_e4m3fn) == [(rows, torch.float8_e4m3fn)] * 2
+    assert shapes(dtype=torch.float8_e4m3fn, block_scales=True, page_bounds=True) == \
+        [(rows, torch.float8_e4m3fn)] * 2 + [scale] * 2 + [bounds]
+    assert shapes(page_bounds=True) == [(rows, torch.bfloat16)] * 2 + [None] * 2 + [bounds]
+
+
+def test_ops_refuse_cpu_tensors():
+    from b200attn import ops
+
+    kc = torch.zeros(4, 2, 32, 64, dtype=torch.int8)
+    s = torch.zeros(4, 2)
+    x = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    table, pos = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    w = torch.ones(64)
+    for call in (lambda: ops.paged_write(kc, kc, x, x, table, pos, k_scale=s, v_scale=s),
+                 lambda: ops.paged_decode(x, kc, kc, table, pos, k_scale=s, v_scale=s),
+                 lambda: ops.select_pages(x, torch.zeros(4, 2, 2, 64).bfloat16(), table, pos, 32, 4),
+                 lambda: ops.qk_norm_rope_kv_scatter_slots(
+                     x.flatten(1), x.flatten(1), None, torch.zeros(1, dtype=torch.int64),
+                     torch.ones(32), 64, 64, w, w)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()

@@ -43,6 +43,9 @@ STR_DTYPE_TO_TORCH_DTYPE = {
     "fp8_e5m2": torch.float8_e5m2,
     "int8": torch.int8,
     "uint8": torch.uint8,
+    # 8-bit codes with one fp32 scale per page and KV head (ops.paged_write)
+    "int8_block": torch.int8,
+    "fp8_block": torch.float8_e4m3fn,
 }
 
 DECODER, ENCODER, ENCODER_ONLY = "decoder", "encoder", "encoder_only"
@@ -241,7 +244,8 @@ class B200AttentionBackend:
     accept_output_buffer = True
     forward_includes_kv_cache_update = True
     supported_dtypes = [torch.bfloat16]
-    supported_kv_cache_dtypes = ["auto", "bfloat16", "fp8", "fp8_e4m3"]   # fp8: head_size 128
+    supported_kv_cache_dtypes = ["auto", "bfloat16", "fp8", "fp8_e4m3",   # fp8: head_size 128
+                                 "int8_block", "fp8_block"]
     supported_head_sizes = [64, 128]
     supported_block_sizes = [32, 64]
 
@@ -384,6 +388,23 @@ class PluginBatch:
         return self.query_num_tokens > 1
 
 
+@dataclass
+class PageValues:
+    """What a cache keeps per page and KV head beyond its rows (entries 2 to 4 of a kv_cache list)."""
+
+    k_scale: Optional[torch.Tensor] = None    # fp32 [num_blocks, num_kv_heads]
+    v_scale: Optional[torch.Tensor] = None
+    k_bounds: Optional[torch.Tensor] = None   # bf16 [num_blocks, num_kv_heads, 2, head_size]
+
+    @property
+    def scales(self) -> dict:
+        return {} if self.k_scale is None else dict(k_scale=self.k_scale, v_scale=self.v_scale)
+
+    @property
+    def all(self) -> dict:
+        return dict(k_scale=self.k_scale, v_scale=self.v_scale, k_bounds=self.k_bounds)
+
+
 class B200AttentionBackendImpl:
     """Per-layer attention implementation (attention.py:221-668)."""
 
@@ -400,7 +421,16 @@ class B200AttentionBackendImpl:
         attn_type: str = DECODER,
         kv_sharing_target_layer_name: Optional[str] = None,
         sinks: Optional[torch.Tensor] = None,
+        sparse_pages: Optional[int] = None,
+        sparse_keep_first: int = 1,
+        sparse_keep_last: int = 1,
     ) -> None:
+        """Beyond the reference's arguments: `kv_cache_dtype` "int8_block" / "fp8_block" (caches with
+        a scale per page and KV head: `kv_cache` is then [k, v, k_scale, v_scale]) and
+        `sparse_pages` (decode rows attend that many pages of their context, chosen per KV head by
+        `ops.select_pages`, the first `sparse_keep_first` and the last `sparse_keep_last` always
+        among them: `kv_cache` then carries the key bounds as its fifth entry).
+        `sharding.allocate_kv_caches` makes both."""
         self.num_heads = num_heads
         self.head_size = head_size
         self.scale = float(scale)
@@ -420,7 +450,10 @@ class B200AttentionBackendImpl:
         # The CUDA kernels store bf16 or unscaled e4m3 and refuse the rest instead of silently
         # converting.
         self.kv_cache_quantized_dtype = None
-        if kv_cache_dtype in ("fp8", "fp8_e4m3"):
+        self.block_scaled = kv_cache_dtype in ("int8_block", "fp8_block")
+        if self.block_scaled:
+            self.kv_cache_quantized_dtype = STR_DTYPE_TO_TORCH_DTYPE[kv_cache_dtype]
+        elif kv_cache_dtype in ("fp8", "fp8_e4m3"):
             self.kv_cache_quantized_dtype = torch.float8_e4m3fn
         elif kv_cache_dtype not in ("auto", "bfloat16"):
             raise NotImplementedError(
@@ -431,6 +464,17 @@ class B200AttentionBackendImpl:
         self._window = 0 if sliding_window is None else int(sliding_window)
         if logits_soft_cap is not None:
             raise NotImplementedError("logits_soft_cap is not supported")
+        if sparse_pages is not None:
+            if sparse_keep_first < 0 or sparse_keep_last < 1 \
+                    or sparse_keep_first + sparse_keep_last > sparse_pages:
+                raise ValueError("sparse_keep_first >= 0 and sparse_keep_last >= 1 must fit into "
+                                 "sparse_pages")
+            if self._window:
+                raise NotImplementedError("sparse_pages does not go with a sliding window")
+            if self.kv_cache_quantized_dtype is not None and not self.block_scaled:
+                raise NotImplementedError("sparse_pages needs a bfloat16 or a block-scaled cache")
+        self.sparse = None if sparse_pages is None else \
+            (int(sparse_pages), int(sparse_keep_first), int(sparse_keep_last))
         self.sinks = sinks
         self._sinks_f32 = None   # ((device, data_ptr, version), fp32 copy)
         # Set by a caller that has already written this step's K / V rows into the cache (the
@@ -480,9 +524,10 @@ class B200AttentionBackendImpl:
     def _forward(self, query, key, value, kv_cache, attn_metadata, output):
         kv_pair = self._split_kv_cache(kv_cache)
         written, self.kv_written_upstream = self.kv_written_upstream, False
+        pages = self._page_values(kv_cache, kv_pair)
         if attn_metadata.is_varlen:
             self._forward_varlen(query, key, value, kv_pair, attn_metadata, output,
-                                 writes_cache=not written)
+                                 writes_cache=not written, pages=pages)
             return output
 
         inputs = self._prepare_inputs(query, key, value, attn_metadata)
@@ -490,14 +535,18 @@ class B200AttentionBackendImpl:
         writes_cache = has_cache and self.kv_sharing_target_layer_name is None and not written
         if inputs.is_prefill:
             if writes_cache:
-                self._handle_paged_attention(inputs, kv_pair, attn_metadata)
-            self._compute_full_attention(inputs, kv_pair, attn_metadata, output)
+                self._handle_paged_attention(inputs, kv_pair, attn_metadata, pages)
+            self._compute_full_attention(inputs, kv_pair, attn_metadata, output, pages)
         else:
             if not has_cache:
                 raise ValueError("decode attention needs the paged KV cache")
-            # the decode step's cache write (attention.py:468-484) rides in the decode launch
+            # the decode step's cache write (attention.py:468-484) rides in the decode launch,
+            # unless it has a page's scale or bounds to keep
+            if writes_cache and pages is not None:
+                self._handle_paged_attention(inputs, kv_pair, attn_metadata, pages)
+                writes_cache = False
             self._compute_decode_attention(inputs, kv_pair, attn_metadata, output,
-                                           write_new_token=writes_cache)
+                                           write_new_token=writes_cache, pages=pages)
         return output
 
     def _split_kv_cache(self, kv_cache):
@@ -517,6 +566,36 @@ class B200AttentionBackendImpl:
                     pair[1].view(self.kv_cache_quantized_dtype))
         return pair
 
+    def _page_values(self, kv_cache, kv_pair) -> Optional["PageValues"]:
+        """What the cache keeps per page beyond its rows: entries 2 to 4 of the kv_cache list."""
+        extra = list(kv_cache[2:5]) if kv_pair is not None and isinstance(kv_cache, (list, tuple)) \
+            else []
+        extra += [None] * (3 - len(extra))
+        if kv_pair is not None:
+            if self.block_scaled and (extra[0] is None or extra[1] is None):
+                raise ValueError("a block-scaled cache is [k_cache, v_cache, k_scale, v_scale, ...]")
+            if not self.block_scaled and (extra[0] is not None or extra[1] is not None):
+                raise ValueError("the cache has scales but kv_cache_dtype is not block-scaled")
+            if self.sparse is not None and extra[2] is None:
+                raise ValueError("sparse_pages needs the key bounds as the cache's fifth entry")
+        if all(x is None for x in extra):
+            return None
+        return PageValues(*extra)
+
+    def _decode(self, query, kv_pair, page_table, cur_pos, out, max_context_len, pages, **fused):
+        """Decode attention of the rows `query` [users, nq, hd] in the form the layer was built for."""
+        scales = {} if pages is None else pages.scales
+        if self.sparse is not None:
+            count, first, last = self.sparse
+            page_table, cur_pos = ops.select_pages(
+                query, pages.k_bounds, page_table, cur_pos, kv_pair[0].shape[2], count,
+                keep_first=first, keep_last=last, max_context_len=max_context_len)
+            max_context_len = 0
+        ops.paged_decode(
+            query, kv_pair[0], kv_pair[1], page_table, cur_pos, scale=self.scale, out=out,
+            max_context_len=max_context_len, sliding_window=self._window,
+            sinks=self._sinks_for(out.device), **scales, **fused)
+
     def _prepare_inputs(self, query, key, value, attn_metadata: B200Metadata) -> PluginBatch:
         """Shapes the three activations by user (what attention.py:381-459 hands its ops)."""
         users = attn_metadata.num_users
@@ -531,9 +610,13 @@ class B200AttentionBackendImpl:
             )
         return PluginBatch(q, k, v, users, q.shape[1], k.shape[1])
 
-    def _handle_paged_attention(self, inputs, kv_pair, attn_metadata: B200Metadata) -> None:
+    def _handle_paged_attention(self, inputs, kv_pair, attn_metadata: B200Metadata,
+                                pages: Optional["PageValues"] = None) -> None:
         """KV-cache write (attention.py:461-515): one launch covers K and V."""
         k_cache, v_cache = kv_pair
+        if pages is not None:
+            self._write_pages(inputs, kv_pair, attn_metadata, pages)
+            return
         if not inputs.is_prefill:
             ops.paged_update_cache(
                 k_cache, v_cache, inputs.key[:, 0], inputs.value[:, 0],
@@ -549,6 +632,32 @@ class B200AttentionBackendImpl:
             k_cache, v_cache, inputs.key, inputs.value, attn_metadata.fill_page_table, batch_idxs
         )
 
+    def _write_pages(self, inputs, kv_pair, md: B200Metadata, pages: "PageValues") -> None:
+        """The plugin-form cache write through `ops.paged_write`.  Rows without a position (padding)
+        write nothing; in a padded prefill row only the tokens up to `cache_position` are written,
+        so that padding does not widen a page's scale or bounds."""
+        if not inputs.is_prefill:
+            ops.paged_write(kv_pair[0], kv_pair[1], inputs.key[:, 0], inputs.value[:, 0],
+                            md.page_table, md.cache_position, **pages.all)
+            return
+        assert md.batch_idx is not None, "batch_idx must be provided for prefill."
+        users, tokens = inputs.users, inputs.kv_num_tokens
+        rows = md.batch_idx
+        if md.dp_size > 1:
+            rows = rows % (users // md.dp_size)
+        table = md.fill_page_table.index_select(0, rows)
+        count = None
+        if md.cache_position is not None:
+            count = md.cache_position + 1
+            if md.chunk_start_idx is not None:
+                count = count - md.chunk_start_idx.reshape(-1)[:1].to(torch.int32)
+            count = count.clamp(0, tokens).to(torch.int32).contiguous()
+        ops.paged_write(
+            kv_pair[0], kv_pair[1], inputs.key.reshape(users * tokens, self.num_kv_heads, -1),
+            inputs.value.reshape(users * tokens, self.num_kv_heads, -1), table,
+            torch.zeros_like(rows),
+            cu_q=self._uniform_cu_q(users, tokens, table.device)[1], q_len=count, **pages.all)
+
     def _uniform_cu_q(self, users: int, tokens: int, device) -> tuple[torch.Tensor, torch.Tensor]:
         key = (users, tokens, str(device))
         cache = self.__dict__.setdefault("_cu_q_cache", {})
@@ -557,7 +666,8 @@ class B200AttentionBackendImpl:
             cache[key] = (host, host.to(device))
         return cache[key]
 
-    def _compute_full_attention(self, inputs, kv_pair, attn_metadata: B200Metadata, output) -> None:
+    def _compute_full_attention(self, inputs, kv_pair, attn_metadata: B200Metadata, output,
+                                pages: Optional["PageValues"] = None) -> None:
         """Prefill (attention.py:517-598): chunk over the paged prefix when chunk_start_idx is
         set, dense causal attention on the fresh K/V otherwise."""
         if attn_metadata.attn_mask is not None or not attn_metadata.is_causal:
@@ -572,12 +682,13 @@ class B200AttentionBackendImpl:
         cu_host, cu_dev = self._uniform_cu_q(users, tokens, q.device)
         has_cache = kv_pair is not None
         shared_kv_mode = self.kv_sharing_target_layer_name is not None and has_cache
+        scales = {} if pages is None else pages.scales
         if attn_metadata.chunk_start_idx is not None and has_cache and not shared_kv_mode:
             q_start = attn_metadata.chunk_start_idx.reshape(-1)[:1].to(torch.int32).expand(users)
             ops.prefill(
                 q, kv_pair[0], kv_pair[1], cu_host, scale=self.scale,
                 page_table=attn_metadata.page_table, q_start=q_start.contiguous(), out=out,
-                cu_q=cu_dev, sliding_window=self._window,
+                cu_q=cu_dev, sliding_window=self._window, **scales,
             )
         elif shared_kv_mode:
             # Shared-KV layers read the target layer's cache (attention.py:562-574); the kernel
@@ -585,7 +696,7 @@ class B200AttentionBackendImpl:
             ops.prefill(
                 q, kv_pair[0], kv_pair[1], cu_host, scale=self.scale,
                 page_table=attn_metadata.page_table, q_start=None, out=out, cu_q=cu_dev,
-                sliding_window=self._window,
+                sliding_window=self._window, **scales,
             )
         else:
             k = inputs.key.reshape(users * tokens, self.num_kv_heads, self.head_size)
@@ -594,7 +705,8 @@ class B200AttentionBackendImpl:
                         sliding_window=self._window)
 
     def _compute_decode_attention(self, inputs, kv_pair, attn_metadata: B200Metadata, output,
-                                  write_new_token: bool = False) -> None:
+                                  write_new_token: bool = False,
+                                  pages: Optional["PageValues"] = None) -> None:
         """attention.py:634-668; with `write_new_token` also the K / V write of attention.py:468-484
         (same positions, same page table) inside the same launch."""
         if attn_metadata.attn_mask is not None or not attn_metadata.is_causal:
@@ -603,18 +715,16 @@ class B200AttentionBackendImpl:
         fused = {}
         if write_new_token:
             fused = dict(new_key=inputs.key[:, 0], new_value=inputs.value[:, 0])
-        ops.paged_decode(
-            inputs.query.reshape(users, self.num_heads, self.head_size),
-            kv_pair[0], kv_pair[1], attn_metadata.page_table, attn_metadata.cache_position,
-            scale=self.scale,
-            out=output.reshape(users, self.num_heads, self.head_size),
-            max_context_len=attn_metadata.max_seq_len,
-            sliding_window=self._window, sinks=self._sinks_for(output.device), **fused,
-        )
+        self._decode(
+            inputs.query.reshape(users, self.num_heads, self.head_size), kv_pair,
+            attn_metadata.page_table, attn_metadata.cache_position,
+            output.reshape(users, self.num_heads, self.head_size), attn_metadata.max_seq_len,
+            pages, **fused)
 
     # ------------------------------------------------------------------ vLLM varlen form
     def _forward_varlen(self, query, key, value, kv_pair, md: B200Metadata, output,
-                        writes_cache: bool = True) -> None:
+                        writes_cache: bool = True,
+                        pages: Optional["PageValues"] = None) -> None:
         if kv_pair is None:
             # Memory-profiling run before the cache exists: nothing to attend to.
             output.zero_()
@@ -629,7 +739,18 @@ class B200AttentionBackendImpl:
         # block_table[pos // bs] * bs + pos % bs, which is what that launch computes; padding
         # rows carry position -1 and are skipped like slot -1); mixed batches scatter by slot.
         fused = {}
-        if writes_cache and nd == n_tok and md.prefill_cu_q_cpu is None:
+        pure_decode = nd == n_tok and md.prefill_cu_q_cpu is None
+        if writes_cache and pages is not None:
+            if pure_decode:
+                start, cu_q = md.decode_cur_pos, None
+            else:
+                cu_q, start = md.query_start_loc, md.prefill_q_start
+                if nd > 0:
+                    start = torch.cat([md.decode_cur_pos, start])
+            ops.paged_write(
+                kv_pair[0], kv_pair[1], key[:n_tok].reshape(n_tok, nkv, hd),
+                value[:n_tok].reshape(n_tok, nkv, hd), md.block_table, start, cu_q=cu_q, **pages.all)
+        elif writes_cache and pure_decode:
             fused = dict(new_key=key[:n_tok].reshape(n_tok, nkv, hd),
                          new_value=value[:n_tok].reshape(n_tok, nkv, hd),
                          wrap_negative_positions=False)
@@ -639,17 +760,15 @@ class B200AttentionBackendImpl:
                 value[:n_tok].reshape(n_tok, nkv, hd), md.slot_mapping[:n_tok],
             )
         if nd > 0:
-            ops.paged_decode(
-                q[:nd], kv_pair[0], kv_pair[1], md.block_table[:nd], md.decode_cur_pos,
-                scale=self.scale, out=out[:nd], max_context_len=md.max_seq_len,
-                sliding_window=self._window, sinks=self._sinks_for(output.device), **fused,
-            )
+            self._decode(q[:nd], kv_pair, md.block_table[:nd], md.decode_cur_pos, out[:nd],
+                         md.max_seq_len, pages, **fused)
         if md.prefill_cu_q_cpu is not None:
             assert self.sinks is None, "Attention sink is unsupported in SDPA prefill"
             ops.prefill(
                 q[nd:], kv_pair[0], kv_pair[1], md.prefill_cu_q_cpu, scale=self.scale,
                 page_table=md.block_table[nd:], q_start=md.prefill_q_start, out=out[nd:],
                 cu_q=md.prefill_cu_q, sliding_window=self._window,
+                **({} if pages is None else pages.scales),
             )
 
 
@@ -683,7 +802,9 @@ class B200Attention(torch.nn.Module):
 
     def __init__(self, num_heads: int, head_size: int, scale: float,
                  num_kv_heads: Optional[int] = None, *, rotary_dim: Optional[int] = None,
-                 rope_theta: float = 10000.0, **impl_kwargs) -> None:
+                 rope_theta: float = 10000.0, q_norm_weight: Optional[torch.Tensor] = None,
+                 k_norm_weight: Optional[torch.Tensor] = None, norm_eps: float = 1e-6,
+                 is_neox_style: bool = True, **impl_kwargs) -> None:
         super().__init__()
         # NeoX-style rotary embedding applied by the layer itself when `forward` is given
         # positions (the plugin's rotary layer, layers/rotary_embedding.py:51-66): one launch
@@ -694,6 +815,18 @@ class B200Attention(torch.nn.Module):
         if rotary_dim is not None:
             self.inv_freq = 1.0 / (rope_theta ** (
                 torch.arange(0, rotary_dim, 2, dtype=torch.float32) / rotary_dim))
+        # RMS norms of every query and key head in front of the rotation (`q_norm_weight` /
+        # `k_norm_weight` [head_size]): the same launch does them
+        # (ops.qk_norm_rope_kv_scatter_slots), in fp32 and for either pairing.
+        if (q_norm_weight is None) != (k_norm_weight is None):
+            raise ValueError("q_norm_weight and k_norm_weight go together")
+        if q_norm_weight is not None and rotary_dim is None:
+            raise ValueError("the head norms come with the rotation: rotary_dim is needed")
+        if not is_neox_style and q_norm_weight is None:
+            raise NotImplementedError("interleaved pairs are supported with the head norms only")
+        self.norm_weights = None if q_norm_weight is None else \
+            [w.detach().contiguous() for w in (q_norm_weight, k_norm_weight)]
+        self.norm_eps, self.is_neox_style = norm_eps, is_neox_style
         self.num_heads = num_heads
         self.head_size = self.head_size_v = head_size
         self.num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
@@ -702,7 +835,9 @@ class B200Attention(torch.nn.Module):
             impl_kwargs.pop("alibi_slopes", None), impl_kwargs.pop("sliding_window", None),
             impl_kwargs.pop("kv_cache_dtype", "auto"), impl_kwargs.pop("logits_soft_cap", None),
             impl_kwargs.pop("attn_type", DECODER),
-            impl_kwargs.pop("kv_sharing_target_layer_name", None), impl_kwargs.pop("sinks", None))
+            impl_kwargs.pop("kv_sharing_target_layer_name", None), impl_kwargs.pop("sinks", None),
+            impl_kwargs.pop("sparse_pages", None), impl_kwargs.pop("sparse_keep_first", 1),
+            impl_kwargs.pop("sparse_keep_last", 1))
         if impl_kwargs:
             raise TypeError(f"unexpected arguments: {sorted(impl_kwargs)}")
         self.kv_cache = None
@@ -718,9 +853,21 @@ class B200Attention(torch.nn.Module):
             self.inv_freq = self.inv_freq.to(q2.device)
         kv_pair = self.impl._split_kv_cache(self.kv_cache)
         slots = getattr(md, "slot_mapping", None)
+        # a cache that keeps scales or bounds per page is written by the Impl (ops.paged_write)
         fused_write = (kv_pair is not None and slots is not None
                        and self.impl.kv_sharing_target_layer_name is None
-                       and kv_pair[0].dtype == torch.bfloat16)
+                       and kv_pair[0].dtype == torch.bfloat16
+                       and self.impl._page_values(self.kv_cache, kv_pair) is None)
+        if self.norm_weights is not None:
+            if self.norm_weights[0].device != q2.device:
+                self.norm_weights = [w.to(q2.device) for w in self.norm_weights]
+            ops.qk_norm_rope_kv_scatter_slots(
+                q2, k2, v2 if fused_write else None, positions.reshape(-1).to(torch.int64),
+                self.inv_freq, self.rotary_dim, self.head_size, *self.norm_weights, self.norm_eps,
+                kv_pair[0] if fused_write else None, kv_pair[1] if fused_write else None,
+                slots[: q2.shape[0]] if fused_write else None, is_neox_style=self.is_neox_style)
+            self.impl.kv_written_upstream = fused_write
+            return
         ops.rope_kv_scatter_slots(
             q2, k2, v2 if fused_write else None, positions.reshape(-1).to(torch.int64),
             self.inv_freq, self.rotary_dim, self.head_size,

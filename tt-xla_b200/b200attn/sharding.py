@@ -100,6 +100,8 @@ def allocate_kv_caches(
     device=None,
     tp_size: int = 1,
     shared_kv_layers=None,
+    block_scales: bool = False,
+    page_bounds: bool = False,
 ) -> dict:
     """Per-layer paged caches the way the plugin's runner creates them
     (`initialize_kv_cache`, model_runner.py:4560-4630): for every attention layer a zeroed
@@ -112,7 +114,11 @@ def allocate_kv_caches(
     `layer_names`: names, or a layer count (names become "layers.<i>.attn").
     `shared_kv_layers`: {layer: target layer} for cross-layer KV sharing; such a layer gets the
     target's pair itself, not a copy (`maybe_setup_cross_layer_kv_sharing`).
-    Returns {layer name: [k_cache, v_cache]} in layer order."""
+    `block_scales` (implied by int8): 8-bit caches with a scale per page and KV head; the list
+    goes on with k_scale and v_scale (fp32 [num_blocks, local KV heads], zeroed).  `page_bounds`: the
+    list's fifth entry is the key bounds `ops.select_pages` reads (bf16 [num_blocks, local KV heads,
+    2, head_size]); entries 2 and 3 are then None for a bf16 cache.
+    Returns {layer name: [k_cache, v_cache, ...]} in layer order."""
     from .backend import B200AttentionBackend
 
     if isinstance(layer_names, int):
@@ -126,8 +132,13 @@ def allocate_kv_caches(
         raise ValueError(f"head_size {head_size} is not supported (64 or 128)")
     if not B200AttentionBackend.supports_block_size(block_size):
         raise ValueError(f"block_size {block_size} is not supported (32 or 64)")
-    if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
-        raise ValueError("KV caches are bfloat16 or float8_e4m3fn")
+    if dtype not in (torch.bfloat16, torch.float8_e4m3fn, torch.int8):
+        raise ValueError("KV caches are bfloat16, float8_e4m3fn or (block-scaled) int8")
+    block_scales = block_scales or dtype == torch.int8
+    if block_scales and dtype == torch.bfloat16:
+        raise ValueError("block_scales goes with 8-bit caches")
+    if page_bounds and dtype == torch.float8_e4m3fn and not block_scales:
+        raise ValueError("page_bounds goes with bfloat16 or block-scaled caches")
     shared_kv_layers = dict(shared_kv_layers or {})
     shape = B200AttentionBackend.get_kv_cache_shape(
         num_blocks, block_size, num_kv_heads // max(tp_size, 1), head_size)
@@ -137,6 +148,13 @@ def allocate_kv_caches(
             continue
         caches[name] = [torch.zeros(shape, dtype=dtype, device=device),
                         torch.zeros(shape, dtype=dtype, device=device)]
+        if block_scales:
+            caches[name] += [torch.zeros(shape[:2], dtype=torch.float32, device=device),
+                             torch.zeros(shape[:2], dtype=torch.float32, device=device)]
+        if page_bounds:
+            caches[name] += [None] * (4 - len(caches[name]))
+            caches[name].append(torch.zeros(shape[:2] + (2, head_size), dtype=torch.bfloat16,
+                                            device=device))
     for name, target in shared_kv_layers.items():
         if target not in caches:
             raise ValueError(f"layer {name} shares the KV cache of unknown layer {target}")
