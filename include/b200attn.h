@@ -390,8 +390,11 @@ int b200attn_paged_write(void* k_cache, void* v_cache, float* k_scale, float* v_
  *     cur_pos % block_size (what b200attn_select_pages writes).  No sliding window then.
  *   num_splits: for scaled caches 0 cuts the whole batch's context into equal shares, one per CTA
  *     (num_splits > 0 cuts every (user, KV head) into that many); the workspace then holds
- *     b200attn_decode_scaled_workspace_bytes of the current device.  For other caches as in
- *     b200attn_paged_decode. */
+ *     b200attn_decode_scaled_workspace_bytes of the current device.  Batches with more (user, KV
+ *     head) pairs than arrival counters are always cut between pairs.  For other caches as in
+ *     b200attn_paged_decode.
+ *   A position behind the end of the page table is reported (diagnostics word 2) for scaled caches;
+ *   the keys up to that end are attended. */
 int b200attn_paged_decode_blocks(void* out, int64_t out_row_stride, const void* q,
                                  int64_t q_row_stride, const void* k_cache, const void* v_cache,
                                  const float* k_scale, const float* v_scale, int cache_dtype,
@@ -421,7 +424,7 @@ size_t b200attn_decode_scaled_workspace_bytes(int num_users, int num_q_heads, in
  * max_context_len (0: unknown) only shapes the launch.  Workspace:
  * b200attn_select_pages_workspace_bytes bytes whose first B200ATTN_DECODE_TICKET_BYTES follow the
  * contract of b200attn_paged_decode's (zero at first use, left zero); the two calls may share a
- * workspace in stream order.  At most B200ATTN_DECODE_TICKET_BYTES / 4 (user, KV head) pairs.
+ * workspace in stream order.
  * ------------------------------------------------------------------------------------------ */
 size_t b200attn_select_pages_workspace_bytes(int num_users, int num_kv_heads,
                                              int page_table_width);

@@ -324,8 +324,57 @@ def test_decode_bad_page_is_reported():
     assert ops.read_error_word() == 2
 
 
-def test_many_users_use_the_second_merge_launch(clean_error_word):
-    """More (user, KV head) pairs than arrival counters: the splits are merged by a second launch."""
+@pytest.mark.parametrize("splits", [0, 2])
+def test_decode_positions_behind_the_table_are_reported(splits):
+    """Up to the largest int: the keys of the table's pages are attended, nothing else is read."""
+    from b200attn import ops
+
+    ops.read_error_word()
+    c = _decode_case(3, 8, 2, 64, 32, [64, 96, 64], torch.int8, seed=8)
+    full = dict(c, pos=torch.tensor([95, 95, 95], dtype=torch.int32))
+    want = _decode(full, num_splits=splits)
+    assert ops.read_error_word() == 0
+    got = _decode(dict(c, pos=torch.tensor([96, 95, 2 ** 31 - 1], dtype=torch.int32)),
+                  num_splits=splits)
+    assert ops.read_error_word() == 2
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 5])
+def test_decode_shares_of_uneven_pairs(clean_error_word, splits):
+    """One long context among short and empty ones: shares begin and end inside pairs."""
+    ctx = [1, 0, 9000, 3, 0, 130, 257, 1]
+    c = _decode_case(8, 6, 3, 64, 64, ctx, torch.float8_e4m3fn, seed=4)
+    got = _decode(c, num_splits=splits)
+    _attention_close(got, c)
+    assert not got[1].any() and not got[4].any()
+
+
+def test_decode_one_pair_uses_many_ctas(clean_error_word):
+    c = _decode_case(1, 4, 1, 128, 64, [20000], torch.int8, seed=4)
+    _attention_close(_decode(c), c)
+    _attention_close(_decode(c, num_splits=200), c)
+
+
+def test_decode_writes_into_out_rows_and_nothing_else(clean_error_word):
+    """A strided `out`, a strided query and fewer users than table rows."""
+    from b200attn import ops
+
+    c = _decode_case(4, 8, 2, 64, 32, [64, 100, 7, 33], torch.int8, seed=8)
+    d = {n: t.cuda() for n, t in c.items()}
+    buf = torch.full((5, 3, 8, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    wide = torch.zeros(4, 12, 64, dtype=torch.bfloat16, device="cuda")
+    wide[:, 2:10] = d["query"]
+    out = buf[:3, 1]
+    r = ops.paged_decode(wide[:3, 2:10], d["k_cache"], d["v_cache"], d["table"], d["pos"][:3],
+                         out=out, k_scale=d["k_scale"], v_scale=d["v_scale"])
+    assert r is out
+    assert torch.equal(out.cpu(), _decode(c)[:3])
+    assert (buf[:, 0] == 3).all() and (buf[:, 2] == 3).all() and (buf[3:] == 3).all()
+
+
+def test_many_users_are_cut_between_pairs(clean_error_word):
+    """More (user, KV head) pairs than arrival counters: no pair is shared by two CTAs."""
     users, nkv = 2100, 8
     c = _decode_case(users, 8, nkv, 64, 32, [1 + i % 70 for i in range(users)], torch.int8, seed=2)
     one, two = _decode(c, num_splits=1), _decode(c, num_splits=2)

@@ -113,6 +113,36 @@ def test_cache_write_is_the_scatter_of_the_results(clean_error_word, kind, hd, b
     assert torch.equal(vc.view(torch.uint8), vc2.view(torch.uint8))
 
 
+def test_outputs_side_by_side_in_one_buffer(clean_error_word):
+    from b200attn import ops
+
+    c = _case(9, 4, 2, 64, 64, seed=8)
+    q, k, v = c["dev"]
+    args = (c["positions"].cuda(), c["inv_freq"].cuda(), 64, 64, c["wq"].cuda(), c["wk"].cuda())
+    both = torch.zeros(9, 6 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    ops.qk_norm_rope_kv_scatter_slots(q, k, None, *args, out_query=both[:, : 4 * 64],
+                                      out_key=both[:, 4 * 64: 6 * 64])
+    assert not both[:, 6 * 64:].any()
+    iq, ik = ops.qk_norm_rope_kv_scatter_slots(q, k, None, *args)
+    assert torch.equal(both[:, : 4 * 64], iq) and torch.equal(both[:, 4 * 64: 6 * 64], ik)
+
+
+def test_a_slot_twice_takes_one_of_the_rows(clean_error_word):
+    from b200attn import ops
+
+    c = _case(2, 2, 1, 64, 64, seed=1)
+    q, k, v = c["dev"]
+    kc = torch.zeros(2, 1, 32, 64, dtype=torch.bfloat16, device="cuda")
+    vc = kc.clone()
+    ops.qk_norm_rope_kv_scatter_slots(
+        q, k, v, c["positions"].cuda(), c["inv_freq"].cuda(), 64, 64, c["wq"].cuda(),
+        c["wk"].cuda(), 1e-6, kc, vc, torch.tensor([7, 7]).cuda())
+    got = torch.stack([kc[0, 0, 7], vc[0, 0, 7]])
+    assert ((got[0] == k[0]) | (got[0] == k[1])).all() and ((got[1] == v[0]) | (got[1] == v[1])).all()
+    kc[0, 0, 7] = 0
+    assert not kc.any()
+
+
 def test_slots_outside_the_cache_are_skipped_and_reported():
     from b200attn import ops
 
@@ -152,6 +182,13 @@ def test_refusals():
     with pytest.raises(ValueError, match="overlap"):                   # shifted by one head
         big = torch.zeros(4, 5 * 64, dtype=torch.bfloat16, device="cuda")
         call(q=big[:, : 4 * 64], out_query=big[:, 64:])
+    with pytest.raises(ValueError, match="overlap"):                   # both in place, one memory
+        call(q=k, k=k)
+    row = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device="cuda").expand(4, -1)
+    with pytest.raises(B200AttnError):                                 # rows on top of each other
+        call(q=row, out_query=torch.empty_like(q))
+    with pytest.raises(B200AttnError):
+        call(q=row, out_query=row)
     with pytest.raises(B200AttnError):                                 # not a multiple of 16
         call(rotary=24, inv=inv[:12].clone())
     with pytest.raises(RuntimeError, match="no CPU path"):

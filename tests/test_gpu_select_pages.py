@@ -60,6 +60,26 @@ def test_the_length_hint_does_not_change_the_choice(clean_error_word, hint):
     _check(c, 32, 20, 1, 1, max_context_len=hint)
 
 
+@pytest.mark.parametrize("pages", [4097, 9000])
+def test_more_pages_than_stay_in_shared_memory(clean_error_word, pages):
+    c = _case(2, 4, 1, 64, 32, [pages * 32 - 5, 4096 * 32], seed=pages)
+    _check(c, 32, 200, 2, 3)
+    c["k_bounds"][:] = c["k_bounds"][0]
+    _check(c, 32, 300, 1, 2)
+
+
+def test_many_users(clean_error_word):
+    """More (user, KV head) pairs than arrival counters."""
+    users = 2100
+    c = _case(users, 8, 8, 64, 32, [1 + (i * 37) % 400 for i in range(users)], seed=2)
+    table, pos = _select(c, 32, 4, 1, 1)
+    sub = [0, 10, 777, 2099]
+    small = dict(c, query=c["query"][sub], table=c["table"][sub], pos=c["pos"][sub])
+    want_t, want_p = blocks.select_pages(small["query"], c["k_bounds"], small["table"], small["pos"],
+                                         32, 4, 1, 1)
+    assert torch.equal(table.cpu()[sub], want_t) and torch.equal(pos.cpu()[sub], want_p)
+
+
 def test_ties_go_to_the_lower_page(clean_error_word):
     """Equal bounds everywhere, two values of bounds, and a zero query."""
     c = _case(3, 8, 2, 64, 32, [700 * 32, 50 * 32, 400 * 32], seed=4)

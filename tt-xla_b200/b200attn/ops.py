@@ -302,7 +302,7 @@ def _rows_meet(a: tuple, b: tuple, tokens: int) -> bool:
     (a0, a_step, a_width), (b0, b_step, b_width) = a, b
     if b0 >= a0 + (tokens - 1) * a_step + a_width or a0 >= b0 + (tokens - 1) * b_step + b_width:
         return False
-    if a_step == b_step:
+    if a_step == b_step and a_step > 0:
         gap = (b0 - a0) % a_step
         return gap < a_width or a_step - gap < b_width
     return True
@@ -415,6 +415,8 @@ def qk_norm_rope_kv_scatter_slots(
         _check_outputs(tokens, (oq_ptr, 2 * oq_stride, 2 * q_width),
                        (ok_ptr, 2 * ok_stride, 2 * k_width), (q_ptr, 2 * q_stride, 2 * q_width),
                        (k_ptr, 2 * k_stride, 2 * k_width), (v_ptr, 2 * v_stride, 2 * k_width))
+    elif _rows_meet((q_ptr, 2 * q_stride, 2 * q_width), (k_ptr, 2 * k_stride, 2 * k_width), tokens):
+        raise ValueError("query and key overlap: they cannot both be replaced in place")
     status = _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
         oq_ptr, oq_stride, ok_ptr, ok_stride, q_ptr, q_stride, k_ptr, k_stride,
         v_ptr, v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
@@ -619,7 +621,7 @@ def select_pages(
         raise ValueError(f"num_q_heads {nq} is not a multiple of num_kv_heads {nkv}")
     q, qstride = _token_major(query, nq, hd, "query")
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < users \
-            or page_table.stride(1) != 1:
+            or page_table.stride(1) != 1 or page_table.shape[1] == 0:
         raise ValueError("page_table must be int32 with a dense row per user")
     if cur_pos.dtype != torch.int32 or not cur_pos.is_contiguous() or cur_pos.numel() != users:
         raise ValueError("cur_pos must be int32 with a dense entry per user")

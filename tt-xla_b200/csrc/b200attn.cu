@@ -834,6 +834,8 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
   size_t need;
   if (scaled) {
+    if (static_cast<int64_t>(page_table_width) * block_size > 0x7fffffffLL - kDsTile)
+      return B200ATTN_ERR_TOO_LARGE;
     // Lists of chosen pages are equally long, so one CTA per pair is as balanced as shares and has
     // nothing to merge, where the pairs about fill the machine (256 pairs of 64 pages: 52 us, 58
     // in shares).
@@ -1214,9 +1216,7 @@ int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
   DeviceInfo* dev;
   if (int rc = get_device(&dev)) return rc;
   if (num_users == 0) return B200ATTN_OK;
-  if (num_users > 65535 || num_kv_heads > 65535 ||
-      static_cast<size_t>(num_users) * num_kv_heads * sizeof(unsigned int) > kDecTicketBytes)
-    return B200ATTN_ERR_TOO_LARGE;
+  if (num_users > 65535 || num_kv_heads > 65535) return B200ATTN_ERR_TOO_LARGE;
   if (!workspace || !aligned16(workspace) ||
       workspace_bytes < b200attn_select_pages_workspace_bytes(num_users, num_kv_heads, page_table_width))
     return B200ATTN_ERR_WORKSPACE;
@@ -1252,7 +1252,7 @@ int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
   // once (one CTA per (user, KV head) needs no second trip of the scores through memory)
   const int64_t ctas = 2 * static_cast<int64_t>(dev->sm_count);
   const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
-  const int64_t per_pair = pairs < ctas ? ctas / pairs : 1;
+  const int64_t per_pair = pairs < ctas ? ctas / pairs : 1;   // 1 for more pairs than counters
   p.slice = static_cast<int>(((pages + per_pair - 1) / per_pair + 127) / 128 * 128);
   const int64_t slices = (static_cast<int64_t>(pages) + p.slice - 1) / p.slice;
   const dim3 grid(static_cast<unsigned>(slices), static_cast<unsigned>(num_kv_heads),

@@ -106,10 +106,18 @@ struct DsSegment {
   int64_t pair_pos;          // where the pair's tiles start among all pairs' tiles
 };
 
-// First attended key and tiles of a pair.
+// First attended key and tiles of a pair.  A position behind the end of the page table is reported
+// and the keys up to that end are attended.
+template <int BS>
 __device__ __forceinline__ int ds_pair_tiles(const DecodeParams& p, int user, int kvh, int* ctx_out,
                                              int* lo_out) {
-  const int ctx = decode_cur_pos(p, user, kvh) + 1;
+  int pos = decode_cur_pos(p, user, kvh);
+  const int64_t most = static_cast<int64_t>(p.page_table_width) * BS - 1;
+  if (pos > most) {
+    atomicExch(p.err_word, kDevBadIndex);
+    pos = static_cast<int>(most);
+  }
+  const int ctx = pos + 1;             // the host keeps width * block_size below 2^31 - kDsTile
   const int lo = (p.window > 0 && ctx > p.window) ? ctx - p.window : 0;
   *ctx_out = ctx;
   *lo_out = lo;
@@ -147,12 +155,13 @@ struct DsShare {
   }
 
   // Next segment; false at the end of the share.  Empty pairs are passed over.
+  template <int BS>
   __device__ __forceinline__ bool next(const DecodeScaledParams& sp, DsSegment& s) {
     const DecodeParams& p = sp.d;
     while (pos < end && pair < sp.num_pairs) {
       s.user = pair / p.num_kv_heads;
       s.kvh = pair - s.user * p.num_kv_heads;
-      s.n_tiles = ds_pair_tiles(p, s.user, s.kvh, &s.ctx, &s.lo);
+      s.n_tiles = ds_pair_tiles<BS>(p, s.user, s.kvh, &s.ctx, &s.lo);
       const int first = offset, left = s.n_tiles - first;
       if (sp.whole_pairs && first > 0) {       // the pair belongs to the share it starts in
         pos += left;
@@ -327,7 +336,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     const int split = blockIdx.x - share.pair * p.num_splits;
     int ctx, lo;
     const int user = share.pair / p.num_kv_heads;
-    const int n = ds_pair_tiles(p, user, share.pair - user * p.num_kv_heads, &ctx, &lo);
+    const int n = ds_pair_tiles<BS>(p, user, share.pair - user * p.num_kv_heads, &ctx, &lo);
     share.divide(n, min(p.num_splits, n));
     share.pos = split < share.shares ? share.start_of(split) : 0;
     share.end = split < share.shares ? share.start_of(split + 1) : 0;
@@ -341,7 +350,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     int64_t mine = 0;
     int ctx, lo, empty = 0;
     for (int q = first; q < last; ++q) {
-      const int n = ds_pair_tiles(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
+      const int n = ds_pair_tiles<BS>(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
       mine += n;
       empty |= n == 0;
     }
@@ -366,8 +375,8 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     share.end = has ? share.start_of(c + 1) : 0;
     if (has && share.pos >= before && share.pos < before + mine) {
       int q = first;
-      for (;; ++q) {
-        const int n = ds_pair_tiles(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
+      for (; q < last; ++q) {
+        const int n = ds_pair_tiles<BS>(p, q / p.num_kv_heads, q % p.num_kv_heads, &ctx, &lo);
         if (share.pos < before + n) break;
         before += n;
       }
@@ -387,7 +396,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     for (; q < sp.num_pairs; q += step) {
       int ctx, lo;
       const int user = q / p.num_kv_heads, kvh = q - user * p.num_kv_heads;
-      if (ds_pair_tiles(p, user, kvh, &ctx, &lo) > 0) continue;
+      if (ds_pair_tiles<BS>(p, user, kvh, &ctx, &lo) > 0) continue;
       for (int i = threadIdx.x; i < G * HD; i += kDecThreads)
         p.out[static_cast<int64_t>(user) * p.out_row_stride + kvh * G * HD + i] = __float2bfloat16(0.f);
     }
@@ -410,7 +419,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
       float ks, vs;     // K scale, log2 of the V scale
     };
     uint32_t it = 0;    // tiles since the start of the share
-    while (share.next(sp, seg)) {
+    while (share.next<BS>(sp, seg)) {
       const int kvh = seg.kvh;
       const int n_pages = (seg.ctx + BS - 1) / BS;
       const int32_t* pt = decode_page_row(p, seg.user, kvh);
@@ -510,7 +519,7 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
   float4* ms = reinterpret_cast<float4*>(mo + 2 * 8 * NG * L::kRow);   // [2][8 NG] m, r, l
   uint32_t it = 0;                  // tiles since the start of the share
   int segments = 0;
-  while (share.next(sp, seg)) {
+  while (share.next<BS>(sp, seg)) {
   // Q fragments (B operand, columns = query heads 8 ng + g; heads >= G are zero).  Within the
   // 16 elements of k-step ks the thread holds 4tq .. 4tq+3; slots {2tq, 2tq+1} take elements 0
   // and 2 of these, slots {2tq+8, 2tq+9} elements 1 and 3: the order codes_to_f16 gives.
