@@ -841,6 +841,10 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
     // in shares).
     const int64_t shares = decode_scaled_ctas(dev->sm_count, pairs, 0);
     if (per_head && num_splits == 0 && pairs <= shares && pairs * 4 >= shares * 3) num_splits = 1;
+    // The pairs of a single user are equally long: cutting each into the same number of pieces is as
+    // balanced as shares, and no piece waits behind another's merge (32768 tokens, 8 pairs: 26.5 us
+    // with 32 pieces, 31.5 in 256 shares).
+    if (num_users == 1 && !per_head && num_splits == 0) num_splits = static_cast<int>(shares / pairs);
     // too many pairs for the arrival counters: shares of whole pairs
     if (pairs * static_cast<int64_t>(sizeof(unsigned int)) > kDecTicketBytes) num_splits = 0;
     if (decode_scaled_ctas(dev->sm_count, pairs, num_splits) > 0x7fffffffLL)
