@@ -23,6 +23,9 @@
 // Memory-bound: 2 bytes read and 1 written per element.  Grid (page of the batch, KV head, K / V),
 // 128 threads that hold a page's rows of one head in registers (16 elements each per pass), so the
 // rows are read once for both the maximum and the codes.
+// Measured: 8192 tokens of 8 heads of 128 (50 MB) 15.6 us in int8, 16.7 us in e4m3 (3.2 / 3.0 TB/s:
+// a round or two of CTAs, each a chain of offsets, rows, maximum and codes); one token for each of
+// 64 sequences 5.1 us, launch and the same chain.
 #pragma once
 #include "kv_scatter.cuh"
 
@@ -379,7 +382,8 @@ __global__ void __launch_bounds__(kPwThreads, 8) paged_write_kernel(const PagedW
 // `factors` gets (f of K, log2 f of V) for each page and head of the pool.  A zero scale gives zeros
 // and f = 1.  A page whose K or V scale is NaN (or no scale at all: negative, infinite)
 // gets NaN keys and zero values: rows that attend it come out as NaN, rows for which it is masked
-// do not.  Memory-bound: 1 byte read and 2 written per element.
+// do not.  Memory-bound: 1 byte read and 2 written per element (2 x 4608 tokens of 8 heads of 128,
+// 55 MB: 15 us).
 struct DequantScaledParams {
   const uint8_t* src[2];
   __nv_bfloat16* dst[2];

@@ -22,6 +22,9 @@
 // a slice of the pages; the one that arrives last (a ticket in the workspace) makes the choice.
 // Choosing is a chain of block-wide counts, so it is a bisection that starts at the highest bit in
 // which the scores differ and ends as soon as the count is right.
+// Measured: 64 of up to 512 pages for 32 users x 8 KV heads of 128 (67 MB of bounds) 29 us, of which
+// scoring takes 20 (3.4 TB/s: 512-byte pieces, one round of CTAs) and choosing 9; 62 with a radix
+// choice in global memory, 33 before the next group's bounds were loaded ahead.
 #pragma once
 #include "kv_scatter.cuh"
 
