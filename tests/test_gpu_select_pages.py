@@ -164,6 +164,29 @@ def test_decode_over_the_chosen_pages(clean_error_word, nq, nkv, hd, bs, splits,
     assert not got[4].any()
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_lists_of_any_length_per_head(clean_error_word, kind, splits):
+    """Lists the caller made: another length for every head, empty ones, a page twice; bf16 and
+    unscaled e4m3 caches."""
+    from b200attn import ops
+
+    g = torch.Generator().manual_seed(11)
+    users, nq, nkv, hd, bs, nb = 3, 12, 3, 128, 32, 20
+    k = torch.randn(nb, nkv, bs, hd, generator=g).to(kind)
+    v = torch.randn(nb, nkv, bs, hd, generator=g).to(kind)
+    q = torch.randn(users, nq, hd, generator=g).bfloat16()
+    table = torch.randint(0, nb, (users, nkv, 9), generator=g).int()
+    pos = torch.tensor([[0, 31, 287], [-1, 32, 100], [5, -1, 250]], dtype=torch.int32)
+    got = ops.paged_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), pos.cuda(),
+                           num_splits=splits).cpu()
+    want = blocks.decode(q, k, v, table, pos)
+    size = blocks.decode(q, k, v.float().abs(), table, pos)
+    err = (got.double() - want).abs()
+    assert (err <= 2.0 ** -8 * want.abs() + 2.0 ** -7 * size).all(), err.max()
+    assert not got[1, :4].any() and not got[2, 4:8].any()
+
+
 def test_a_list_of_every_page_is_the_dense_decode(clean_error_word):
     from b200attn import ops
 

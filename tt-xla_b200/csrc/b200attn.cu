@@ -834,7 +834,8 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   const int64_t pairs = static_cast<int64_t>(num_users) * num_kv_heads;
   size_t need;
   if (scaled) {
-    if (static_cast<int64_t>(page_table_width) * block_size > 0x7fffffffLL - kDsTile)
+    if (static_cast<int64_t>(page_table_width) * block_size > 0x7fffffffLL - kDsTile ||
+        pairs > 0x7fffffffLL)
       return B200ATTN_ERR_TOO_LARGE;
     // Lists of chosen pages are equally long, so one CTA per pair is as balanced as shares and has
     // nothing to merge, where the pairs about fill the machine (256 pairs of 64 pages: 52 us, 58
@@ -900,7 +901,6 @@ static int decode_any(void* out, int64_t out_row_stride, const void* q, int64_t 
   p.err_word = dev->err_word;
   p.per_head = per_head;
   p.page_table_head_stride = page_table_head_stride;
-  p.keep_nan = scaled ? 1 : 0;
   if (scaled) {
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const size_t rows_p = static_cast<size_t>(decode_scaled_ctas(dev->sm_count, pairs, num_splits)) *

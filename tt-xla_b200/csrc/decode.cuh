@@ -54,7 +54,6 @@ struct DecodeParams {
   int per_head;        // 1: page_table is [users, nkv, width] and cur_pos [users, nkv]: a page list
                        // (and the position within the list) of its own for every KV head
   int64_t page_table_head_stride;
-  int keep_nan;        // 1: a row whose sum is NaN comes out as NaN, 0: as zeros
 };
 
 __device__ __forceinline__ int decode_cur_pos(const DecodeParams& p, int user, int kvh) {
@@ -199,7 +198,7 @@ __device__ __forceinline__ void decode_split_finish(const DecodeParams& p, int u
     const int head = kvh * G + r;
     if (p.sinks) acc *= apply_sink(m, l, p.sinks[head] * 1.4426950408889634f);
     p.out[static_cast<int64_t>(user) * p.out_row_stride + head * HD + d] =
-        __float2bfloat16(l > 0.f || (p.keep_nan && l != l) ? acc / l : 0.f);
+        __float2bfloat16(l > 0.f ? acc / l : 0.f);
   }
   if (tid == 0) *ticket = 0u;              // leave the counter as the next launch expects it
 }
@@ -559,7 +558,7 @@ __global__ void __launch_bounds__(HD) decode_combine_kernel(const DecodeParams p
   }
   if (p.sinks) acc *= apply_sink(m, l, p.sinks[head] * 1.4426950408889634f);
   p.out[static_cast<int64_t>(user) * p.out_row_stride + head * HD + d] =
-      __float2bfloat16(l > 0.f || (p.keep_nan && l != l) ? acc / l : 0.f);
+      __float2bfloat16(l > 0.f ? acc / l : 0.f);
 }
 
 }  // namespace b200attn
