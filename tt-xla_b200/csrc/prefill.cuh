@@ -288,7 +288,11 @@ __device__ __forceinline__ void setmaxnreg_dec() {
 // SCALED: K and V come from dequant_scaled_kernel's pool, whose pages hold code * 2^e, exact in bf16;
 // what is left of a page's scale is a factor in [1, 2) that is applied here in fp32.  The K factor
 // multiplies the scores (in the FMA that scales them anyway), the V factor enters the exponent of
-// the weights, and the row sum takes it out again per 32-key chunk (a chunk lies in one page).
+// the weights, and the row sum takes it out again per 32-key chunk (a chunk lies in one page).  With
+// the factor in it even the largest weight of a row is rounded (without it that is a 1), so the sum
+// is taken of the rounded weights: a row that few keys carry then loses nothing to the rounding
+// (2 x 512 tokens behind 4096, 32 heads of 128: 86 us instead of 75, for an error against fp64 of at
+// most 1.4 times the result's own rounding instead of 1.7).
 template <int HD, int BS, bool WIN, bool SCALED>
 __global__ void __launch_bounds__(kPfThreads, 1)
 prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
@@ -866,8 +870,12 @@ prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q,
               e0 = fast_exp2(x0);
               e1 = fast_exp2(x1);
             }
-            sum2[(kx >> 1) & 1] = add_f32x2(sum2[(kx >> 1) & 1], pack_f32x2(e0, e1));
             preg[kx >> 1] = pack_bf16x2(e0, e1);
+            if constexpr (SCALED) {   // the sum of the rounded weights: see above
+              e0 = __uint_as_float(preg[kx >> 1] << 16);
+              e1 = __uint_as_float(preg[kx >> 1] & 0xffff0000u);
+            }
+            sum2[(kx >> 1) & 1] = add_f32x2(sum2[(kx >> 1) & 1], pack_f32x2(e0, e1));
           }
           tmem_st_32x16(s_addr + c * 16, preg);
           if constexpr (SCALED) {
