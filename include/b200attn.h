@@ -330,8 +330,8 @@ size_t b200attn_decode_workspace_bytes(int num_users, int num_q_heads, int head_
  * (i, i + rotary_dim / 2) when is_neox_style, (2 i, 2 i + 1) otherwise (rotary_dim a multiple of
  * 16, <= head_size).  Computed in fp32 (the angle in fp64) and rounded to bf16 once, unlike
  * b200attn_rope_kv_scatter_slots, which rounds after every operation as the reference layer does.
- * q_out / k_out may be q / k themselves (same pointer and stride) or memory that overlaps neither
- * q, k nor v.  weight_f32: the weights are fp32, else bf16.  With slot_mapping the rounded k_out
+ * q_out / k_out may be q / k themselves (same pointer and stride); otherwise they overlap no part of
+ * q, k and each other, nor v when it is read.  weight_f32: the weights are fp32, else bf16.  With slot_mapping the rounded k_out
  * rows and v go to the caches (cache_dtype bf16 or unscaled e4m3) as b200attn_kv_scatter_slots_ex
  * writes them; of tokens with the same slot one, unspecified, wins.  slot_mapping == NULL: v and
  * the caches are not touched and may be NULL.

@@ -140,3 +140,44 @@ def test_ops_refuse_cpu_tensors():
                      torch.ones(32), 64, 64, w, w)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def _row_sets():
+    """40 tokens of 4 query heads and 2 + 2 KV heads of 64 side by side in rows of 512 elements, and
+    memory apart, as (pointer, row stride, row width) in bytes."""
+    step = 2 * 8 * 64
+    q, k, v = (4096, step, 512), (4096 + 512, step, 256), (4096 + 768, step, 256)
+    far = 1 << 20
+    return q, k, v, (far, 512, 512), (far + 40 * 512, 256, 256)
+
+
+def test_outputs_that_overlap_nothing_they_may_not_are_taken():
+    from b200attn.ops import _check_outputs
+
+    q, k, v, oq, ok = _row_sets()
+    unread = (0, 0, 256)
+    for outs in ((q, k), (oq, ok), (q, ok), (oq, k)):
+        for val in (v, unread):
+            _check_outputs(40, *outs, q, k, val)
+    # value where a key goes is nothing to a call that does not read it
+    _check_outputs(40, q, k, q, k, unread)
+    for n in (1, 40):                                    # memory side by side, strides apart
+        _check_outputs(n, (0, 512, 512), (n * 512, 256, 256), (0, 512, 512), (n * 512, 256, 256),
+                       (n * 768, 256, 256))
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_outputs_that_overlap_what_is_still_read_are_refused(tokens):
+    """In place or not: an output on the value's rows, on the other input's, on the other output's,
+    or on part of its own input's."""
+    from b200attn.ops import _check_outputs
+
+    q, k, v, oq, ok = _row_sets()
+    half = (k[0] + 128, k[1], k[2])
+    for outs, ins in (((q, k), (q, k, k)),               # value is the key, both in place
+                      ((oq, k), (q, k, k)), ((q, ok), (q, k, q)), ((q, k), (q, k, q)),
+                      ((q, v), (q, k, v)), ((v, ok), (q, k, v)), ((oq, k), (q, k, half)),
+                      ((q, ok), (q, q, v)), ((oq, k), (k, k, v)), ((q, k), (q, half, v)),
+                      ((oq, half), (q, k, v)), ((k, ok), (q, k, v)), ((oq, oq), (q, k, v))):
+        with pytest.raises(ValueError, match="overlap"):
+            _check_outputs(tokens, *outs, *ins)

@@ -194,3 +194,22 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="no CPU path"):
         call(wq=wq.cpu())
     call()
+
+
+def test_value_rows_under_an_output_are_refused():
+    """The value is read while rows are stored: it may not lie under a result, in place or not."""
+    from b200attn import ops
+
+    c = _case(4, 4, 2, 64, 64, seed=2, fused=False)
+    q, k, v = c["dev"]
+    args = (c["positions"].cuda(), c["inv_freq"].cuda(), 64, 64, c["wq"].cuda(), c["wk"].cuda())
+    kc = torch.zeros(2, 2, 32, 64, dtype=torch.bfloat16, device="cuda")
+    write = dict(eps=1e-6, k_cache=kc, v_cache=kc.clone(), slot_mapping=torch.arange(4).cuda())
+    before = q.clone(), k.clone()
+    for value, outs in ((k, {}), (k, dict(out_query=torch.empty_like(q))), (q[:, :128], {}),
+                        (q[:, 64:192], dict(out_key=torch.empty_like(k))),
+                        (v, dict(out_query=torch.empty_like(q), out_key=v))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.qk_norm_rope_kv_scatter_slots(q, k, value, *args, **write, **outs)
+    assert torch.equal(q, before[0]) and torch.equal(k, before[1]) and not kc.any()
+    ops.qk_norm_rope_kv_scatter_slots(q, k, k, *args)        # nothing reads the value here

@@ -309,8 +309,9 @@ def _rows_meet(a: tuple, b: tuple, tokens: int) -> bool:
 
 
 def _check_outputs(tokens: int, oq: tuple, ok: tuple, q: tuple, k: tuple, v: tuple) -> None:
-    """Each output is its input or shares no memory with any input, nor with the other output; all
-    as (pointer, row stride, row width) in bytes, v's pointer 0 when it is not read."""
+    """Each output is its input or shares no memory with it, and shares none with the other input,
+    with v (read when its pointer is not 0) and with the other output: the kernel stores a token's
+    rows while it still reads others of them.  All as (pointer, row stride, row width) in bytes."""
     # the usual case first: outputs on either side of everything else
     last = tokens - 1
     lo = min(q[0], k[0], v[0] or q[0])
@@ -319,9 +320,9 @@ def _check_outputs(tokens: int, oq: tuple, ok: tuple, q: tuple, k: tuple, v: tup
     if (oq[0] >= hi or oq_end <= lo) and (ok[0] >= hi or ok_end <= lo) and \
             (oq[0] >= ok_end or ok[0] >= oq_end):
         return
-    for out, own in ((oq, q), (ok, k)):
-        if out != own and (_rows_meet(out, q, tokens) or _rows_meet(out, k, tokens)
-                           or (v[0] and _rows_meet(out, v, tokens))):
+    for out, own, other in ((oq, q, k), (ok, k, q)):
+        if _rows_meet(out, other, tokens) or (v[0] and _rows_meet(out, v, tokens)) \
+                or (out != own and _rows_meet(out, own, tokens)):
             raise ValueError("an output must be its input or overlap none of the inputs")
     if _rows_meet(oq, ok, tokens):
         raise ValueError("the outputs must not overlap")
@@ -351,7 +352,8 @@ def qk_norm_rope_kv_scatter_slots(
     pass.  Computed in fp32 (angles in fp64) and rounded to bf16 once.  `query` [tokens, nq*hd],
     `key` / `value` [tokens, nkv*hd], dense rows of any row stride; results go to `out_query` /
     `out_key` of the same shapes, or in place when these are not given.  An output either is its
-    input or overlaps none of the inputs.  Pairs are (i, i + rotary_dim/2) for `is_neox_style`,
+    input or does not overlap it; it overlaps no other input (nor `value`, when that is written to
+    the cache) and not the other output.  Pairs are (i, i + rotary_dim/2) for `is_neox_style`,
     (2i, 2i + 1) otherwise.  Caches: bf16 or unscaled e4m3 (`paged_write` fills block-scaled
     ones).  Returns (out_query, out_key)."""
     oq = query if out_query is None else out_query
@@ -411,12 +413,9 @@ def qk_norm_rope_kv_scatter_slots(
     if tokens == 0:
         return oq, ok
     oq_ptr, ok_ptr, q_ptr, k_ptr = oq.data_ptr(), ok.data_ptr(), query.data_ptr(), key.data_ptr()
-    if oq_ptr != q_ptr or ok_ptr != k_ptr or oq_stride != q_stride or ok_stride != k_stride:
-        _check_outputs(tokens, (oq_ptr, 2 * oq_stride, 2 * q_width),
-                       (ok_ptr, 2 * ok_stride, 2 * k_width), (q_ptr, 2 * q_stride, 2 * q_width),
-                       (k_ptr, 2 * k_stride, 2 * k_width), (v_ptr, 2 * v_stride, 2 * k_width))
-    elif _rows_meet((q_ptr, 2 * q_stride, 2 * q_width), (k_ptr, 2 * k_stride, 2 * k_width), tokens):
-        raise ValueError("query and key overlap: they cannot both be replaced in place")
+    _check_outputs(tokens, (oq_ptr, 2 * oq_stride, 2 * q_width),
+                   (ok_ptr, 2 * ok_stride, 2 * k_width), (q_ptr, 2 * q_stride, 2 * q_width),
+                   (k_ptr, 2 * k_stride, 2 * k_width), (v_ptr, 2 * v_stride, 2 * k_width))
     status = _lib.lib().b200attn_qk_norm_rope_kv_scatter_slots(
         oq_ptr, oq_stride, ok_ptr, ok_stride, q_ptr, q_stride, k_ptr, k_stride,
         v_ptr, v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
