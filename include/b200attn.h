@@ -420,6 +420,8 @@ size_t b200attn_decode_scaled_workspace_bytes(int num_users, int num_q_heads, in
  *   out_table [num_users, num_kv_heads, num_pages]: the page ids in context order, 0 behind them;
  *   out_pos   [num_users, num_kv_heads]: position of the newest key within that list, -1 for a
  *     user without context (cur_pos < 0).
+ * A position behind the end of the page table is reported (diagnostics word 2) and gives the choice
+ * at the table's last key, as b200attn_paged_decode_blocks attends up to it.
  * Both are what b200attn_paged_decode_blocks takes.  num_q_heads / num_kv_heads <= 16.
  * max_context_len (0: unknown) only shapes the launch.  Workspace:
  * b200attn_select_pages_workspace_bytes bytes whose first B200ATTN_DECODE_TICKET_BYTES follow the

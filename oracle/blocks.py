@@ -153,8 +153,8 @@ def select_pages(query, k_bounds, page_table, cur_pos, bs, num_pages, keep_first
     table = torch.zeros(users, nkv, num_pages, dtype=torch.int32)
     pos = torch.full((users, nkv), -1, dtype=torch.int32)
     for u in range(users):
-        p = int(cur_pos[u])
-        n = min(p // bs + 1, page_table.shape[1]) if p >= 0 else 0
+        p = min(int(cur_pos[u]), page_table.shape[1] * bs - 1)      # behind the table: its last key
+        n = p // bs + 1 if p >= 0 else 0
         for h in range(nkv):
             if n == 0:
                 continue

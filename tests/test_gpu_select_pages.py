@@ -135,6 +135,23 @@ def test_bad_pages_are_reported_and_rank_last():
     assert -2 not in table.cpu()[0].flatten().tolist()
 
 
+@pytest.mark.parametrize("pages", [6, 64])
+@pytest.mark.parametrize("behind", [0, 5, 2 ** 31])
+def test_positions_behind_the_table_are_reported(pages, behind):
+    """The choice is the one at the table's last key, whether every page is taken or some are."""
+    from b200attn import ops
+
+    ops.read_error_word()
+    c = _case(2, 4, 2, 64, 32, [20 * 32, 20 * 32], seed=8)
+    c["table"] = c["table"][:, :20].contiguous()
+    want = _check(c, 32, pages, 1, 1)
+    assert ops.read_error_word() == 0
+    c["pos"][1] = min(20 * 32 + behind, 2 ** 31 - 1)
+    got = _check(c, 32, pages, 1, 1)
+    assert ops.read_error_word() == 2
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("nq,nkv,hd,bs", [(8, 2, 64, 32), (32, 8, 128, 64), (32, 2, 128, 32)])
 @pytest.mark.parametrize("splits", [0, 1, 3])
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.int8, torch.float8_e4m3fn])

@@ -601,7 +601,8 @@ def select_pages(
     queries (equal scores: the lower page).  `query` [users, nq, hd]; `k_bounds` as `paged_write`
     keeps them; `page_table` [users, width] and `cur_pos` [users] as for `paged_decode`.
     Returns (table [users, nkv, num_pages], pos [users, nkv]): hand them to `paged_decode` as
-    `page_table` and `cur_pos`.  `max_context_len` only shapes the launch."""
+    `page_table` and `cur_pos`.  A position behind the table is reported (diagnostics word 2) and
+    gives the choice at the table's last key.  `max_context_len` only shapes the launch."""
     index = _device_of(query, k_bounds, page_table, cur_pos, workspace)
     if _current_device() != index:       # the library works on the current device
         with torch.cuda.device(index):

@@ -180,10 +180,11 @@ __global__ void __launch_bounds__(kSelThreads, NG == 1 ? 2 : 1) select_pages_ker
   const int64_t uh = static_cast<int64_t>(user) * p.num_kv_heads + kvh;
   int32_t* table = p.out_table + uh * p.num_pages;
   const int32_t* pt = p.page_table + static_cast<int64_t>(user) * p.page_table_stride;
-  int n = pos < 0 ? 0 : pos / BS + 1;
-  n = min(n, p.max_pages);
-  // position within the last page: a context longer than the table ends with the table
-  const int in_page = pos < 0 ? 0 : (pos / BS + 1 > n ? BS - 1 : pos % BS);
+  // a position behind the table is reported; the choice is then the one at the table's last key
+  const bool behind = pos >= 0 && pos / BS >= p.max_pages;
+  if (behind && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.err_word, kDevBadIndex);
+  const int n = pos < 0 ? 0 : behind ? p.max_pages : pos / BS + 1;
+  const int in_page = pos < 0 ? 0 : behind ? BS - 1 : pos % BS;    // of the newest key
 
   if (n <= p.num_pages) {            // everything is taken
     if (blockIdx.x != 0) return;
