@@ -152,6 +152,15 @@ def test_positions_behind_the_table_are_reported(pages, behind):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("q_exp,b_exp", [(-70, -75), (-100, -30), (-76, -76), (-85, -66)])
+def test_scores_below_the_normal_range(clean_error_word, q_exp, b_exp):
+    """Products and sums that fp32 flushes or holds in a few bits: the exact order decides."""
+    c = _case(2, 8, 2, 64, 32, [100 * 32, 37 * 32 + 5], seed=12)
+    c["query"] *= 2.0 ** q_exp
+    c["k_bounds"] *= 2.0 ** b_exp
+    _check(c, 32, 20, 1, 1)
+
+
 @pytest.mark.parametrize("nq,nkv,hd,bs", [(8, 2, 64, 32), (32, 8, 128, 64), (32, 2, 128, 32)])
 @pytest.mark.parametrize("splits", [0, 1, 3])
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.int8, torch.float8_e4m3fn])

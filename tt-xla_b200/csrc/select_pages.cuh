@@ -14,7 +14,9 @@
 // The choice is the one the exact scores make.  bf16 products are exact in fp32 and the fp32 sum of
 // 2 * head_size of them is off by at most 4 * head_size * 2^-23 times the sum of their magnitudes
 // (a second MMA with |q| and |bounds|): 2 * head_size terms and head_size / 8 accumulators are
-// added, each addition truncating at worst, and the factor covers that almost twice.  Only pages
+// added, each addition truncating at worst, and the factor covers that almost twice.  Below the
+// normal range a product or an addition may lose all of itself, less than FLT_MIN each: 4 * head_size
+// times that is added, which no score of an ordinary size notices.  Only pages
 // whose fp32 score is within twice that of the border can be on the wrong side of it: these few
 // are summed again in fp64, and the border is drawn among them.
 //
@@ -26,6 +28,8 @@
 // scoring takes 20 (3.4 TB/s: 512-byte pieces, one round of CTAs) and choosing 9; 62 with a radix
 // choice in global memory, 33 before the next group's bounds were loaded ahead.
 #pragma once
+#include <cfloat>
+
 #include "kv_scatter.cuh"
 
 namespace b200attn {
@@ -332,7 +336,8 @@ __global__ void __launch_bounds__(kSelThreads, NG == 1 ? 2 : 1) select_pages_ker
           mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
         }
         if (tq == 0 && cur.row[r] >= 0)
-          put[cur.row[r]] = cur.blk[r] >= 0 ? make_float2(best, mag * (4.f * HD / 8388608.f))
+          put[cur.row[r]] = cur.blk[r] >= 0
+                                ? make_float2(best, mag * (4.f * HD / 8388608.f) + 4.f * HD * FLT_MIN)
                                             : make_float2(-INFINITY, 0.f);
       }
       cur = nxt;
