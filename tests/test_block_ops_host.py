@@ -1,5 +1,7 @@
 """Refusals of the block-scaled / page-list / norm entry points, and the shapes that
 allocate_kv_caches makes for them: no GPU needed, nothing is launched."""
+import threading
+
 import pytest
 import torch
 
@@ -181,3 +183,106 @@ def test_outputs_that_overlap_what_is_still_read_are_refused(tokens):
                       ((oq, half), (q, k, v)), ((k, ok), (q, k, v)), ((oq, oq), (q, k, v))):
         with pytest.raises(ValueError, match="overlap"):
             _check_outputs(tokens, *outs, *ins)
+
+
+class _RecordingLibrary:
+    """Stands in for the library: notes which memory each launch is given; a `meet` barrier holds
+    every thread between its two launches until all of them are there."""
+
+    def __init__(self, meet=None):
+        self.meet, self.widened, self.attended = meet, {}, {}
+
+    def _note_widened(self, spans):
+        self.widened[threading.get_ident()] = spans
+        if self.meet is not None:
+            self.meet.wait(30)
+        return 0
+
+    def b200attn_dequant_pages_scaled(self, k, v, factors, *rest):
+        width, seqs, nkv, hd, bs = rest[7], rest[10], rest[11], rest[12], rest[13]
+        pages = seqs * width
+        half = pages * nkv * bs * hd * 2
+        return self._note_widened([(k, half), (v, half), (factors, pages * nkv * 8)])
+
+    def b200attn_prefill_scaled(self, out, ostride, q, qstride, k, v, factors, *rest):
+        self.attended[threading.get_ident()] = [k, v, factors]
+        return 0
+
+
+@pytest.fixture()
+def stubbed(monkeypatch):
+    """ops on CPU tensors against a recording library."""
+    from b200attn import ops
+
+    def use(library):
+        monkeypatch.setattr(ops._lib, "lib", lambda: library)
+        for name, value in (("_need_cuda", lambda *t: None), ("_device_of", lambda *t: 0),
+                            ("_current_device", lambda: 0), ("_raw_stream", lambda index: 7),
+                            ("_stream", lambda t: 7)):
+            monkeypatch.setattr(ops, name, value)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        return ops
+
+    return use
+
+
+def _prefill_call(ops, kind, seqs=2, width=4, **kw):
+    cache = torch.zeros(8, 2, 32, 128, dtype=kind)
+    scales = {} if kind == torch.float8_e4m3fn and kw.pop("unscaled", False) else \
+        dict(k_scale=torch.ones(8, 2), v_scale=torch.ones(8, 2))
+    cu = torch.arange(seqs + 1, dtype=torch.int32) * 3
+    return ops.prefill(torch.zeros(3 * seqs, 4, 128, dtype=torch.bfloat16), cache, cache.clone(), cu,
+                       page_table=torch.zeros(seqs, width, dtype=torch.int32), cu_q=cu,
+                       q_start=torch.zeros(seqs, dtype=torch.int32), **scales, **kw)
+
+
+def _check_each_thread_attends_what_it_widened(lib, threads):
+    spans = []
+    assert len(lib.widened) == len(lib.attended) == threads
+    for thread, mine in lib.widened.items():
+        assert lib.attended[thread] == [at for at, _ in mine]
+        spans += mine
+    spans.sort()
+    assert all(a + n <= b for (a, n), (b, _) in zip(spans, spans[1:]))
+
+
+def _in_threads(n, call):
+    errors = []
+
+    def run():
+        try:
+            call()
+        except Exception as e:                   # noqa: BLE001  (reported by the caller's thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run) for _ in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_prefills_on_one_stream_widen_into_pools_of_their_own(stubbed):
+    """Three threads have all widened their pages before the first of them attends."""
+    lib = _RecordingLibrary(threading.Barrier(3))
+    ops = stubbed(lib)
+    _in_threads(3, lambda: _prefill_call(ops, torch.int8))
+    _check_each_thread_attends_what_it_widened(lib, 3)
+
+
+def test_identity_tables(stubbed, monkeypatch):
+    """One per stream, whatever shapes ask for it; a capture makes its own."""
+    ops = stubbed(_RecordingLibrary())
+    monkeypatch.setattr(ops, "_identity_tables", {})
+    dev = torch.device("cpu")
+    for seqs, width in ((1, 1), (3, 5), (7, 3), (5, 2000), (2, 9)):
+        want = torch.arange(seqs * width, dtype=torch.int32).view(seqs, width)
+        assert torch.equal(ops._identity_table(dev, 1, seqs, width), want)
+    assert len(ops._identity_tables) == 1
+    kept = ops._identity_tables[(None, 1)]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    own = ops._identity_table(dev, 1, 2, 3)
+    assert own.data_ptr() != kept.data_ptr() and own.tolist() == [[0, 1, 2], [3, 4, 5]]
+    assert ops._identity_table(dev, 2, 2, 3).data_ptr() != own.data_ptr()
+    assert list(ops._identity_tables) == [(None, 1)]

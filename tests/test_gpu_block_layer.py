@@ -348,3 +348,35 @@ def test_layer_refusals():
     sparse = B200AttentionBackendImpl(NQ, HD, 0.1, NKV, sparse_pages=4)
     with pytest.raises(ValueError, match="bounds"):
         sparse._page_values(kv, tuple(kv))
+
+
+def test_prefills_of_two_threads_on_one_stream(clean_error_word):
+    """Each attends over the pages it widened, whatever the other enqueues in between."""
+    import threading
+
+    from b200attn import ops
+
+    cases = []
+    for i in range(2):
+        cache, table = _decode_setup("int8_block", 2, 300, 60 + i)
+        cu = torch.tensor([0, 33, 97], dtype=torch.int32)
+        q = torch.randn(97, NQ, HD, generator=torch.Generator().manual_seed(i)).bfloat16().cuda()
+        args = (q, cache[0], cache[1], cu)
+        kw = dict(page_table=table, q_start=torch.tensor([200, 230], dtype=torch.int32).cuda(),
+                  cu_q=cu.cuda(), k_scale=cache[2], v_scale=cache[3])
+        cases.append((args, kw, ops.prefill(*args, **kw).clone()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+
+    def run(i):
+        args, kw, _ = cases[i]
+        outs[i] += [ops.prefill(*args, **kw) for _ in range(200)]
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for mine, (_, _, want) in zip(outs, cases):
+        assert len(mine) == 200 and all(torch.equal(o, want) for o in mine)

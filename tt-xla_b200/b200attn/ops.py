@@ -912,8 +912,8 @@ def prefill(
         cu_q = cu_q_host.to(query.device, non_blocking=True)
     _i32(cu_q, "cu_q")
     if scaled:
-        k, v, factors, page_table, nb = _widen_scaled_pages(k_src, v_src, k_scale, v_scale,
-                                                            page_table, cu_q, q_start, num_seqs)
+        pool, k_ptr, v_ptr, factors, page_table, nb = _widen_scaled_pages(
+            k_src, v_src, k_scale, v_scale, page_table, cu_q, q_start, num_seqs)
     elif paged and k_src.dtype == torch.float8_e4m3fn:
         # The tcgen05 kernel takes 16-bit tiles: widen the pages this batch reads into a bf16
         # scratch pool laid out [sequence][page slot] and attend over that through the identity
@@ -934,10 +934,10 @@ def prefill(
     if scaled:
         status = L.b200attn_prefill_scaled(
             out_t.data_ptr(), ostride, q.data_ptr(),
-            qstride if total_q > 1 else max(qstride, nq * hd), k.data_ptr(), v.data_ptr(),
-            factors.data_ptr(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-            cu_q.data_ptr(), cu_q_host.data_ptr(), q_start.data_ptr() if q_start is not None else 0,
-            num_seqs, total_q, nq, nkv, hd, bs, nb, scale, sliding_window, _raw_stream(index))
+            qstride if total_q > 1 else max(qstride, nq * hd), k_ptr, v_ptr, factors,
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_q.data_ptr(),
+            cu_q_host.data_ptr(), q_start.data_ptr() if q_start is not None else 0, num_seqs,
+            total_q, nq, nkv, hd, bs, nb, scale, sliding_window, _raw_stream(index))
         if status:
             _lib.check("b200attn_prefill_scaled", status)
         return out if out is not None else out_t
@@ -994,40 +994,49 @@ def _widen_fp8_pages(k_cache, v_cache, page_table, cu_q, q_start, num_seqs):
     return k_pool, v_pool, ident, k_pool.shape[0]
 
 
-_scaled_scratch: dict[tuple, tuple] = {}
+_identity_tables: dict[tuple, torch.Tensor] = {}
+
+
+def _identity_table(device: torch.device, stream: int, seqs: int, width: int) -> torch.Tensor:
+    """[seqs, width] int32 table of the pages 0, 1, 2, ... on the current device: a view of one table
+    per stream that grows on demand; under stream capture one of the graph's own."""
+    pages = seqs * width
+    have = None
+    capturing = torch.cuda.is_current_stream_capturing()
+    if not capturing:
+        have = _identity_tables.get((device.index, stream))
+    if have is None or have.numel() < pages:
+        size = pages if capturing else max(4096, 1 << (pages - 1).bit_length())
+        have = torch.arange(size, dtype=torch.int32, device=device)
+        if not capturing:
+            _identity_tables[(device.index, stream)] = have
+    return have[:pages].view(seqs, width)
 
 
 def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_start, num_seqs):
-    """_widen_fp8_pages for a block-scaled cache pair on the current device: (k_pool, v_pool, the pages' factors, identity
-    page table, pool size).  Under stream capture the pool belongs to the graph being captured."""
+    """bf16 pages, laid out as _widen_fp8_pages does, of a block-scaled cache pair on the current
+    device, and what is left of their scales; returns (the memory that holds them, the addresses
+    of the K pages, of the V pages and of the factors in it, identity page table, pages).  The
+    memory belongs to the call: what another thread enqueues between the two launches, on this
+    stream too, has its own.  torch's allocator hands it out again in stream order only."""
     nb, nkv, bs, hd = k_cache.shape
     width = page_table.shape[1]
     pages = max(num_seqs * width, 1)
     dev = k_cache.device
     stream = _raw_stream(dev.index)
-    capturing = torch.cuda.is_current_stream_capturing()
-    key = (dev.index, stream, nkv, bs, hd)
-    have = None if capturing else _scaled_scratch.get(key)
-    if have is None or have[0].shape[0] < pages:
-        grow = pages if have is None else max(pages, 2 * have[0].shape[0])
-        have = (torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
-                torch.empty((grow, nkv, bs, hd), dtype=torch.bfloat16, device=dev),
-                torch.empty((grow, nkv, 2), dtype=torch.float32, device=dev), {})
-        if not capturing:
-            _scaled_scratch[key] = have
-    k_pool, v_pool, factors, tables = have
-    ident = tables.get((num_seqs, width))
-    if ident is None:
-        ident = torch.arange(num_seqs * width, dtype=torch.int32, device=dev)
-        ident = tables[(num_seqs, width)] = ident.reshape(num_seqs, width)
+    half = pages * nkv * bs * hd * 2
+    pool = torch.empty(2 * half + pages * nkv * 8, dtype=torch.uint8, device=dev)
+    k_pool = pool.data_ptr()
+    v_pool, factors = k_pool + half, k_pool + 2 * half
     _lib.check(
         "b200attn_dequant_pages_scaled",
         _lib.lib().b200attn_dequant_pages_scaled(
-            k_pool.data_ptr(), v_pool.data_ptr(), factors.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _cache_dtype(k_cache),
-            page_table.data_ptr(), page_table.stride(0), width, cu_q.data_ptr(),
-            q_start.data_ptr() if q_start is not None else 0, num_seqs, nkv, hd, bs, nb, stream))
-    return k_pool, v_pool, factors, ident, k_pool.shape[0]
+            k_pool, v_pool, factors, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), _cache_dtype(k_cache), page_table.data_ptr(), page_table.stride(0),
+            width, cu_q.data_ptr(), q_start.data_ptr() if q_start is not None else 0, num_seqs,
+            nkv, hd, bs, nb, stream))
+    table = _identity_table(dev, stream, num_seqs, width)
+    return pool, k_pool, v_pool, factors, table, pages
 
 
 def read_error_word(device: Optional[torch.device] = None) -> int:
