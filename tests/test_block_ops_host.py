@@ -1,6 +1,8 @@
 """Refusals of the block-scaled / page-list / norm entry points, and the shapes that
 allocate_kv_caches makes for them: no GPU needed, nothing is launched."""
 import threading
+import time
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -190,7 +192,7 @@ class _RecordingLibrary:
     every thread between its two launches until all of them are there."""
 
     def __init__(self, meet=None):
-        self.meet, self.widened, self.attended = meet, {}, {}
+        self.meet, self.widened, self.attended, self.order = meet, {}, {}, []
 
     def _note_widened(self, spans):
         self.widened[threading.get_ident()] = spans
@@ -203,6 +205,16 @@ class _RecordingLibrary:
         pages = seqs * width
         half = pages * nkv * bs * hd * 2
         return self._note_widened([(k, half), (v, half), (factors, pages * nkv * 8)])
+
+    def b200attn_dequant_pages_fp8(self, k, v, *rest):
+        self.order.append(("widen", threading.get_ident()))
+        if self.meet is not None:
+            time.sleep(0.05)                     # time for another thread to come in between
+        return 0
+
+    def b200attn_prefill_ex(self, *args):
+        self.order.append(("attend", threading.get_ident()))
+        return 0
 
     def b200attn_prefill_scaled(self, out, ostride, q, qstride, k, v, factors, *rest):
         self.attended[threading.get_ident()] = [k, v, factors]
@@ -226,10 +238,9 @@ def stubbed(monkeypatch):
     return use
 
 
-def _prefill_call(ops, kind, seqs=2, width=4, **kw):
-    cache = torch.zeros(8, 2, 32, 128, dtype=kind)
-    scales = {} if kind == torch.float8_e4m3fn and kw.pop("unscaled", False) else \
-        dict(k_scale=torch.ones(8, 2), v_scale=torch.ones(8, 2))
+def _prefill_call(ops, kind, seqs=2, width=4, scaled=True, **kw):
+    cache = torch.zeros(8, 2, 32, 128).to(kind)
+    scales = dict(k_scale=torch.ones(8, 2), v_scale=torch.ones(8, 2)) if scaled else {}
     cu = torch.arange(seqs + 1, dtype=torch.int32) * 3
     return ops.prefill(torch.zeros(3 * seqs, 4, 128, dtype=torch.bfloat16), cache, cache.clone(), cu,
                        page_table=torch.zeros(seqs, width, dtype=torch.int32), cu_q=cu,
@@ -269,6 +280,18 @@ def test_prefills_on_one_stream_widen_into_pools_of_their_own(stubbed):
     ops = stubbed(lib)
     _in_threads(3, lambda: _prefill_call(ops, torch.int8))
     _check_each_thread_attends_what_it_widened(lib, 3)
+
+
+def test_unscaled_e4m3_prefills_do_not_come_between_each_other(stubbed, monkeypatch):
+    """The pool of a stream is shared: who has widened into it attends before anyone else widens."""
+    lib = _RecordingLibrary(threading.Barrier(1))
+    ops = stubbed(lib)
+    monkeypatch.setattr(ops, "_fp8_scratch", {})
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: SimpleNamespace(cuda_stream=7))
+    _in_threads(3, lambda: _prefill_call(ops, torch.float8_e4m3fn, scaled=False))
+    assert len(lib.order) == 6
+    for first, second in zip(lib.order[::2], lib.order[1::2]):
+        assert first == ("widen", first[1]) and second == ("attend", first[1])
 
 
 def test_identity_tables(stubbed, monkeypatch):

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import threading
 from typing import Optional
 
 import torch
@@ -911,14 +912,6 @@ def prefill(
     if cu_q is None:
         cu_q = cu_q_host.to(query.device, non_blocking=True)
     _i32(cu_q, "cu_q")
-    if scaled:
-        pool, k_ptr, v_ptr, factors, page_table, nb = _widen_scaled_pages(
-            k_src, v_src, k_scale, v_scale, page_table, cu_q, q_start, num_seqs)
-    elif paged and k_src.dtype == torch.float8_e4m3fn:
-        # The tcgen05 kernel takes 16-bit tiles: widen the pages this batch reads into a bf16
-        # scratch pool laid out [sequence][page slot] and attend over that through the identity
-        # page table.  e4m3 -> bf16 is exact, so the kernel sees the cache's own values.
-        k, v, page_table, nb = _widen_fp8_pages(k_src, v_src, page_table, cu_q, q_start, num_seqs)
     if out is None:
         out_t = torch.empty((total_q, nq, hd), dtype=torch.bfloat16, device=query.device)
     else:
@@ -930,9 +923,10 @@ def prefill(
     ostride = out_t.stride(0) if total_q > 1 else max(out_t.stride(0), nq * hd)
     if scale is None:
         scale = hd ** -0.5
-    L = _lib.lib()
     if scaled:
-        status = L.b200attn_prefill_scaled(
+        pool, k_ptr, v_ptr, factors, page_table, nb = _widen_scaled_pages(
+            k_src, v_src, k_scale, v_scale, page_table, cu_q, q_start, num_seqs)
+        status = _lib.lib().b200attn_prefill_scaled(
             out_t.data_ptr(), ostride, q.data_ptr(),
             qstride if total_q > 1 else max(qstride, nq * hd), k_ptr, v_ptr, factors,
             page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_q.data_ptr(),
@@ -941,29 +935,43 @@ def prefill(
         if status:
             _lib.check("b200attn_prefill_scaled", status)
         return out if out is not None else out_t
-    _lib.check(
-        "b200attn_prefill_ex",
-        L.b200attn_prefill_ex(
-            out_t.data_ptr(), ostride, q.data_ptr(), qstride, k.data_ptr(), v.data_ptr(),
-            1 if paged else 0, kstride,
-            page_table.data_ptr() if paged else None,
-            page_table.stride(0) if paged else 0, page_table.shape[1] if paged else 0,
-            cu_q.data_ptr(), cu_q_host.data_ptr(),
-            q_start.data_ptr() if q_start is not None else None,
-            num_seqs, total_q, nq, nkv, hd, bs, nb, float(scale), int(sliding_window),
-            _stream(query),
-        ),
-    )
+
+    def attend(k, v, page_table, nb):
+        _lib.check(
+            "b200attn_prefill_ex",
+            _lib.lib().b200attn_prefill_ex(
+                out_t.data_ptr(), ostride, q.data_ptr(), qstride, k.data_ptr(), v.data_ptr(),
+                1 if paged else 0, kstride,
+                page_table.data_ptr() if paged else None,
+                page_table.stride(0) if paged else 0, page_table.shape[1] if paged else 0,
+                cu_q.data_ptr(), cu_q_host.data_ptr(),
+                q_start.data_ptr() if q_start is not None else None,
+                num_seqs, total_q, nq, nkv, hd, bs, nb, float(scale), int(sliding_window),
+                _stream(query),
+            ),
+        )
+
+    if paged and k_src.dtype == torch.float8_e4m3fn:
+        # The tcgen05 kernel takes 16-bit tiles: widen the pages this batch reads into a bf16
+        # scratch pool laid out [sequence][page slot] and attend over that through the identity
+        # page table.  e4m3 -> bf16 is exact, so the kernel sees the cache's own values.  The pool
+        # is shared by the calls on a stream, so no other thread may come between the two launches.
+        with _fp8_lock:
+            attend(*_widen_fp8_pages(k_src, v_src, page_table, cu_q, q_start, num_seqs))
+    else:
+        attend(k, v, page_table, nb)
     return out if out is not None else out_t
 
 
 _fp8_scratch: dict[tuple, tuple] = {}
+_fp8_lock = threading.Lock()
 
 
 def _widen_fp8_pages(k_cache, v_cache, page_table, cu_q, q_start, num_seqs):
     """bf16 copies of the pages `page_table[:num_seqs]` lists for an e4m3 cache pair; returns
     (k_pool, v_pool, identity page table, pool size in pages).  The scratch is cached per
-    (device, stream) and grown on demand; torch owns it."""
+    (device, stream) and grown on demand; torch owns it, and _fp8_lock is held from here to the
+    launch that reads it."""
     nb, nkv, bs, hd = k_cache.shape
     width = page_table.shape[1]
     pages = num_seqs * width
