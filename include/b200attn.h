@@ -446,7 +446,8 @@ int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
  * what is left of the scales: scale = factor * 2^e with the factor in [1, 2), the K factor itself
  * and the base-2 logarithm of the V factor.  b200attn_prefill_scaled is b200attn_prefill_ex
  * (kv_is_paged = 1) over that pool; it applies the factors in fp32, so the 8-bit values reach the
- * attention unrounded.  Rows that attend a page with a NaN scale come out as NaN. */
+ * attention unrounded.  Rows that attend a page with a NaN scale, or one whose id is out of range
+ * (reported: diagnostics word 2), come out as NaN. */
 int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, const void* k_cache,
                                   const void* v_cache, const float* k_scale, const float* v_scale,
                                   int cache_dtype, const int32_t* page_table,

@@ -451,6 +451,34 @@ def test_prefill_scales_far_apart_zero_and_nan(clean_error_word, bs):
         c[which] = keep
 
 
+@pytest.mark.parametrize("bad", [99, -3, 2 ** 31 - 1])
+def test_prefill_bad_page_is_reported_and_comes_out_as_nan(bad):
+    """For the rows that attend it and no others; no row shows what memory held before."""
+    from b200attn import ops
+
+    n, nq, nkv, hd, bs = 150, 4, 2, 64, 32
+    c = _decode_case(2, nq, nkv, hd, bs, [n, n], torch.int8, seed=5)
+    q = torch.randn(2 * n, nq, hd, generator=torch.Generator().manual_seed(2)).bfloat16()
+    cu = torch.tensor([0, n, 2 * n], dtype=torch.int32)
+
+    def run():
+        return ops.prefill(q.cuda(), c["k_cache"].cuda(), c["v_cache"].cuda(), cu,
+                           page_table=c["table"].cuda(), k_scale=c["k_scale"].cuda(),
+                           v_scale=c["v_scale"].cuda()).cpu()
+
+    ops.read_error_word()
+    want = run()
+    assert ops.read_error_word() == 0
+    c["table"][1, 2] = bad
+    for fill in (float("nan"), 1.0, 0.0):
+        junk = torch.full((1 << 22,), fill, device="cuda")      # what the allocator hands out next
+        del junk
+        got = run()
+        assert ops.read_error_word() == 2
+        assert torch.equal(got[: n + 2 * bs], want[: n + 2 * bs])
+        assert got[n + 2 * bs:].isnan().all()
+
+
 # ----------------------------------------------------------------------------------- refusals
 def test_refusals():
     from b200attn import ops

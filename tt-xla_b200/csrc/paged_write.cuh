@@ -380,9 +380,9 @@ __global__ void __launch_bounds__(kPwThreads, 8) paged_write_kernel(const PagedW
 // its rounding would be as large as the one of the result.  The pool therefore holds code * 2^e
 // with scale = f * 2^e, 1 <= f < 2, and the attention kernel applies the factors f in fp32:
 // `factors` gets (f of K, log2 f of V) for each page and head of the pool.  A zero scale gives zeros
-// and f = 1.  A page whose K or V scale is NaN (or no scale at all: negative, infinite)
-// gets NaN keys and zero values: rows that attend it come out as NaN, rows for which it is masked
-// do not.  Memory-bound: 1 byte read and 2 written per element (2 x 4608 tokens of 8 heads of 128,
+// and f = 1.  A page whose K or V scale is NaN (or no scale at all: negative, infinite), or whose id
+// is out of range (reported), gets NaN keys and zero values: rows that attend it come out as NaN,
+// rows for which it is masked do not.  Memory-bound: 1 byte read and 2 written per element (2 x 4608 tokens of 8 heads of 128,
 // 55 MB: 15 us).
 struct DequantScaledParams {
   const uint8_t* src[2];
@@ -428,14 +428,10 @@ __global__ void __launch_bounds__(128) dequant_scaled_kernel(const DequantScaled
   const int64_t dst_page =
       (static_cast<int64_t>(seq) * p.page_table_width + slot) * p.num_kv_heads + h;
   const bool ok = blk >= 0 && blk < p.num_blocks;
-  if (!ok && threadIdx.x == 0) {
-    atomicExch(p.err_word, kDevBadIndex);
-    if (z == 0) p.factors[dst_page] = make_float2(1.f, 0.f);
-  }
-  if (!ok) return;
-  const int64_t src_page = blk * p.num_kv_heads + h;
+  if (!ok && threadIdx.x == 0) atomicExch(p.err_word, kDevBadIndex);
+  const int64_t src_page = (ok ? blk : 0) * p.num_kv_heads + h;
   const float ks = __ldg(p.scale[0] + src_page), vs = __ldg(p.scale[1] + src_page);
-  const bool live = ks >= 0.f && ks < INFINITY && vs >= 0.f && vs < INFINITY;
+  const bool live = ok && ks >= 0.f && ks < INFINITY && vs >= 0.f && vs < INFINITY;
   const SplitScale sp = split_scale(z ? vs : ks);
   if (threadIdx.x == 0 && z == 0)
     p.factors[dst_page] = live ? make_float2(sp.f, log2f(split_scale(vs).f)) : make_float2(1.f, 0.f);
