@@ -383,7 +383,8 @@ int b200attn_paged_write(void* k_cache, void* v_cache, float* k_scale, float* v_
  *   k_scale / v_scale: both NULL (caches bf16, or unscaled e4m3 with head_size 128), or fp32
  *     [num_blocks, num_kv_heads] of caches written by b200attn_paged_write (cache_dtype INT8 or
  *     FP8_E4M3, head_size 64 or 128).  Codes are widened exactly; q (scaled by a power of two per
- *     head) and the softmax weights are rounded to f16, sums are fp32.  NaN scales give NaN rows.
+ *     head) and the softmax weights are rounded to f16, sums are fp32.  A page whose scale is
+ *     NaN, negative or infinite gives NaN rows.
  *   page_table_head_stride > 0: page_table is [num_users, num_kv_heads, width] with that stride
  *     between heads, cur_pos is [num_users, num_kv_heads] and counts within the list: the keys
  *     of the list's pages 0 .. cur_pos / block_size are attended, the last page up to
@@ -446,8 +447,8 @@ int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
  * what is left of the scales: scale = factor * 2^e with the factor in [1, 2), the K factor itself
  * and the base-2 logarithm of the V factor.  b200attn_prefill_scaled is b200attn_prefill_ex
  * (kv_is_paged = 1) over that pool; it applies the factors in fp32, so the 8-bit values reach the
- * attention unrounded.  Rows that attend a page with a NaN scale, or one whose id is out of range
- * (reported: diagnostics word 2), come out as NaN. */
+ * attention unrounded.  Rows that attend a page whose scale is NaN, negative or infinite, or whose
+ * id is out of range (reported: diagnostics word 2), come out as NaN. */
 int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, const void* k_cache,
                                   const void* v_cache, const float* k_scale, const float* v_scale,
                                   int cache_dtype, const int32_t* page_table,

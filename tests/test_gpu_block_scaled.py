@@ -385,6 +385,33 @@ def test_many_users_are_cut_between_pairs(clean_error_word):
     _attention_close(two[sub], small)
 
 
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("value", [-0.01, float("-inf"), float("inf"), float("nan")])
+def test_what_is_no_scale_comes_out_as_nan(clean_error_word, which, value):
+    """Negative and infinite scales in decode and in prefill: NaN for who attends the page and no
+    one else, as a NaN scale."""
+    from b200attn import ops
+
+    n, bs, nq, nkv, hd = 150, 32, 8, 2, 64
+    c = _decode_case(2, nq, nkv, hd, bs, [n, n], torch.int8, seed=6)
+    q = torch.randn(n, nq, hd, generator=torch.Generator().manual_seed(2)).bfloat16()
+    cu = torch.tensor([0, n], dtype=torch.int32)
+
+    def prefill():
+        return ops.prefill(q.cuda(), c["k_cache"].cuda(), c["v_cache"].cuda(), cu,
+                           page_table=c["table"][:1].cuda(), k_scale=c["k_scale"].cuda(),
+                           v_scale=c["v_scale"].cuda()).cpu()
+
+    good = [[_decode(c, num_splits=s) for s in (0, 1, 3)], prefill()]
+    c[which][int(c["table"][0, 2]), 1] = value
+    for got, want in zip([_decode(c, num_splits=s) for s in (0, 1, 3)], good[0]):
+        assert got[0, 4:].isnan().all()
+        assert torch.equal(got[0, :4], want[0, :4]) and torch.equal(got[1], want[1])
+    got = prefill()
+    assert got[2 * bs:, 4:].isnan().all()
+    assert torch.equal(got[: 2 * bs], good[1][: 2 * bs]) and torch.equal(got[:, :4], good[1][:, :4])
+
+
 # ------------------------------------------------------------------------------------ prefill
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("nq,nkv,hd,bs", [(8, 2, 64, 32), (8, 8, 128, 64), (12, 3, 128, 32)])

@@ -432,8 +432,10 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
         w.id = pt[idx];
         const bool ok = w.id >= 0 && w.id < p.num_blocks;
         const int64_t at = ok ? static_cast<int64_t>(w.id) * p.num_kv_heads + kvh : kvh;
-        w.ks = __ldg(sp.k_scale + at);
-        w.vs = __log2f(__ldg(sp.v_scale + at));
+        // what is no scale (negative, infinite) is read as NaN, as prefill does
+        const float ks = __ldg(sp.k_scale + at), vs = __ldg(sp.v_scale + at);
+        w.ks = ks >= 0.f && ks < INFINITY ? ks : NAN;
+        w.vs = vs >= 0.f && vs < INFINITY ? __log2f(vs) : NAN;
         return w;
       };
       int win_base = seg.t_begin * L::kPages;
