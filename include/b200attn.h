@@ -379,12 +379,13 @@ int b200attn_paged_write(void* k_cache, void* v_cache, float* k_scale, float* v_
 /* ------------------------------------------------------------------------------------------
  * Paged GQA decode attention over block-scaled 8-bit caches and / or over a page list per KV head.
  * No counterpart in the reference; b200attn_paged_decode_ex in every other respect (splits,
- * workspace, sinks, NaN in masked rows).
+ * workspace, sinks, NaN behind the context).
  *   k_scale / v_scale: both NULL (caches bf16, or unscaled e4m3 with head_size 128), or fp32
  *     [num_blocks, num_kv_heads] of caches written by b200attn_paged_write (cache_dtype INT8 or
  *     FP8_E4M3, head_size 64 or 128).  Codes are widened exactly; q (scaled by a power of two per
  *     head) and the softmax weights are rounded to f16, sums are fp32.  A page whose scale is
- *     NaN, negative or infinite gives NaN rows.
+ *     NaN, negative or infinite gives NaN rows; what codes masked rows hold (behind the context, in
+ *     front of the window), NaN among them, does not matter.
  *   page_table_head_stride > 0: page_table is [num_users, num_kv_heads, width] with that stride
  *     between heads, cur_pos is [num_users, num_kv_heads] and counts within the list: the keys
  *     of the list's pages 0 .. cur_pos / block_size are attended, the last page up to

@@ -385,6 +385,22 @@ def test_many_users_are_cut_between_pairs(clean_error_word):
     _attention_close(two[sub], small)
 
 
+@pytest.mark.parametrize("hd,bs", [(64, 32), (128, 64)])
+@pytest.mark.parametrize("splits", [0, 1, 2])
+@pytest.mark.parametrize("window", [1, 13, 40])
+def test_decode_ignores_nan_codes_in_front_of_the_window(clean_error_word, hd, bs, splits, window):
+    """e4m3 NaN codes in rows that a sliding window has left behind."""
+    ctx = [20, 64, 139, 300]
+    c = _decode_case(4, 8, 2, hd, bs, ctx, torch.float8_e4m3fn, seed=8)
+    want = _decode(c, num_splits=splits, sliding_window=window)
+    for u, n in enumerate(ctx):
+        for j in range(max(0, n - window)):
+            blk = int(c["table"][u, j // bs])
+            for name in ("k_cache", "v_cache"):
+                c[name].view(torch.uint8)[blk, :, j % bs] = 0x7F
+    assert torch.equal(_decode(c, num_splits=splits, sliding_window=window), want)
+
+
 @pytest.mark.parametrize("which", ["k_scale", "v_scale"])
 @pytest.mark.parametrize("value", [-0.01, float("-inf"), float("inf"), float("nan")])
 def test_what_is_no_scale_comes_out_as_nan(clean_error_word, which, value):

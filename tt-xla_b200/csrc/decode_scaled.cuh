@@ -591,10 +591,11 @@ paged_decode_scaled_kernel(const __grid_constant__ CUtensorMap tm_k,
     if (tok0 < ctx && tok0 + kDsWarpTokens > lo) {  // at least one of this warp's keys is attended
       const bool tail = (tok0 + kDsWarpTokens > ctx) || (tok0 < lo);
       if (tail && FMT != kPageInt8) {
-        // Rows past the context may hold NaN codes: zero them, 0 * NaN would reach the sums.
+        // Rows past the context, and rows a window has left behind, may hold NaN codes: zero them,
+        // 0 * NaN would reach the sums.
         for (int i = lane; i < kDsWarpTokens * (HD / 16); i += 32) {
           const int r = warp * kDsWarpTokens + i / (HD / 16), c = i % (HD / 16);
-          if (t * kDsTile + r >= ctx) {
+          if (t * kDsTile + r >= ctx || t * kDsTile + r < lo) {
             const uint32_t b = static_cast<uint32_t>(r * HD + c * 16);
             const uint32_t a = vbase + (b & ~127u) + ((((b >> 4) & 7u) ^ ((b >> 7) & 7u)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory");
