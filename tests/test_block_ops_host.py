@@ -309,3 +309,31 @@ def test_identity_tables(stubbed, monkeypatch):
     assert own.data_ptr() != kept.data_ptr() and own.tolist() == [[0, 1, 2], [3, 4, 5]]
     assert ops._identity_table(dev, 2, 2, 3).data_ptr() != own.data_ptr()
     assert list(ops._identity_tables) == [(None, 1)]
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=torch.int8), dict(page_bounds=True),
+                                dict(dtype=torch.float8_e4m3fn, block_scales=True),
+                                dict(dtype=torch.float8_e4m3fn, block_scales=True, page_bounds=True)])
+def test_write_to_kv_cache_refuses_what_it_would_leave_stale(stubbed, kw):
+    """A slot write knows nothing of a page's scales or bounds."""
+    from b200attn.backend import write_to_kv_cache
+
+    stubbed(SimpleNamespace(b200attn_kv_scatter_slots_ex=lambda *a: 0,
+                            b200attn_kv_scatter_slots=lambda *a: 0))
+    cache = sharding.allocate_kv_caches(1, 6, 2, 32, 64, **kw)["layers.0.attn"]
+    rows = torch.ones(3, 2 * 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="paged_write"):
+        write_to_kv_cache(rows, rows, cache, torch.arange(3))
+
+
+@pytest.mark.parametrize("extra", [[], [None, None], [None, None, None]])
+def test_write_to_kv_cache_takes_plain_caches(stubbed, extra, monkeypatch):
+    from b200attn import backend
+
+    calls = []
+    monkeypatch.setattr(backend.ops, "kv_scatter_slots", lambda *a: calls.append(a))
+    pair = sharding.allocate_kv_caches(1, 6, 2, 32, 64)["layers.0.attn"]
+    rows = torch.ones(3, 2 * 64, dtype=torch.bfloat16)
+    backend.write_to_kv_cache(rows, rows, list(pair) + extra, torch.arange(3))
+    backend.write_to_kv_cache(rows, rows, torch.stack(pair), torch.arange(3))
+    assert len(calls) == 2 and calls[0][0] is pair[0] and calls[0][2].shape == (3, 2, 64)

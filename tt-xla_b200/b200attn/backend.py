@@ -900,7 +900,10 @@ class B200Attention(torch.nn.Module):
 
 
 def write_to_kv_cache(key, value, kv_cache, slot_mapping, *unused, **unused_kw) -> None:
-    """Slot-mapping cache write (attention.py:671-716) on the live [k_cache, v_cache] layout."""
+    """Slot-mapping cache write (attention.py:671-716) on the live [k_cache, v_cache] layout.  A cache
+    that keeps scales or key bounds per page is refused: its rows alone would not be the write."""
+    if isinstance(kv_cache, (list, tuple)) and any(x is not None for x in kv_cache[2:5]):
+        raise ValueError("a cache with scales or key bounds is written by ops.paged_write")
     k_cache, v_cache = kv_cache[0], kv_cache[1]
     nkv, hd = k_cache.shape[1], k_cache.shape[3]
     ops.kv_scatter_slots(
