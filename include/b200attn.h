@@ -449,7 +449,13 @@ int b200attn_select_pages(int32_t* out_table, int32_t* out_pos, const void* q,
  * and the base-2 logarithm of the V factor.  b200attn_prefill_scaled is b200attn_prefill_ex
  * (kv_is_paged = 1) over that pool; it applies the factors in fp32, so the 8-bit values reach the
  * attention unrounded.  Rows that attend a page whose scale is NaN, negative or infinite, or whose
- * id is out of range (reported: diagnostics word 2), come out as NaN. */
+ * id is out of range (reported: diagnostics word 2), come out as NaN.
+ * A page table is as wide as the longest context a runner allows, which may be far more than the
+ * batch's: b200attn_dequant_pages_scaled_ex is for a host that knows how long its contexts are.  It
+ * passes the columns they need as page_table_width (the pool and the launch go by it, and so does
+ * b200attn_prefill_scaled over that pool) and max_context_len, the longest cu_q[s+1] - cu_q[s] +
+ * q_start[s] it reckons with: a longer one is reported (word 2), and what its rows attend behind
+ * that is unspecified.  0: nothing is checked. */
 int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, const void* k_cache,
                                   const void* v_cache, const float* k_scale, const float* v_scale,
                                   int cache_dtype, const int32_t* page_table,
@@ -457,6 +463,14 @@ int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, cons
                                   const int32_t* cu_q, const int32_t* q_start, int num_seqs,
                                   int num_kv_heads, int head_size, int block_size,
                                   int64_t num_blocks, void* stream);
+int b200attn_dequant_pages_scaled_ex(void* k_dst, void* v_dst, float* factors, const void* k_cache,
+                                     const void* v_cache, const float* k_scale,
+                                     const float* v_scale, int cache_dtype,
+                                     const int32_t* page_table, int64_t page_table_stride,
+                                     int page_table_width, const int32_t* cu_q,
+                                     const int32_t* q_start, int max_context_len, int num_seqs,
+                                     int num_kv_heads, int head_size, int block_size,
+                                     int64_t num_blocks, void* stream);
 int b200attn_prefill_scaled(void* out, int64_t out_row_stride, const void* q,
                             int64_t q_row_stride, const void* k_pool, const void* v_pool,
                             const float* factors, const int32_t* page_table,

@@ -200,8 +200,9 @@ class _RecordingLibrary:
             self.meet.wait(30)
         return 0
 
-    def b200attn_dequant_pages_scaled(self, k, v, factors, *rest):
-        width, seqs, nkv, hd, bs = rest[7], rest[10], rest[11], rest[12], rest[13]
+    def b200attn_dequant_pages_scaled_ex(self, k, v, factors, *rest):
+        width, limit, seqs, nkv, hd, bs = rest[7], *rest[10:15]
+        self.columns = (width, limit)
         pages = seqs * width
         half = pages * nkv * bs * hd * 2
         return self._note_widened([(k, half), (v, half), (factors, pages * nkv * 8)])
@@ -217,6 +218,7 @@ class _RecordingLibrary:
         return 0
 
     def b200attn_prefill_scaled(self, out, ostride, q, qstride, k, v, factors, *rest):
+        assert rest[2] == self.columns[0]
         self.attended[threading.get_ident()] = [k, v, factors]
         return 0
 
@@ -292,6 +294,45 @@ def test_unscaled_e4m3_prefills_do_not_come_between_each_other(stubbed, monkeypa
     assert len(lib.order) == 6
     for first, second in zip(lib.order[::2], lib.order[1::2]):
         assert first == ("widen", first[1]) and second == ("attend", first[1])
+
+
+@pytest.mark.parametrize("hint,columns", [(0, 2048), (1, 1), (32, 1), (33, 2), (100, 4),
+                                          (65536, 2048), (1 << 30, 2048)])
+def test_widening_goes_by_the_longest_context(stubbed, monkeypatch, hint, columns):
+    """Not by the width of the page table, where the caller says how long contexts are; a captured
+    call keeps all columns."""
+    lib = _RecordingLibrary()
+    ops = stubbed(lib)
+    sizes = []
+    empty = torch.empty
+    monkeypatch.setattr(ops.torch, "empty", lambda *a, **kw: sizes.append(a) or empty(*a, **kw))
+    _prefill_call(ops, torch.int8, width=2048, max_context_len=hint)
+    assert lib.columns == (columns, hint)
+    assert (2 * columns * 2 * 32 * 128 * 4 + 2 * columns * 2 * 8,) in sizes
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    _prefill_call(ops, torch.int8, width=2048, max_context_len=hint)
+    assert lib.columns == (2048, 0)
+
+
+def test_a_negative_longest_context_is_refused(stubbed):
+    with pytest.raises(ValueError, match="max_context_len"):
+        _prefill_call(stubbed(_RecordingLibrary()), torch.int8, max_context_len=-1)
+
+
+WIDEN = dict(kd=16, vd=16, f=16, k=16, v=16, ks=16, vs=16, kind=INT8, table=16, tstride=4, width=4,
+             cu=16, start=16, ctx=0, seqs=2, nkv=2, hd=128, bs=32, nb=8, stream=None)
+
+
+@pytest.mark.parametrize("changes,status", [
+    (dict(kd=None), NULL), (dict(f=None), NULL), (dict(ks=None), NULL), (dict(cu=None), NULL),
+    (dict(kind=BF16), BAD), (dict(width=0), BAD), (dict(seqs=-1), BAD), (dict(ctx=-1), BAD),
+    (dict(hd=96), UNSUPPORTED), (dict(vd=8), MISALIGNED), (dict(seqs=1 << 30), -8),
+])
+def test_dequant_pages_scaled_refusals(L, changes, status):
+    assert _call(L.b200attn_dequant_pages_scaled_ex, WIDEN, **changes) == status
+    if "ctx" not in changes:
+        old = {n: x for n, x in {**WIDEN, **changes}.items() if n != "ctx"}
+        assert L.b200attn_dequant_pages_scaled(*old.values()) == status
 
 
 def test_identity_tables(stubbed, monkeypatch):

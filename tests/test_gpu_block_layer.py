@@ -319,6 +319,36 @@ def test_a_run_is_the_same_bits_every_time(clean_error_word):
         assert torch.equal(_step(cache, table, x, pos, 60), first)
 
 
+def test_a_layer_widens_by_the_longest_sequence(clean_error_word, monkeypatch):
+    """A runner's block table is as wide as its longest allowed context."""
+    from b200attn import B200AttentionBackendImpl, ops
+    from b200attn.backend import build_varlen_metadata
+
+    impl = B200AttentionBackendImpl(NQ, HD, HD ** -0.5, NKV, None, None, "int8_block")
+    table = torch.zeros(2, 1024, dtype=torch.int32)
+    table[:, :4] = torch.randperm(8, generator=torch.Generator().manual_seed(1)).view(2, 4).int()
+    cu, seq = torch.tensor([0, 50, 150]).int(), torch.tensor([50, 100]).int()
+    slots = torch.zeros(150, dtype=torch.int64)             # positions come from the block table
+    x = _qkv(150, 3).cuda()
+    outs, columns = [], []
+    widen = ops._widen_scaled_pages
+
+    def note(*a, **kw):
+        got = widen(*a, **kw)
+        columns.append(got[4].shape[1])
+        return got
+
+    monkeypatch.setattr(ops, "_widen_scaled_pages", note)
+    for longest in (100, 0):
+        cache = _caches("int8_block", 8, False)
+        md = build_varlen_metadata(cu.cuda(), cu, seq.cuda(), table.cuda(), slots.cuda(),
+                                   max_seq_len=longest)
+        out = torch.empty(150, NQ * HD, dtype=torch.bfloat16, device="cuda")
+        impl.forward(None, *[t.contiguous() for t in _split(x)], cache, md, output=out)
+        outs.append(out)
+    assert columns == [4, 1024] and torch.equal(*outs)
+
+
 def test_layer_refusals():
     from b200attn import B200AttentionBackendImpl, B200Attention, sharding
 

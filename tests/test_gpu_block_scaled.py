@@ -522,6 +522,54 @@ def test_prefill_bad_page_is_reported_and_comes_out_as_nan(bad):
         assert got[n + 2 * bs:].isnan().all()
 
 
+def test_prefill_through_a_table_much_wider_than_its_contexts(clean_error_word):
+    """The columns of the longest context count, for the result and for the memory."""
+    from b200attn import ops
+
+    lens, starts = [33, 1, 130], [0, 64, 15]
+    c = _decode_case(3, 8, 2, 128, 64, [a + b for a, b in zip(lens, starts)], torch.int8, seed=5)
+    cu = torch.tensor([0] + lens).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), 8, 128, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    wide = torch.full((3, 2048), 10 ** 8, dtype=torch.int32)
+    wide[:, : c["table"].shape[1]] = c["table"]
+    d = {n: t.cuda() for n, t in c.items()}
+
+    def run(table, **kw):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = ops.prefill(q, d["k_cache"], d["v_cache"], cu, page_table=table,
+                          q_start=torch.tensor(starts, dtype=torch.int32).cuda(),
+                          k_scale=d["k_scale"], v_scale=d["v_scale"], **kw)
+        torch.cuda.synchronize()
+        return out, torch.cuda.max_memory_allocated() - before
+
+    want, _ = run(d["table"])
+    for hint in (145, 192, 1000, 0):
+        got, used = run(wide.cuda(), max_context_len=hint)
+        assert torch.equal(got, want)
+        if hint:         # bf16 K and V of 2 heads of 128, and room for the rest
+            assert used < 3 * (hint // 64 + 1) * 2 * 64 * 128 * 4 + (4 << 20)
+
+
+@pytest.mark.parametrize("hint", [1, 64, 144])
+def test_prefill_of_a_context_longer_than_promised_is_reported(hint):
+    from b200attn import ops
+
+    c = {n: t.cuda() for n, t in _decode_case(2, 8, 2, 64, 32, [40, 145], torch.int8, seed=5).items()}
+    cu = torch.tensor([0, 40, 75], dtype=torch.int32)
+    q = torch.zeros(75, 8, 64, dtype=torch.bfloat16, device="cuda")
+
+    def run(n):
+        ops.prefill(q, c["k_cache"], c["v_cache"], cu, page_table=c["table"], max_context_len=n,
+                    q_start=torch.tensor([0, 110], dtype=torch.int32).cuda(), k_scale=c["k_scale"],
+                    v_scale=c["v_scale"])
+        return ops.read_error_word()
+
+    ops.read_error_word()
+    assert run(145) == 0 and run(hint) == 2 and run(0) == 0
+
+
 # ----------------------------------------------------------------------------------- refusals
 def test_refusals():
     from b200attn import ops

@@ -111,6 +111,11 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
          c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_void_p],
     ),
+    "b200attn_dequant_pages_scaled_ex": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+         c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p],
+    ),
     "b200attn_prefill_scaled": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,

@@ -76,7 +76,7 @@ class B200Metadata:
     seq_lens: Optional[torch.Tensor] = None         # [seqs] i32, device
     block_table: Optional[torch.Tensor] = None      # [seqs, nblk] i32
     num_decodes: int = 0                            # leading rows with one query token
-    max_seq_len: int = 0
+    max_seq_len: int = 0                            # no sequence is longer; 0: unknown
     # derived once per step by the builder (shared by all layers)
     decode_cur_pos: Optional[torch.Tensor] = None
     prefill_cu_q: Optional[torch.Tensor] = None
@@ -768,7 +768,7 @@ class B200AttentionBackendImpl:
                 q[nd:], kv_pair[0], kv_pair[1], md.prefill_cu_q_cpu, scale=self.scale,
                 page_table=md.block_table[nd:], q_start=md.prefill_q_start, out=out[nd:],
                 cu_q=md.prefill_cu_q, sliding_window=self._window,
-                **({} if pages is None else pages.scales),
+                **({} if pages is None else pages.scales), max_context_len=md.max_seq_len,
             )
 
 

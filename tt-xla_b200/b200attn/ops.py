@@ -852,6 +852,7 @@ def prefill(
     sliding_window: int = 0,
     k_scale: Optional[torch.Tensor] = None,
     v_scale: Optional[torch.Tensor] = None,
+    max_context_len: int = 0,
 ) -> torch.Tensor:
     """Causal varlen prefill (`tt.scaled_dot_product_attention`, custom_ops.py:635-742) when
     `page_table` is None and `k_src`/`v_src` are the fresh [tokens, nkv, hd] K/V of the same
@@ -860,7 +861,10 @@ def prefill(
     given and `k_src`/`v_src` are the caches.  `query`: [tokens, nq, hd] with sequence s owning
     rows cu_q[s]:cu_q[s+1]; `q_start[s]` is the absolute position of its first row.
     `k_scale` / `v_scale`: paged int8 or e4m3 caches with a scale per page and KV head
-    (`paged_write`)."""
+    (`paged_write`).  For these the pages that the batch reads are widened into memory of the call,
+    as many columns of the page table as `max_context_len` takes (0: all of them).  It must not be
+    less than any sequence's q_start + rows: a longer context is reported (diagnostics word 2).
+    Under stream capture all columns are taken, since a replay may have longer contexts."""
     _need_cuda(query, k_src, v_src, page_table, q_start, out, cu_q)
     if cu_q_host.is_cuda or cu_q_host.dtype != torch.int32 or not cu_q_host.is_contiguous():
         raise ValueError("cu_q_host must be a dense int32 CPU tensor")
@@ -878,7 +882,7 @@ def prefill(
         if _current_device() != index:       # the library works on the current device
             with torch.cuda.device(index):
                 return prefill(query, k_src, v_src, cu_q_host, scale, page_table, q_start, out,
-                               cu_q, sliding_window, k_scale, v_scale)
+                               cu_q, sliding_window, k_scale, v_scale, max_context_len)
     if paged:
         scaled = _check_scales(k_scale, v_scale, k_src)
         nb, nkv, bs, _hd = _check_cache(k_src, v_src, scaled)
@@ -925,7 +929,7 @@ def prefill(
         scale = hd ** -0.5
     if scaled:
         pool, k_ptr, v_ptr, factors, page_table, nb = _widen_scaled_pages(
-            k_src, v_src, k_scale, v_scale, page_table, cu_q, q_start, num_seqs)
+            k_src, v_src, k_scale, v_scale, page_table, cu_q, q_start, num_seqs, max_context_len)
         status = _lib.lib().b200attn_prefill_scaled(
             out_t.data_ptr(), ostride, q.data_ptr(),
             qstride if total_q > 1 else max(qstride, nq * hd), k_ptr, v_ptr, factors,
@@ -1021,7 +1025,8 @@ def _identity_table(device: torch.device, stream: int, seqs: int, width: int) ->
     return have[:pages].view(seqs, width)
 
 
-def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_start, num_seqs):
+def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_start, num_seqs,
+                        max_context_len=0):
     """bf16 pages, laid out as _widen_fp8_pages does, of a block-scaled cache pair on the current
     device, and what is left of their scales; returns (the memory that holds them, the addresses
     of the K pages, of the V pages and of the factors in it, identity page table, pages).  The
@@ -1029,6 +1034,12 @@ def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_
     stream too, has its own.  torch's allocator hands it out again in stream order only."""
     nb, nkv, bs, hd = k_cache.shape
     width = page_table.shape[1]
+    if max_context_len < 0:
+        raise ValueError("max_context_len must not be negative")
+    if max_context_len > 0 and torch.cuda.is_current_stream_capturing():
+        max_context_len = 0
+    if max_context_len > 0:
+        width = min(width, (max_context_len + bs - 1) // bs)
     pages = max(num_seqs * width, 1)
     dev = k_cache.device
     stream = _raw_stream(dev.index)
@@ -1037,12 +1048,12 @@ def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_
     k_pool = pool.data_ptr()
     v_pool, factors = k_pool + half, k_pool + 2 * half
     _lib.check(
-        "b200attn_dequant_pages_scaled",
-        _lib.lib().b200attn_dequant_pages_scaled(
+        "b200attn_dequant_pages_scaled_ex",
+        _lib.lib().b200attn_dequant_pages_scaled_ex(
             k_pool, v_pool, factors, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), _cache_dtype(k_cache), page_table.data_ptr(), page_table.stride(0),
-            width, cu_q.data_ptr(), q_start.data_ptr() if q_start is not None else 0, num_seqs,
-            nkv, hd, bs, nb, stream))
+            width, cu_q.data_ptr(), q_start.data_ptr() if q_start is not None else 0,
+            max_context_len, num_seqs, nkv, hd, bs, nb, stream))
     table = _identity_table(dev, stream, num_seqs, width)
     return pool, k_pool, v_pool, factors, table, pages
 

@@ -1141,10 +1141,25 @@ int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, cons
                                   const int32_t* cu_q, const int32_t* q_start, int num_seqs,
                                   int num_kv_heads, int head_size, int block_size,
                                   int64_t num_blocks, void* stream) {
+  return b200attn_dequant_pages_scaled_ex(k_dst, v_dst, factors, k_cache, v_cache, k_scale, v_scale,
+                                          cache_dtype, page_table, page_table_stride,
+                                          page_table_width, cu_q, q_start, 0, num_seqs,
+                                          num_kv_heads, head_size, block_size, num_blocks, stream);
+}
+
+int b200attn_dequant_pages_scaled_ex(void* k_dst, void* v_dst, float* factors, const void* k_cache,
+                                     const void* v_cache, const float* k_scale,
+                                     const float* v_scale, int cache_dtype,
+                                     const int32_t* page_table, int64_t page_table_stride,
+                                     int page_table_width, const int32_t* cu_q,
+                                     const int32_t* q_start, int max_context_len, int num_seqs,
+                                     int num_kv_heads, int head_size, int block_size,
+                                     int64_t num_blocks, void* stream) {
   if (!k_dst || !v_dst || !factors || !k_cache || !v_cache || !k_scale || !v_scale ||
       !page_table || !cu_q)
     return B200ATTN_ERR_NULL_POINTER;
-  if (num_seqs < 0 || page_table_width <= 0) return B200ATTN_ERR_BAD_ARGUMENT;
+  if (num_seqs < 0 || page_table_width <= 0 || max_context_len < 0)
+    return B200ATTN_ERR_BAD_ARGUMENT;
   if (cache_dtype != B200ATTN_CACHE_FP8_E4M3 && cache_dtype != B200ATTN_CACHE_INT8)
     return B200ATTN_ERR_BAD_ARGUMENT;
   if (int rc = check_cache_geometry(num_kv_heads, head_size, block_size, num_blocks)) return rc;
@@ -1170,6 +1185,7 @@ int b200attn_dequant_pages_scaled(void* k_dst, void* v_dst, float* factors, cons
   p.page_table_width = page_table_width;
   p.cu_q = cu_q;
   p.q_start = q_start;
+  p.max_context_len = max_context_len;
   p.num_kv_heads = num_kv_heads;
   p.num_blocks = num_blocks;
   p.err_word = dev->err_word;

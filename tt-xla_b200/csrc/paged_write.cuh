@@ -394,6 +394,7 @@ struct DequantScaledParams {
   int page_table_width;
   const int32_t* cu_q;
   const int32_t* q_start;
+  int max_context_len;        // > 0: a longer context is reported
   int num_kv_heads;
   int64_t num_blocks;
   int* err_word;
@@ -423,6 +424,9 @@ __global__ void __launch_bounds__(128) dequant_scaled_kernel(const DequantScaled
   const int seq = blockIdx.y, z = blockIdx.z;
   const int len = p.cu_q[seq + 1] - p.cu_q[seq];
   const int64_t ctx = static_cast<int64_t>(p.q_start ? p.q_start[seq] : 0) + len;
+  if (blockIdx.x == 0 && z == 0 && threadIdx.x == 0 && p.max_context_len > 0 && len > 0 &&
+      ctx > p.max_context_len)
+    atomicExch(p.err_word, kDevBadIndex);
   if (len <= 0 || slot >= (ctx + BS - 1) / BS) return;
   const int64_t blk = p.page_table[static_cast<int64_t>(seq) * p.page_table_stride + slot];
   const int64_t dst_page =
