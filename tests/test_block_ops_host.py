@@ -378,3 +378,32 @@ def test_write_to_kv_cache_takes_plain_caches(stubbed, extra, monkeypatch):
     backend.write_to_kv_cache(rows, rows, list(pair) + extra, torch.arange(3))
     backend.write_to_kv_cache(rows, rows, torch.stack(pair), torch.arange(3))
     assert len(calls) == 2 and calls[0][0] is pair[0] and calls[0][2].shape == (3, 2, 64)
+
+
+class _NormCalls(list):
+    """Takes the place of ops.qk_norm_rope_kv_scatter_slots: keeps the weights of every call."""
+
+    def __call__(self, q, k, v, positions, inv_freq, rotary, hd, wq, wk, *rest, **kw):
+        self.append((wq, wk, wq.clone(), wk.clone()))
+        return q, k
+
+
+def _norm_layer(monkeypatch, wq, wk):
+    from b200attn import B200Attention, backend
+
+    calls = _NormCalls()
+    monkeypatch.setattr(backend.ops, "qk_norm_rope_kv_scatter_slots", calls)
+    layer = B200Attention(4, 64, 0.125, 2, rotary_dim=64, q_norm_weight=wq, k_norm_weight=wk)
+    monkeypatch.setattr(layer.impl, "forward", lambda *a, output, **kw: output.zero_())
+    q = torch.zeros(3, 4 * 64, dtype=torch.bfloat16)
+    kv = torch.zeros(3, 2, 2 * 64, dtype=torch.bfloat16)
+    return calls, lambda pos=torch.arange(3): layer(q, kv[:, 0], kv[:, 1], positions=pos)
+
+
+def test_a_layer_with_head_norms_refuses_a_call_without_positions(monkeypatch):
+    calls, forward = _norm_layer(monkeypatch, torch.ones(64), torch.ones(64))
+    with pytest.raises(ValueError, match="positions"):
+        forward(None)
+    assert not calls
+    forward()
+    assert len(calls) == 1

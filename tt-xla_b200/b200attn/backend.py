@@ -885,6 +885,9 @@ class B200Attention(torch.nn.Module):
         out = torch.empty(output_shape if output_shape is not None else q2.shape,
                           dtype=q2.dtype, device=q2.device)
         md = attn_metadata if attn_metadata is not None else self.attn_metadata
+        if positions is None and self.norm_weights is not None:
+            raise ValueError("a layer built with head norms needs positions: norms and rotation are "
+                             "one launch")
         if positions is not None:
             if self.inv_freq is None:
                 raise ValueError("positions given to a layer built without rotary_dim")
