@@ -407,3 +407,39 @@ def test_a_layer_with_head_norms_refuses_a_call_without_positions(monkeypatch):
     assert not calls
     forward()
     assert len(calls) == 1
+
+
+@pytest.mark.parametrize("make", [lambda: torch.ones(64), lambda: torch.nn.Parameter(torch.ones(64)),
+                                  lambda: torch.ones(128)[::2]])
+def test_a_layer_sees_head_norm_weights_that_change(monkeypatch, make):
+    """Loaded after the layer was made, or again later; a copy, where one is needed, keeps its
+    address."""
+    wq, wk = make(), make()
+    calls, forward = _norm_layer(monkeypatch, wq, wk)
+    with torch.inference_mode():
+        forward()
+    with torch.no_grad():
+        wq.copy_(torch.arange(64.0))
+    forward()
+    with torch.no_grad():
+        wk.mul_(3.0)
+    forward()
+    want_q = [torch.ones(64), torch.arange(64.0), torch.arange(64.0)]
+    want_k = [torch.ones(64), torch.ones(64), torch.full((64,), 3.0)]
+    for call, q, k in zip(calls, want_q, want_k):
+        assert torch.equal(call[2], q) and torch.equal(call[3], k)
+        assert call[0].is_contiguous() and call[1].is_contiguous()
+    assert len({c[0].data_ptr() for c in calls}) == 1 and len({c[1].data_ptr() for c in calls}) == 1
+    if isinstance(wq, torch.nn.Parameter):               # a module that is moved swaps the data
+        wq.data = torch.full((64,), 5.0)
+        forward()
+        assert torch.equal(calls[-1][2], torch.full((64,), 5.0))
+
+
+def test_a_layer_takes_head_norm_weights_made_in_inference_mode(monkeypatch):
+    with torch.inference_mode():
+        w = torch.ones(128)[::2]
+    calls, forward = _norm_layer(monkeypatch, w, w)
+    forward()
+    forward()
+    assert len(calls) == 2 and torch.equal(calls[1][2], torch.ones(64))

@@ -410,3 +410,26 @@ def test_prefills_of_two_threads_on_one_stream(clean_error_word):
     torch.cuda.synchronize()
     for mine, (_, _, want) in zip(outs, cases):
         assert len(mine) == 200 and all(torch.equal(o, want) for o in mine)
+
+
+def test_head_norm_weights_on_another_device_are_followed(clean_error_word):
+    """Weights on the host, changed in place between two forwards."""
+    from b200attn import B200Attention, B200Metadata
+
+    w = [torch.ones(HD).bfloat16(), torch.ones(HD).bfloat16()]
+    layer = B200Attention(NQ, HD, HD ** -0.5, NKV, rotary_dim=HD, q_norm_weight=w[0],
+                          k_norm_weight=w[1])
+    layer.kv_cache = _caches("auto", 2, False)
+    md = B200Metadata(cache_position=torch.zeros(1).int().cuda(), num_users=1,
+                      page_table=torch.ones(1, 1).int().cuda(), batch_idx=torch.zeros(1).int().cuda())
+    for by in (1.0, 2.0, 0.5):
+        w[0].mul_(by)
+        w[1].mul_(by)
+        x = _qkv(1, 3).cuda()
+        q, k, v = [t.contiguous() for t in _split(x)]
+        before = q.clone()
+        layer(q, k, v, attn_metadata=md, positions=torch.zeros(1).long().cuda())
+        rows = before.float().view(NQ, HD)
+        want = rows * torch.rsqrt(rows.square().mean(-1, keepdim=True) + 1e-6) * w[0].cuda().float()
+        err = (q.float().view(NQ, HD) - want).abs()
+        assert (err <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * want.abs().amax()).all()

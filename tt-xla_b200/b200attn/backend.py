@@ -824,8 +824,9 @@ class B200Attention(torch.nn.Module):
             raise ValueError("the head norms come with the rotation: rotary_dim is needed")
         if not is_neox_style and q_norm_weight is None:
             raise NotImplementedError("interleaved pairs are supported with the head norms only")
-        self.norm_weights = None if q_norm_weight is None else \
-            [w.detach().contiguous() for w in (q_norm_weight, k_norm_weight)]
+        # The caller's own tensors: whoever owns them loads and moves them.
+        self.norm_weights = None if q_norm_weight is None else [q_norm_weight, k_norm_weight]
+        self._norm_copies = [None, None]     # ((data_ptr, version), dense copy on the device)
         self.norm_eps, self.is_neox_style = norm_eps, is_neox_style
         self.num_heads = num_heads
         self.head_size = self.head_size_v = head_size
@@ -846,6 +847,28 @@ class B200Attention(torch.nn.Module):
     def set_metadata(self, attn_metadata: B200Metadata) -> None:
         self.attn_metadata = attn_metadata
 
+    def _norm_weights_for(self, device) -> list:
+        """The head-norm weights on `device`, dense: the caller's tensors where they are that, else
+        copies.  A weight that changes (tensors made in inference mode do not tell) is copied into
+        the same memory again, which captured graphs go on reading."""
+        weights = []
+        for i, w in enumerate(self.norm_weights):
+            if w.device != device or not w.is_contiguous():
+                key = (w.data_ptr(), 0 if w.is_inference() else w._version)
+                have = self._norm_copies[i]
+                if have is None or have[0] != key or have[1].device != device:
+                    # an ordinary tensor wherever the call comes from: it is written again later
+                    with torch.inference_mode(False), torch.no_grad():
+                        copy = None if have is None else have[1]
+                        if copy is None or copy.device != device or copy.shape != w.shape \
+                                or copy.dtype != w.dtype:
+                            copy = torch.empty(w.shape, dtype=w.dtype, device=device)
+                        copy.copy_(w)
+                    self._norm_copies[i] = have = (key, copy)
+                w = have[1]
+            weights.append(w)
+        return weights
+
     def _rotate_and_write(self, q2, k2, v2, positions, md) -> None:
         """q2 / k2 rotated in place; with a slot mapping in the metadata and a cache of its own
         the same launch writes k and v, and the Impl is told so."""
@@ -859,11 +882,10 @@ class B200Attention(torch.nn.Module):
                        and kv_pair[0].dtype == torch.bfloat16
                        and self.impl._page_values(self.kv_cache, kv_pair) is None)
         if self.norm_weights is not None:
-            if self.norm_weights[0].device != q2.device:
-                self.norm_weights = [w.to(q2.device) for w in self.norm_weights]
             ops.qk_norm_rope_kv_scatter_slots(
                 q2, k2, v2 if fused_write else None, positions.reshape(-1).to(torch.int64),
-                self.inv_freq, self.rotary_dim, self.head_size, *self.norm_weights, self.norm_eps,
+                self.inv_freq, self.rotary_dim, self.head_size,
+                *self._norm_weights_for(q2.device), self.norm_eps,
                 kv_pair[0] if fused_write else None, kv_pair[1] if fused_write else None,
                 slots[: q2.shape[0]] if fused_write else None, is_neox_style=self.is_neox_style)
             self.impl.kv_written_upstream = fused_write
