@@ -443,3 +443,24 @@ def test_a_layer_takes_head_norm_weights_made_in_inference_mode(monkeypatch):
     forward()
     forward()
     assert len(calls) == 2 and torch.equal(calls[1][2], torch.ones(64))
+
+
+@pytest.mark.parametrize("which", ["key", "query", "part"])
+def test_a_layer_with_head_norms_refuses_a_value_that_is_rotated_away(monkeypatch, which):
+    """Also where the cache write comes later (block-scaled caches): the value would be read after
+    the key was normed and rotated in place."""
+    from b200attn import B200Attention, backend
+
+    calls = _NormCalls()
+    monkeypatch.setattr(backend.ops, "qk_norm_rope_kv_scatter_slots", calls)
+    w = torch.ones(64)
+    layer = B200Attention(4, 64, 0.125, 2, rotary_dim=64, q_norm_weight=w, k_norm_weight=w)
+    monkeypatch.setattr(layer.impl, "forward", lambda *a, output, **kw: output.zero_())
+    rows = torch.zeros(3, 8 * 64, dtype=torch.bfloat16)
+    q, k, v = rows.split([256, 128, 128], 1)
+    bad = {"key": k, "query": q[:, :128], "part": rows[:, 320:448]}[which]
+    with pytest.raises(ValueError, match="shares memory"):
+        layer(q, k, bad, positions=torch.arange(3))
+    assert not calls
+    layer(q, k, v, positions=torch.arange(3))
+    assert len(calls) == 1

@@ -882,6 +882,10 @@ class B200Attention(torch.nn.Module):
                        and kv_pair[0].dtype == torch.bfloat16
                        and self.impl._page_values(self.kv_cache, kv_pair) is None)
         if self.norm_weights is not None:
+            if v2 is not None and self.impl.kv_sharing_target_layer_name is None \
+                    and (ops.rows_overlap(v2, k2) or ops.rows_overlap(v2, q2)):
+                raise ValueError("value shares memory with query or key, which are normed and rotated "
+                                 "in place: hand over a copy")
             ops.qk_norm_rope_kv_scatter_slots(
                 q2, k2, v2 if fused_write else None, positions.reshape(-1).to(torch.int64),
                 self.inv_freq, self.rotary_dim, self.head_size,

@@ -309,6 +309,14 @@ def _rows_meet(a: tuple, b: tuple, tokens: int) -> bool:
     return True
 
 
+def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the dense rows of two 2-D tensors with as many rows share memory (as exact as
+    _rows_meet)."""
+    spans = [(t.data_ptr(), t.stride(0) * t.element_size(), t.shape[1] * t.element_size())
+             for t in (a, b)]
+    return a.shape[0] > 0 and _rows_meet(*spans, a.shape[0])
+
+
 def _check_outputs(tokens: int, oq: tuple, ok: tuple, q: tuple, k: tuple, v: tuple) -> None:
     """Each output is its input or shares no memory with it, and shares none with the other input,
     with v (read when its pointer is not 0) and with the other output: the kernel stores a token's
