@@ -1,5 +1,6 @@
 """Refusals of the block-scaled / page-list / norm entry points, and the shapes that
 allocate_kv_caches makes for them: no GPU needed, nothing is launched."""
+import functools
 import threading
 import time
 from types import SimpleNamespace
@@ -464,3 +465,23 @@ def test_a_layer_with_head_norms_refuses_a_value_that_is_rotated_away(monkeypatc
     assert not calls
     layer(q, k, v, positions=torch.arange(3))
     assert len(calls) == 1
+
+
+def test_split_counts_of_page_lists_are_kept_per_device(stubbed, monkeypatch):
+    """They go by the SM count of the device that is current."""
+    at, splits = [0], []
+    library = SimpleNamespace(
+        b200attn_decode_auto_splits=lambda *a: 1 + at[0],
+        b200attn_decode_workspace_bytes=lambda *a: 0,
+        b200attn_paged_decode_blocks=lambda *a: splits.append(a[24]) or 0)
+    ops = stubbed(library)
+    monkeypatch.setattr(ops, "_device_of", lambda *t: at[0])
+    monkeypatch.setattr(ops, "_current_device", lambda: at[0])
+    for kept in (ops._list_splits, ops._decode_bytes):
+        monkeypatch.setattr(ops, kept.__name__, functools.lru_cache(kept.__wrapped__))
+    cache = torch.zeros(4, 2, 32, 64, dtype=torch.bfloat16)
+    for device in (0, 3, 0):
+        at[0] = device
+        ops.paged_decode(torch.zeros(1, 2, 64, dtype=torch.bfloat16), cache, cache,
+                         torch.zeros(1, 2, 3, dtype=torch.int32), torch.zeros(1, 2, dtype=torch.int32))
+    assert splits == [1, 4, 1]

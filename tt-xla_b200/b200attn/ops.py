@@ -571,14 +571,15 @@ def _scratch(index: int, stream: int, nbytes: int) -> Optional[torch.Tensor]:
     return have[1]
 
 
-# Sizes and split counts are pure functions of whole numbers that the library computes.
+# Sizes and split counts are functions of whole numbers, and where the SM count is among them of the
+# device (which is the current one when they are asked for).
 @functools.lru_cache(maxsize=4096)
 def _select_bytes(users: int, nkv: int, width: int) -> int:
     return _lib.lib().b200attn_select_pages_workspace_bytes(users, nkv, width)
 
 
 @functools.lru_cache(maxsize=4096)
-def _list_splits(users: int, nkv: int, hd: int, ctx: int) -> int:
+def _list_splits(device: int, users: int, nkv: int, hd: int, ctx: int) -> int:
     return _lib.lib().b200attn_decode_auto_splits(users, nkv, hd, ctx)
 
 
@@ -719,8 +720,8 @@ def _decode_blocks(query, k_cache, v_cache, page_table, cur_pos, scale, out, num
             ws = _scratch(index, stream, _scaled_bytes(index, users, nq, nkv, hd, num_splits))
     else:
         if num_splits == 0:
-            num_splits = _list_splits(users, nkv, hd, max_context_len if max_context_len > 0
-                                      else width * bs)
+            num_splits = _list_splits(index, users, nkv, hd,
+                                      max_context_len if max_context_len > 0 else width * bs)
         if ws is None and num_splits > 1:
             ws = _scratch(index, stream, _decode_bytes(users, nq, hd, num_splits))
     status = _lib.lib().b200attn_paged_decode_blocks(
