@@ -305,8 +305,9 @@ def test_widening_goes_by_the_longest_context(stubbed, monkeypatch, hint, column
     lib = _RecordingLibrary()
     ops = stubbed(lib)
     sizes = []
-    empty = torch.empty
-    monkeypatch.setattr(ops.torch, "empty", lambda *a, **kw: sizes.append(a) or empty(*a, **kw))
+    new_empty = torch.Tensor.new_empty
+    monkeypatch.setattr(torch.Tensor, "new_empty",
+                        lambda t, *a, **kw: sizes.append(a) or new_empty(t, *a, **kw))
     _prefill_call(ops, torch.int8, width=2048, max_context_len=hint)
     assert lib.columns == (columns, hint)
     assert (2 * columns * 2 * 32 * 128 * 4 + 2 * columns * 2 * 8,) in sizes
@@ -336,21 +337,21 @@ def test_dequant_pages_scaled_refusals(L, changes, status):
         assert L.b200attn_dequant_pages_scaled(*old.values()) == status
 
 
-def test_identity_tables(stubbed, monkeypatch):
-    """One per stream, whatever shapes ask for it; a capture makes its own."""
-    ops = stubbed(_RecordingLibrary())
+def test_identity_tables(monkeypatch):
+    """One per stream, whatever sizes ask for it; a capture makes its own."""
+    from b200attn import ops
+
     monkeypatch.setattr(ops, "_identity_tables", {})
     dev = torch.device("cpu")
-    for seqs, width in ((1, 1), (3, 5), (7, 3), (5, 2000), (2, 9)):
-        want = torch.arange(seqs * width, dtype=torch.int32).view(seqs, width)
-        assert torch.equal(ops._identity_table(dev, 1, seqs, width), want)
-    assert len(ops._identity_tables) == 1
-    kept = ops._identity_tables[(None, 1)]
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-    own = ops._identity_table(dev, 1, 2, 3)
-    assert own.data_ptr() != kept.data_ptr() and own.tolist() == [[0, 1, 2], [3, 4, 5]]
-    assert ops._identity_table(dev, 2, 2, 3).data_ptr() != own.data_ptr()
-    assert list(ops._identity_tables) == [(None, 1)]
+    for pages in (1, 15, 4096, 4097, 10000, 18):
+        got = ops._identity_table(dev, 1, pages, False)
+        assert got.dtype == torch.int32 and got.numel() >= pages
+        assert torch.equal(got, torch.arange(got.numel(), dtype=torch.int32))
+    assert list(ops._identity_tables) == [(None, 1)] and ops._identity_tables[(None, 1)] is got
+    own = ops._identity_table(dev, 1, 6, True)
+    assert own is not got and own.tolist() == list(range(6))
+    assert ops._identity_table(dev, 2, 6, False) is not got
+    assert list(ops._identity_tables) == [(None, 1), (None, 2)]
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=torch.int8), dict(page_bounds=True),
@@ -485,3 +486,14 @@ def test_split_counts_of_page_lists_are_kept_per_device(stubbed, monkeypatch):
         ops.paged_decode(torch.zeros(1, 2, 64, dtype=torch.bfloat16), cache, cache,
                          torch.zeros(1, 2, 3, dtype=torch.int32), torch.zeros(1, 2, dtype=torch.int32))
     assert splits == [1, 4, 1]
+
+
+def test_prefill_over_a_scaled_cache_refuses_cpu_tensors():
+    from b200attn import ops
+
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        _prefill_call(ops, torch.int8)
+    with pytest.raises(ValueError, match="paged cache"):
+        x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+        ops.prefill(x, x, x, torch.tensor([0, 2], dtype=torch.int32), k_scale=torch.ones(1, 2),
+                    v_scale=torch.ones(1, 2))

@@ -335,7 +335,7 @@ def test_a_layer_widens_by_the_longest_sequence(clean_error_word, monkeypatch):
 
     def note(*a, **kw):
         got = widen(*a, **kw)
-        columns.append(got[4].shape[1])
+        columns.append(got[5])
         return got
 
     monkeypatch.setattr(ops, "_widen_scaled_pages", note)

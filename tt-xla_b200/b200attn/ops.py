@@ -874,7 +874,8 @@ def prefill(
     as many columns of the page table as `max_context_len` takes (0: all of them).  It must not be
     less than any sequence's q_start + rows: a longer context is reported (diagnostics word 2).
     Under stream capture all columns are taken, since a replay may have longer contexts."""
-    _need_cuda(query, k_src, v_src, page_table, q_start, out, cu_q)
+    if k_scale is None:                      # else _device_of looks at all of them below
+        _need_cuda(query, k_src, v_src, page_table, q_start, out, cu_q)
     if cu_q_host.is_cuda or cu_q_host.dtype != torch.int32 or not cu_q_host.is_contiguous():
         raise ValueError("cu_q_host must be a dense int32 CPU tensor")
     num_seqs = cu_q_host.numel() - 1
@@ -937,14 +938,14 @@ def prefill(
     if scale is None:
         scale = hd ** -0.5
     if scaled:
-        pool, k_ptr, v_ptr, factors, page_table, nb = _widen_scaled_pages(
+        pool, k_ptr, v_ptr, factors, table, width, nb = _widen_scaled_pages(
             k_src, v_src, k_scale, v_scale, page_table, cu_q, q_start, num_seqs, max_context_len)
         status = _lib.lib().b200attn_prefill_scaled(
             out_t.data_ptr(), ostride, q.data_ptr(),
             qstride if total_q > 1 else max(qstride, nq * hd), k_ptr, v_ptr, factors,
-            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_q.data_ptr(),
-            cu_q_host.data_ptr(), q_start.data_ptr() if q_start is not None else 0, num_seqs,
-            total_q, nq, nkv, hd, bs, nb, scale, sliding_window, _raw_stream(index))
+            table.data_ptr(), width, width, cu_q.data_ptr(), cu_q_host.data_ptr(),
+            q_start.data_ptr() if q_start is not None else 0, num_seqs, total_q, nq, nkv, hd, bs, nb,
+            scale, sliding_window, _raw_stream(index))
         if status:
             _lib.check("b200attn_prefill_scaled", status)
         return out if out is not None else out_t
@@ -1018,34 +1019,32 @@ def _widen_fp8_pages(k_cache, v_cache, page_table, cu_q, q_start, num_seqs):
 _identity_tables: dict[tuple, torch.Tensor] = {}
 
 
-def _identity_table(device: torch.device, stream: int, seqs: int, width: int) -> torch.Tensor:
-    """[seqs, width] int32 table of the pages 0, 1, 2, ... on the current device: a view of one table
-    per stream that grows on demand; under stream capture one of the graph's own."""
-    pages = seqs * width
-    have = None
-    capturing = torch.cuda.is_current_stream_capturing()
-    if not capturing:
-        have = _identity_tables.get((device.index, stream))
+def _identity_table(device: torch.device, stream: int, pages: int, capturing: bool) -> torch.Tensor:
+    """int32 0, 1, 2, ... for `pages` or more pages on the current device: one tensor per stream that
+    grows on demand; under stream capture one of the graph's own."""
+    if capturing:
+        return torch.arange(pages, dtype=torch.int32, device=device)
+    have = _identity_tables.get((device.index, stream))
     if have is None or have.numel() < pages:
-        size = pages if capturing else max(4096, 1 << (pages - 1).bit_length())
-        have = torch.arange(size, dtype=torch.int32, device=device)
-        if not capturing:
-            _identity_tables[(device.index, stream)] = have
-    return have[:pages].view(seqs, width)
+        have = torch.arange(max(4096, 1 << (pages - 1).bit_length()), dtype=torch.int32, device=device)
+        _identity_tables[(device.index, stream)] = have
+    return have
 
 
 def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_start, num_seqs,
                         max_context_len=0):
     """bf16 pages, laid out as _widen_fp8_pages does, of a block-scaled cache pair on the current
     device, and what is left of their scales; returns (the memory that holds them, the addresses
-    of the K pages, of the V pages and of the factors in it, identity page table, pages).  The
-    memory belongs to the call: what another thread enqueues between the two launches, on this
-    stream too, has its own.  torch's allocator hands it out again in stream order only."""
+    of the K pages, of the V pages and of the factors in it, the identity page table's memory and
+    its columns, pages).  The memory belongs to the call: what another thread enqueues between the
+    two launches, on this stream too, has its own.  torch's allocator hands it out again in stream
+    order only."""
     nb, nkv, bs, hd = k_cache.shape
     width = page_table.shape[1]
+    capturing = torch.cuda.is_current_stream_capturing()
     if max_context_len < 0:
         raise ValueError("max_context_len must not be negative")
-    if max_context_len > 0 and torch.cuda.is_current_stream_capturing():
+    if capturing:
         max_context_len = 0
     if max_context_len > 0:
         width = min(width, (max_context_len + bs - 1) // bs)
@@ -1053,7 +1052,7 @@ def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_
     dev = k_cache.device
     stream = _raw_stream(dev.index)
     half = pages * nkv * bs * hd * 2
-    pool = torch.empty(2 * half + pages * nkv * 8, dtype=torch.uint8, device=dev)
+    pool = k_cache.new_empty(2 * half + pages * nkv * 8)         # elements of one byte
     k_pool = pool.data_ptr()
     v_pool, factors = k_pool + half, k_pool + 2 * half
     _lib.check(
@@ -1063,8 +1062,7 @@ def _widen_scaled_pages(k_cache, v_cache, k_scale, v_scale, page_table, cu_q, q_
             v_scale.data_ptr(), _cache_dtype(k_cache), page_table.data_ptr(), page_table.stride(0),
             width, cu_q.data_ptr(), q_start.data_ptr() if q_start is not None else 0,
             max_context_len, num_seqs, nkv, hd, bs, nb, stream))
-    table = _identity_table(dev, stream, num_seqs, width)
-    return pool, k_pool, v_pool, factors, table, pages
+    return pool, k_pool, v_pool, factors, _identity_table(dev, stream, pages, capturing), width, pages
 
 
 def read_error_word(device: Optional[torch.device] = None) -> int:
