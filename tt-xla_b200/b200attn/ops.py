@@ -466,7 +466,8 @@ def paged_write(
     Caches: int8 or float8_e4m3fn with `k_scale` / `v_scale` (fp32 [num_blocks, num_kv_heads], an
     element reads as code * scale), or bf16 without scales (`k_bounds` is then what the call is
     for).  A page whose first row is written starts afresh; one that goes on grows its scale by a
-    power of two when a new row needs it and re-rounds the rows that stay.  A NaN or infinity makes
+    power of two when a new row needs it and re-rounds the rows that stay: those before the first
+    new one (what lies behind the new rows counts as free).  A NaN or infinity makes
     the scale NaN, and with it everything read through the page.  `k_bounds` (bf16 [num_blocks,
     num_kv_heads, 2, head_size]) keeps the least and greatest key of each channel for
     `select_pages`.  The sequences of one call must write to different pages."""

@@ -25,7 +25,9 @@
 //     P' = 2^((s - m) + log2 vs - r), with a maximum r of its own (relative to m, so that scores of
 //     any size leave the scale its bits): the f16 weights are then at most 2^8 whatever the scales
 //     are, and a page's values keep 11 bits next to pages whose scale is far larger but whose
-//     weight is small.  The row sum uses 2^(s - m), in fp32, unrounded;
+//     weight is small.  Weights below 2^-14 of the largest a warp has seen lose bits, up to 2^-25 of
+//     it each: 2^-12 of the mean |v| over 8192 keys, a sixteenth of the result's own rounding.  The row
+//     sum uses 2^(s - m), in fp32, unrounded;
 //   * a tile is 128 tokens, 32 per warp in two halves of 16 that share one page (and its scales),
 //     one vote and one set of waits: with 8-bit keys the issue slots and the length of the chain
 //     load - widen - MMA - softmax - MMA bound a warp, not the bytes;
@@ -34,8 +36,9 @@
 //     fp32 sums hold without loss;
 //   * q is scaled by a power of two per head to at most 1 before it is rounded to f16.
 // Measured (head_size 128, 8 KV heads): 32 users of 32768 tokens 350 us, 6.1 TB/s, 0.94 of the
-// measured copy rate; 64 users of 1024 to 8192 tokens 110 us, 5.4 TB/s; one user of 32768 tokens
-// 26 us, of which the stream is 10: the rest is launch, first loads and the merge.
+// measured copy rate; 64 users of 1024 to 8192 tokens 110 us, 5.4 TB/s (138 us with
+// 16 query heads per KV head, whose fragments take more registers than there are); one user of 32768
+// tokens 26 us, of which the stream is 10: the rest is launch, first loads and the merge.
 #pragma once
 #include <cfloat>
 

@@ -9,10 +9,11 @@
 // (qmax 127 or 448, its reciprocal rounded to fp32):
 //   * a page whose first row is written starts afresh: scale = need;
 //   * a page that goes on keeps its scale while need <= scale, else the scale grows by the
-//     smallest power of two that is enough, 2^n, and the rows that stay are re-rounded to
-//     code * 2^-n.  Power-of-two steps make that exact for e4m3 (but for its subnormals), and for
-//     int8 bound what all re-roundings of a page together can cost by one step of the final scale,
-//     however often a page grows (steps s, s/2, s/4, ... add up to less than s);
+//     smallest power of two that is enough, 2^n, and the rows that stay (those before the first new
+//     one; what lies behind the new rows is dead) are re-rounded to code * 2^-n.  Power-of-two steps
+//     make that exact for e4m3 (but for its subnormals), and for int8 bound what all re-roundings of
+//     a page together can cost by one step of the final scale, however often a page grows (steps s,
+//     s/2, s/4, ... add up to less than s);
 //   * a NaN or an infinity cannot be held: the scale becomes NaN, so everything read through the
 //     page is NaN until it is started afresh, and the codes are 0.
 // code = round(x / scale), ties to even, of the 32-bit quotient, so the codes are reproducible.
@@ -23,9 +24,10 @@
 // Memory-bound: 2 bytes read and 1 written per element.  Grid (page of the batch, KV head, K / V),
 // 128 threads that hold a page's rows of one head in registers (16 elements each per pass), so the
 // rows are read once for both the maximum and the codes.
-// Measured: 8192 tokens of 8 heads of 128 (50 MB) 15.6 us in int8, 16.7 us in e4m3 (3.2 / 3.0 TB/s:
-// a round or two of CTAs, each a chain of offsets, rows, maximum and codes); one token for each of
-// 64 sequences 5.1 us, launch and the same chain.
+// Measured: 8192 tokens of 8 heads of 128 (50 MB) 15.7 us in int8 (16.7 with bounds), 16.9 us in e4m3
+// (3.2 / 3.0 TB/s: nearly two rounds of CTAs, each a chain of offsets, rows, maximum and codes during
+// which nothing of another page is loaded); in bf16 with bounds (68 MB) 14.2 us; one token for each
+// of 64 sequences 5.1 us in int8, 4.1 in bf16, launch and the same chain.
 #pragma once
 #include "kv_scatter.cuh"
 

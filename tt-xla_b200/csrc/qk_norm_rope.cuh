@@ -10,8 +10,9 @@
 // product would be off by up to 0.03 rad.
 //
 // HBM-bound: each row is read once and written once.  One CTA per token; a head is held by
-// HD / 8 neighbouring lanes (16 bytes each), so the sum of squares is a few shuffles and the
-// rotation partner is in the same thread or warp: no shared memory but the token's cos / sin row.
+// HD / 8 neighbouring lanes (eight elements each, in one or two accesses), so the sum of squares is a
+// few shuffles and the rotation partner is in the same thread or warp: no shared memory but the
+// token's cos / sin row.
 #pragma once
 #include "kv_scatter.cuh"
 
@@ -65,7 +66,8 @@ constexpr int kNrPrefetch = 3;   // head slices a thread loads before it needs t
 // 8192 tokens of 32 + 8 + 8 heads of 128, cache written: kNrSplit 48 us, kNrAdjacent 51 us,
 // kNrShuffle 57 us (its four 64-bit shuffles per thread and head; kNrSplit would need the rotated
 // part to be the whole head).  Floor 33 us (218 MB at the measured copy rate); what is left is
-// issue slots (packed fp32 took it from 54 us) and the cos / sin row that a CTA waits for once.
+// instructions (packed fp32 took it from 54 us; value heads, which only go to the cache, pass through
+// the norm too) and the cos / sin row that a CTA waits for once.
 enum NrLayout : int { kNrSplit = 0, kNrShuffle = 1, kNrAdjacent = 2 };
 
 template <int HD, int LAYOUT>
