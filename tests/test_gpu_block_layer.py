@@ -380,6 +380,31 @@ def test_layer_refusals():
         sparse._page_values(kv, tuple(kv))
 
 
+def test_a_captured_prefill_serves_longer_contexts_than_it_was_captured_with(clean_error_word):
+    """A bound on the contexts holds for the eager call only."""
+    from b200attn import ops
+
+    cache, table = _decode_setup("int8_block", 2, 400, 8)
+    cu = torch.tensor([0, 40, 70], dtype=torch.int32)
+    q = torch.randn(70, NQ, HD, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    start = torch.zeros(2, dtype=torch.int32).cuda()
+    cu_dev = cu.cuda()
+
+    def run(longest):
+        return ops.prefill(q, cache[0], cache[1], cu, page_table=table, q_start=start, cu_q=cu_dev,
+                           k_scale=cache[2], v_scale=cache[3], max_context_len=longest)
+
+    run(40)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(40)
+    for a, b in ((0, 0), (100, 7), (360, 370)):
+        start.copy_(torch.tensor([a, b], dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, run(max(a + 40, b + 30)))
+
+
 def test_prefills_of_two_threads_on_one_stream(clean_error_word):
     """Each attends over the pages it widened, whatever the other enqueues in between."""
     import threading
